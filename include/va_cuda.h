@@ -63,9 +63,10 @@ extern "C" {
 #define VA_PREC_TF32 2 /* tcgen05 kind::tf32 on the fp32 rows + exact rerank                 */
 #define VA_PREC_BF16 3 /* tcgen05 kind::f16 (bf16) + exact rerank                            */
 
-/* Row element types of a database. */
+/* Row element types of a database; VA_DTYPE_INT8 is a type of 4-bit matvec queries only. */
 #define VA_DTYPE_F32 0
 #define VA_DTYPE_BF16 1
+#define VA_DTYPE_INT8 2
 
 /* Selection modes (Metal4SelectionMode, TopKSelectionKernel.swift:23-29). */
 #define VA_SELECT_MIN 0
@@ -324,6 +325,53 @@ int va_minmax(va_context* ctx, const float* x, int64_t n, float* out_minmax);
 int va_sq_perdim_minmax(va_context* ctx, const float* x, int64_t n, int dim, float* out_min, float* out_max);
 
 /* ------------------------------------------------------------------------------------------ */
+/* 4-bit rows with group scales (no reference counterpart: the reference's int4 quantizer,       */
+/* DataTransformations.metal:226-306, has one scale per array and no product with the codes)     */
+/* ------------------------------------------------------------------------------------------ */
+/* Bytes of a row of dim 4-bit codes: element 2i in the low, 2i + 1 in the high nibble of byte i
+ * (two's complement, [-8, 7]), padded with zeros to a multiple of 16 bytes. */
+#define VA_INT4_ROW_BYTES(dim) ((((dim) + 31) / 32) * 16)
+/* Codes of the rows x[n x dim] (dtype VA_DTYPE_F32 or VA_DTYPE_BF16, row stride x_stride elements)
+ * in groups of 32, 64 or 128 columns (a last group may be shorter): codes [n x
+ * VA_INT4_ROW_BYTES(dim)], aligned to 16 bytes; scales [n x ceil(dim / group)] of scale_dtype (F32
+ * or BF16); zeros [the same] or NULL. A code c stands for scale * (c - zero). Without zeros
+ * (symmetric): scale = max(max |x| / 7, 1e-8), code = clamp(rint(x / scale), -8, 7). With zeros:
+ * lo = min(x, 0), hi = max(x, 0), scale = max((hi - lo) / 15, 1e-8), zero = clamp(rint(-8 - lo /
+ * scale), -8, 7), code = clamp(rint(x / scale + zero), -8, 7). The scale is rounded to its type
+ * before the codes are formed. Rows are expected to be finite. */
+int va_sq_quantize_int4_groups(va_context* ctx, const void* x, int dtype, int64_t n, int dim, int64_t x_stride,
+                               int group, int scale_dtype, uint8_t* codes, void* scales, int8_t* zeros);
+/* The fp32 values [n x dim] that the codes stand for. */
+int va_sq_dequantize_int4_groups(va_context* ctx, const uint8_t* codes, const void* scales, const int8_t* zeros,
+                                 int64_t n, int dim, int group, int scale_dtype, float* out);
+/* Scores of nq queries against the coded rows: out[q * out_stride + r] = sum_j x[q, j] *
+ * scale[r, g(j)] * (code[r, j] - zero[r, g(j)]), fp32, times x_scales[q] when given. Queries
+ * [nq x dim] are fp32 or bf16, or int8 codes (VA_DTYPE_INT8) whose scale per query is x_scales (fp32;
+ * NULL: 1), e.g. va_rms_norm_int8's rows. Products are exact (an fp32 query is used in full), sums
+ * are fp32 per group and over the groups, in a fixed order. Zero points lie in [-8, 7]. The codes are
+ * read once per pass of up to 32 bf16 / int8 or 8 fp32 queries (half of it above 2048 dimensions). No
+ * allocation and no wait: the call may be captured into a graph. */
+int va_int4_matvec(va_context* ctx, const void* x, int x_dtype, const float* x_scales, int nq, const uint8_t* codes,
+                   const void* scales, const int8_t* zeros, int64_t n, int dim, int group, int scale_dtype,
+                   float* out, int64_t out_stride);
+
+/* ------------------------------------------------------------------------------------------ */
+/* Root-mean-square norm with int8 codes (no reference counterpart; its L2 normalisation,        */
+/* L2Normalization.metal, makes fp32 rows)                                                     */
+/* ------------------------------------------------------------------------------------------ */
+/* Per row: h = x + residual (rounded to the type; h = x when residual is NULL), z = h * weight,
+ * a = max |z| over the row (group = 0) or over each group of 32, 64 or 128 columns, codes [rows x dim]
+ * = rint(127 z / a) and scales [rows x ceil(dim / group), or rows x 1] = a / (127 sqrt(mean(h^2) + eps)),
+ * so that code * scale = z / rms(h) to 8 bits. x, residual and weight [dim] are fp32 or bf16
+ * (dtype), x and residual with row strides in elements. residual_out (optional, [rows x dim]
+ * contiguous; may be x or residual itself when that is contiguous) receives h. Codes are those of
+ * exact arithmetic. A row or group of zeros has codes 0 and scale 0; a row whose sum of squares is not
+ * finite, and a group whose a is not, has codes 0 and scale NaN. One launch; may be captured. */
+int va_rms_norm_int8(va_context* ctx, const void* x, const void* residual, const void* weight, int64_t rows, int dim,
+                     int dtype, int64_t x_stride, int64_t residual_stride, float eps, int group, void* residual_out,
+                     int8_t* codes, float* scales);
+
+/* ------------------------------------------------------------------------------------------ */
 /* int8 scalar-quantized search                                                                */
 /* ------------------------------------------------------------------------------------------ */
 /* Resident int8 database: per-dimension codes of the fp32 rows[n x dim] (host or device), with
@@ -424,6 +472,32 @@ int va_ivf_search(va_context* ctx, const va_ivf* ivf, const float* queries, int6
  * reference call IVFSearchPipeline.search(queries:structure:k:). */
 int va_ivf_search_host(va_context* ctx, const va_ivf* ivf, const float* queries_host, int64_t nq, int k, int nprobe,
                        float* out_vals_host, uint32_t* out_ids_host);
+
+/* ------------------------------------------------------------------------------------------ */
+/* Softmax cross entropy against all rows of a table (no reference counterpart: LogSumExp.metal   */
+/* reduces logits that are already in memory)                                                  */
+/* ------------------------------------------------------------------------------------------ */
+/* hidden [tokens x dim] and table [rows x dim] are bf16 with row strides in elements (16-byte aligned
+ * rows: strides and dim are multiples of 8). Logits logit_scale * hidden_t . table_v are formed tile by
+ * tile and never kept. lse[t] = ln sum_v exp(logit), loss[t] = lse[t] - logit[t, labels[t]] (fp32). A label
+ * outside [0, rows) marks a token without loss: loss 0, no gradient, and its hidden row is not read into
+ * the table's gradient. Sums are fp32 in a fixed order. */
+/* Device bytes of scratch that a call of these sizes needs (backward: 0 or 1). */
+int va_softmax_xent_workspace(va_context* ctx, int64_t tokens, int64_t rows, int dim, int backward, size_t* bytes);
+/* workspace: device memory of at least the size above, aligned to 128 bytes, used until the call's work has
+ * run; NULL uses the context's scratch, which is refused while the stream is being captured
+ * (VA_ERR_UNSUPPORTED). Graphs that may run at the same time need a workspace each. */
+int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hidden_stride, const uint16_t* table,
+                            int64_t table_stride, const int64_t* labels, int64_t tokens, int64_t rows, int dim,
+                            float logit_scale, void* workspace, size_t workspace_bytes, float* loss, float* lse);
+/* Gradients of sum_t grad_loss[t] * loss[t] (grad_loss NULL: 1) with respect to hidden and table, bf16,
+ * contiguous [tokens x dim] and [rows x dim], both written whole; lse is the forward pass's. The logits are
+ * recomputed in chunks of table rows; their gradient is rounded to bf16 before it is multiplied
+ * with table and hidden. */
+int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hidden_stride, const uint16_t* table,
+                             int64_t table_stride, const int64_t* labels, const float* lse, const float* grad_loss,
+                             int64_t tokens, int64_t rows, int dim, float logit_scale, void* workspace,
+                             size_t workspace_bytes, uint16_t* grad_hidden, uint16_t* grad_table);
 
 /* ------------------------------------------------------------------------------------------ */
 /* Seeded synthetic data on the device (restates Tests/.../Utilities/TestRNG.swift:57-161;     */

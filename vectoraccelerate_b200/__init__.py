@@ -6,8 +6,8 @@ The compute lives in ``libva_cuda.so`` (hand-written CUDA for sm_100a behind the
 """
 
 from . import _ffi
-from ._ffi import (DTYPE_BF16, DTYPE_F32, INVALID_ID, METRIC_COSINE, METRIC_IP, METRIC_L2SQ, PREC_AUTO, PREC_BF16,
-                   PREC_FP32, PREC_TF32)
+from ._ffi import (DTYPE_BF16, DTYPE_F32, DTYPE_INT8, INVALID_ID, METRIC_COSINE, METRIC_IP, METRIC_L2SQ, PREC_AUTO,
+                   PREC_BF16, PREC_FP32, PREC_TF32)
 from .context import DeviceBuffer, GPUContext, Metal4Configuration, Metal4Context, nccl_unique_id
 from .errors import (BufferAllocationFailed, CollectiveFailed, ComputeFailed, InvalidInput, Timeout, Unsupported,
                      VectorError)
@@ -20,6 +20,8 @@ from .kernels import (BinaryDatabase, BinaryQuantizationKernel, CosineSimilarity
                       Metal4BinaryVector, Metal4FusedL2Config, Metal4FusedL2TopKResult, Metal4QuantizationResult,
                       ScalarQuantizationKernel, ShardedDatabase, TopKMergeKernel, TopKSelectionKernel,
                       WarpOptimizedSelectionKernel, knn_search_host)
+from .scoring import (Int4Database, Int4GroupQuantizationKernel, Int4MatVecKernel, Int4Rows, RMSNormInt8Kernel,
+                      SoftmaxCrossEntropyKernel)
 
 # Type aliases of the reference (VectorAccelerate.swift:265-296).
 L2Kernel = L2DistanceKernel

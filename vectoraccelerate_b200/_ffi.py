@@ -19,7 +19,7 @@ VA_OK = 0
 METRIC_L2SQ, METRIC_COSINE, METRIC_IP = 0, 1, 2
 IVF_INIT_KMEANSPP, IVF_INIT_GIVEN, IVF_INIT_RANDOM = 0, 1, 2
 PREC_AUTO, PREC_FP32, PREC_TF32, PREC_BF16 = 0, 1, 2, 3
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_INT8 = 0, 1, 2
 SELECT_MIN, SELECT_MAX = 0, 1
 MAX_DIM, MAX_K, MAX_SELECT_K = 4096, 1024, 4096
 NCCL_ID_BYTES = 128
@@ -107,6 +107,13 @@ SIGNATURES = {
     "va_ivf_list_sizes": [_P, _P],
     "va_ivf_search": [_P, _P, _P, _I64, _I, _I, _P, _P],
     "va_ivf_search_host": [_P, _P, _P, _I64, _I, _I, _P, _P],
+    "va_sq_quantize_int4_groups": [_P, _P, _I, _I64, _I, _I64, _I, _I, _P, _P, _P],
+    "va_sq_dequantize_int4_groups": [_P, _P, _P, _P, _I64, _I, _I, _I, _P],
+    "va_int4_matvec": [_P, _P, _I, _P, _I, _P, _P, _P, _I64, _I, _I, _I, _P, _I64],
+    "va_rms_norm_int8": [_P, _P, _P, _P, _I64, _I, _I, _I64, _I64, _F, _I, _P, _P, _P],
+    "va_softmax_xent_workspace": [_P, _I64, _I64, _I, _I, ctypes.POINTER(_SZ)],
+    "va_softmax_xent_forward": [_P, _P, _I64, _P, _I64, _P, _I64, _I64, _I, _F, _P, _SZ, _P, _P],
+    "va_softmax_xent_backward": [_P, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I, _F, _P, _SZ, _P, _P],
     "va_gen_gaussian": [_P, _P, _I64, _I, _U64, _I64],
     "va_gen_mixture": [_P, _P, _I64, _I, _U64, _I64, _I, _F, _I],
     "va_f32_to_bf16": [_P, _P, _I64, _P],

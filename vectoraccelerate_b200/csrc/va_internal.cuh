@@ -47,6 +47,26 @@ struct VaRange {
         if (!(cond)) return va_set_error(VA_ERR_INVALID_ARG, __VA_ARGS__); \
     } while (0)
 
+// Makes the context's device current for one call and puts the caller's back: a host program (or
+// another library in it) keeps its own current device.
+struct VaDeviceGuard {
+    explicit VaDeviceGuard(int device) {
+        err = cudaGetDevice(&prev);
+        if (err == cudaSuccess && prev != device) {
+            err = cudaSetDevice(device);
+            moved = err == cudaSuccess;
+        }
+    }
+    ~VaDeviceGuard() {
+        if (moved) cudaSetDevice(prev);
+    }
+    VaDeviceGuard(const VaDeviceGuard&) = delete;
+    VaDeviceGuard& operator=(const VaDeviceGuard&) = delete;
+    int prev = 0;
+    bool moved = false;
+    cudaError_t err = cudaSuccess;
+};
+
 // Device-side error codes written to the context's error word.
 #define VA_DEVERR_WAIT_TIMEOUT 1
 

@@ -1,0 +1,915 @@
+// va_xent.cu -- softmax cross entropy of tokens against all rows of a table, and its gradients, on the
+// tensor cores; the logits are never kept.
+//
+// tokens h [T x D], table w [V x D] (bf16), c = logit_scale:
+//   z_tv = c h_t . w_v        lse_t = ln sum_v exp z_tv        loss_t = lse_t - z_{t, label_t}
+//   G_tv = c g_t (exp(z_tv - lse_t) - [v = label_t])           dh = G w        dw = G^T h
+// with g_t the gradient of loss_t. A token whose label is outside [0, V) has no loss: loss 0, G row 0.
+//
+// Forward, 2TVD operations: k_xent_scores<FORWARD> walks 128-token x 256-row tiles (TMA ring, one
+// thread issuing tcgen05.mma, two TMEM accumulators) and its epilogue keeps each token's running
+// maximum and sum of exponentials (in powers of two) in registers; the partial pairs of the row splits
+// are joined by k_xent_join, which also forms the label's logit.
+// Backward, 6TVD: the table is taken in chunks of rows so that G of a chunk (bf16) is at most 256 MB.
+// k_xent_scores<GRADIENT> recomputes the chunk's logits and stores G; k_xent_grads multiplies it both
+// ways, with operands that are contiguous along the wrong axis read as MN-major tiles instead of being
+// transposed in memory: dw tiles (M = rows, K = tokens) are finished in one go; dh tiles (M = tokens, K = the
+// chunk's rows) add into an fp32 buffer per K split, which k_xent_finish sums and rounds.
+// Both directions are compute-bound once T and V pass a few hundred: the tensor pipe is the limit and
+// the exponentials (16 per clock and SM) hide behind it above D = 256.
+//
+// Roundings: G to bf16 once (its products with w and h are summed in fp32, so the error of a gradient
+// stays near that of its own rounding to bf16); everything else fp32. All orders of summation are fixed.
+#include <algorithm>
+#include <cmath>
+
+#include "va_tcgen05.cuh"
+
+namespace {
+
+using namespace va::tc;
+
+constexpr int BM = 128;                   // tile rows (TMEM lanes)
+constexpr int BN = 256;                   // columns of an accumulator
+constexpr int BK = 64;                    // elements of K per stage (128 bytes)
+constexpr int BOX = 64 * 128;             // bytes of a 64-row box of 128-byte rows
+constexpr int A_BYTES = 2 * BOX;
+constexpr int B_BYTES = 4 * BOX;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int STAGES = 4;
+constexpr int EPI_BYTES = 32 * 128;       // one staged 32-row x 128-byte piece of an epilogue warp
+constexpr int THREADS = 192;              // TMA warp, MMA warp, four epilogue warps
+constexpr int TMEM_COLS = 512;
+constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 4 * 2 * EPI_BYTES + (2 * STAGES + 5) * 8 + 16;
+constexpr int64_t G_ENTRIES = 1 << 27;    // gradient entries of a chunk (256 MB of bf16)
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+enum { FORWARD = 0, GRADIENT = 1 };
+
+// Per token of the backward pass: lse in powers of two, c * g (0: no loss) and the label.
+struct TokenGrad {
+    float lse2, scale;
+    int64_t label;
+};
+
+struct Roles {
+    uint8_t *sA, *sB, *sE;
+    uint64_t *full, *empty, *tfull, *tempty, *dbar;
+    volatile int* abort_flag;
+    uint32_t tmem;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// Instruction descriptor: fp32 accumulator, bf16 operands, M = 128, N columns; an operand is K-major (0)
+// or MN-major (1).
+__host__ __device__ constexpr uint32_t idesc_of(int n, int a_mn, int b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+
+// MN-major operand, 128B swizzle: boxes of 64 (MN) x 64 (K), 128 bytes per K row. Groups of 8 K rows are
+// 1024 B apart (SBO), neighbouring 64-element blocks of MN one box (LBO). A step of 16 along K is 2048 B.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(BOX >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
+                 "r"(smem_u32(src)), "r"(c0), "r"(c1)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_add_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
+                 "r"(smem_u32(src)), "r"(c0), "r"(c1)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// Shared set-up of the two kernels: barriers, TMEM.
+__device__ __forceinline__ Roles set_up(uint8_t* smem_raw) {
+    Roles r;
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    r.sA = smem;
+    r.sB = smem + (size_t)STAGES * A_BYTES;
+    r.sE = r.sB + (size_t)STAGES * B_BYTES;
+    r.full = (uint64_t*)(r.sE + 4 * 2 * EPI_BYTES);
+    r.empty = r.full + STAGES;
+    r.tfull = r.empty + STAGES;
+    r.tempty = r.tfull + 2;
+    r.dbar = r.tempty + 2;
+    uint32_t* s_tmem = (uint32_t*)(r.dbar + 1);
+    r.abort_flag = (volatile int*)(s_tmem + 1);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&r.full[s], 1);
+            mbar_init(&r.empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&r.tfull[b], 1);
+            mbar_init(&r.tempty[b], 4);
+        }
+        mbar_init(r.dbar, 1);
+        *r.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x >> 5 == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
+                     "r"(TMEM_COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    r.tmem = *s_tmem;
+    return r;
+}
+
+// Every role rejoins; TMEM is freed after the last read and the last MMA.
+__device__ __forceinline__ void tear_down(const Roles& r) {
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x >> 5 == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(r.tmem), "r"(TMEM_COLS));
+    }
+}
+
+// A ring position shared by the producer and the MMA issuer.
+struct Ring {
+    uint32_t it = 0;
+    __device__ __forceinline__ int slot() const { return (int)(it % STAGES); }
+    __device__ __forceinline__ uint32_t phase() const { return (it / STAGES) & 1u; }
+};
+
+// Waits for accumulator `tile`; the whole warp follows lane 0's verdict.
+__device__ __forceinline__ bool wait_accumulator(const Roles& r, uint32_t tile, int lane, int* err, uint64_t limit_ns) {
+    int ok = 1;
+    if (lane == 0) ok = mbar_wait(&r.tfull[tile & 1u], (tile >> 1) & 1u, r.abort_flag, err, limit_ns) ? 1 : 0;
+    ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+    tc_fence_after();
+    return ok != 0;
+}
+__device__ __forceinline__ void release_accumulator(const Roles& r, uint32_t tile, int lane) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&r.tempty[tile & 1u]);
+}
+
+// One lane's 128 bytes of a staged piece: row `lane` of 32, 16-byte units in the 128B swizzle order.
+__device__ __forceinline__ void stage_unit(uint8_t* piece, int lane, int unit, uint4 v) {
+    *reinterpret_cast<uint4*>(piece + lane * 128 + ((unit ^ (lane & 7)) << 4)) = v;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Logits: forward statistics, or the gradient of a chunk
+// ------------------------------------------------------------------------------------------------
+struct ScoreWork {
+    int64_t tokens, rows;  // rows: of this launch (the whole table, or one chunk), from row0
+    int64_t row0;
+    int token_tiles, row_tiles, splits, k_blocks;
+    float scale2;          // c * log2(e)
+    float2* part;          // forward: (maximum, sum) per [split][token_tiles * 128]
+    const TokenGrad* tok;  // gradient
+};
+
+__device__ __forceinline__ void score_item(const ScoreWork& w, int item, int& tt, int& split, int& r0, int& r1) {
+    split = item / w.token_tiles;
+    tt = item - split * w.token_tiles;
+    r0 = (int)((int64_t)w.row_tiles * split / w.splits);
+    r1 = (int)((int64_t)w.row_tiles * (split + 1) / w.splits);
+}
+
+// Running maximum and sum of 2^z over 64 columns of a row, z = acc * scale2; columns at or past
+// `valid` do not exist. The maximum is kept as nb = -max z (finite even while no logit was finite).
+__device__ __forceinline__ void lse_chunk(uint32_t (&r)[64], float scale2, int valid, float& top, float& nb, float& sum) {
+    if (valid < 64) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+            if (i >= valid) r[i] = 0xFF800000u;
+    }
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 64; ++i) m[i & 3] = fmaxf(m[i & 3], __uint_as_float(r[i]));
+    const float mx = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    if (mx > top) {
+        const float was = nb;
+        top = mx;
+        nb = -mx * scale2;
+        if (sum != 0.f) sum *= ex2(nb - was);
+    }
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 64; ++i) s[i & 3] += ex2(fmaf(__uint_as_float(r[i]), scale2, nb));
+    sum += (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// Gradient entries of 64 columns of a token, staged as 128 bytes of bf16. `label` is the label's
+// column in the chunk (outside [0, 64): not here).
+__device__ __forceinline__ void grad_chunk(const uint32_t (&r)[64], float scale2, float lse2, float scale, int label,
+                                           uint8_t* piece, int lane) {
+    const bool here = (unsigned)label < 64u;
+    const bool any = __any_sync(0xFFFFFFFFu, here);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        uint32_t p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float v[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int i = u * 8 + k * 2 + e;
+                // a token without loss has exact zeros, whatever its logits are
+                v[e] = scale == 0.f ? 0.f : ex2(fmaf(__uint_as_float(r[i]), scale2, -lse2)) * scale;
+                if (any && label == i) v[e] -= scale;
+            }
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[k]) : "f"(v[1]), "f"(v[0]));
+        }
+        stage_unit(piece, lane, u, make_uint4(p[0], p[1], p[2], p[3]));
+    }
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(THREADS, 1)
+    k_xent_scores(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
+                  const __grid_constant__ CUtensorMap map_g, ScoreWork w, int* err, uint64_t limit_ns) {
+    extern __shared__ uint8_t smem_raw[];
+    const Roles r = set_up(smem_raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_items = w.token_tiles * w.splits;
+    int tt, split, r0, r1;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            Ring ring;
+            for (int item = blockIdx.x; item < n_items && !*r.abort_flag; item += gridDim.x) {
+                score_item(w, item, tt, split, r0, r1);
+                for (int t = r0; t < r1; ++t)
+                    for (int kb = 0; kb < w.k_blocks; ++kb, ++ring.it) {
+                        const int s = ring.slot();
+                        if (!mbar_wait(&r.empty[s], ring.phase() ^ 1u, r.abort_flag, err, limit_ns)) goto loads_done;
+                        mbar_expect_tx(&r.full[s], STAGE_BYTES);
+                        tma_load_2d(r.sA + (size_t)s * A_BYTES, &map_h, &r.full[s], kb * BK, tt * BM);
+                        tma_load_2d(r.sB + (size_t)s * B_BYTES, &map_w, &r.full[s], kb * BK, (int)(w.row0 + (int64_t)t * BN));
+                    }
+            }
+        loads_done:
+            if (*r.abort_flag) drain_loads(r.full, STAGES, ring.it);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            Ring ring;
+            uint32_t tile = 0;
+            constexpr uint32_t idesc = idesc_of(BN, 0, 0);
+            for (int item = blockIdx.x; item < n_items && !*r.abort_flag; item += gridDim.x) {
+                score_item(w, item, tt, split, r0, r1);
+                for (int t = r0; t < r1; ++t, ++tile) {
+                    if (!mbar_wait(&r.tempty[tile & 1u], ((tile >> 1) & 1u) ^ 1u, r.abort_flag, err, limit_ns)) goto mma_done;
+                    tc_fence_after();
+                    const uint32_t d = r.tmem + (tile & 1u) * BN;
+                    for (int kb = 0; kb < w.k_blocks; ++kb, ++ring.it) {
+                        const int s = ring.slot();
+                        if (!mbar_wait(&r.full[s], ring.phase(), r.abort_flag, err, limit_ns)) goto mma_done;
+                        tc_fence_after();
+                        const uint32_t a0 = smem_u32(r.sA + (size_t)s * A_BYTES), b0 = smem_u32(r.sB + (size_t)s * B_BYTES);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            mma_f16(d, smem_desc(a0 + 32 * j), smem_desc(b0 + 32 * j), idesc, (kb | j) ? 1u : 0u);
+                        mma_commit(&r.empty[s]);
+                    }
+                    mma_commit(&r.tfull[tile & 1u]);
+                }
+            }
+        mma_done:
+            if (*r.abort_flag) {
+                mma_commit(r.dbar);
+                mbar_drain(r.dbar, 0u, kDrainLimitNs);
+            }
+        }
+    } else {
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        uint8_t* piece = r.sE + (size_t)quarter * 2 * EPI_BYTES;
+        uint32_t tile = 0;
+        for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+            score_item(w, item, tt, split, r0, r1);
+            const int64_t token = (int64_t)tt * BM + row;
+            float top = -INFINITY, nb = 0.f, sum = 0.f;
+            TokenGrad tg{0.f, 0.f, -1};
+            if constexpr (MODE == GRADIENT) {
+                if (token < w.tokens) tg = w.tok[token];
+            }
+            for (int t = r0; t < r1; ++t, ++tile) {
+                if (!wait_accumulator(r, tile, lane, err, limit_ns)) goto epilogue_done;
+                const uint32_t at = r.tmem + ((uint32_t)(quarter * 32) << 16) + (tile & 1u) * BN;
+                const int64_t col0 = (int64_t)t * BN;
+                const int valid = (int)min((int64_t)BN, w.rows - col0);
+                uint32_t ra[64], rb[64];
+                if constexpr (MODE == FORWARD) {
+                    tmem_ld64(at, ra);
+                    tmem_wait64(ra);
+                    tmem_ld64(at + 64, rb);
+                    lse_chunk(ra, w.scale2, valid, top, nb, sum);
+                    tmem_wait64(rb);
+                    tmem_ld64(at + 128, ra);
+                    lse_chunk(rb, w.scale2, valid - 64, top, nb, sum);
+                    tmem_wait64(ra);
+                    tmem_ld64(at + 192, rb);
+                    lse_chunk(ra, w.scale2, valid - 128, top, nb, sum);
+                    tmem_wait64(rb);
+                    release_accumulator(r, tile, lane);
+                    lse_chunk(rb, w.scale2, valid - 192, top, nb, sum);
+                } else {
+                    const int64_t lab = tg.label - w.row0 - col0;
+                    const int label = lab >= 0 && lab < BN ? (int)lab : -BN;
+                    const int64_t token0 = (int64_t)tt * BM + quarter * 32;
+                    auto put = [&](int c, const uint32_t(&v)[64]) {
+                        uint8_t* p = piece + (c & 1) * EPI_BYTES;
+                        // the store that last used this piece has read it
+                        if (lane == 0) bulk_wait_read<1>();
+                        __syncwarp();
+                        grad_chunk(v, w.scale2, tg.lse2, tg.scale, label - 64 * c, p, lane);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (token0 < w.tokens && col0 + 64 * c < w.rows) tma_store_2d(&map_g, p, (int)(col0 + 64 * c), (int)token0);
+                            bulk_commit();
+                        }
+                    };
+                    tmem_ld64(at, ra);
+                    tmem_wait64(ra);
+                    tmem_ld64(at + 64, rb);
+                    put(0, ra);
+                    tmem_wait64(rb);
+                    tmem_ld64(at + 128, ra);
+                    put(1, rb);
+                    tmem_wait64(ra);
+                    tmem_ld64(at + 192, rb);
+                    put(2, ra);
+                    tmem_wait64(rb);
+                    release_accumulator(r, tile, lane);
+                    put(3, rb);
+                }
+            }
+            if constexpr (MODE == FORWARD) w.part[(int64_t)split * w.token_tiles * BM + token] = make_float2(-nb, sum);
+        }
+    epilogue_done:
+        if (MODE == GRADIENT && lane == 0) bulk_wait_all();
+    }
+    tear_down(r);
+}
+
+// ------------------------------------------------------------------------------------------------
+// The two products of a chunk's G
+// ------------------------------------------------------------------------------------------------
+// Items: n_h = token_tiles * d_tiles * splits of dh (K = a split of the chunk's rows) and n_w = row_tiles *
+// d_tiles of dw (K = the tokens).
+struct GradWork {
+    int64_t row0;           // first table row of the chunk
+    int64_t rows;           // rows of the whole table
+    int dim;
+    int64_t tokens_pad;     // token_tiles * 128: rows of one split's dh buffer
+    int token_tiles, row_tiles, d_tiles, splits;
+    int n;                  // columns of a tile: 64, 128, 192 or 256
+    int kb_rows, kb_tokens; // K blocks of 64: chunk rows, tokens
+    int first;              // first chunk: dh is stored, else added
+    int long_h;             // dh items are the longer ones and go out first
+    int extra;              // shorter items given first to the blocks that got one longer item less
+};
+
+// The k-th item of this block, or -1. The longer items go round the blocks first; then `extra` shorter
+// ones to each block left with one longer item less (as many as make up for it), then the rest to all.
+__device__ __forceinline__ int grad_item(const GradWork& w, int k, bool& is_h) {
+    const int n_h = w.token_tiles * w.d_tiles * w.splits, n_w = w.row_tiles * w.d_tiles;
+    const int n_long = w.long_h ? n_h : n_w, n_short = w.long_h ? n_w : n_h;
+    const int grid = gridDim.x, b = blockIdx.x, over = n_long % grid;
+    const int longs = n_long / grid + (b < over ? 1 : 0);
+    if (k < longs) {
+        is_h = w.long_h;
+        return b + k * grid;
+    }
+    is_h = !w.long_h;
+    k -= longs;
+    const int late = over ? grid - over : 0;  // blocks with one longer item less
+    const int given = min(late * w.extra, n_short);
+    if (b >= over && late) {
+        const int j = (b - over) + k * late;
+        if (k < w.extra) {
+            if (j < given) return j;
+            return -1;  // the shorter items are used up
+        }
+        k -= w.extra;
+    }
+    const int64_t j = given + (int64_t)k * grid + (grid - 1 - b);
+    return j < n_short ? (int)j : -1;
+}
+
+struct GradTile {
+    int m, d, kb0, kb1, split;
+};
+__device__ __forceinline__ GradTile grad_tile(const GradWork& w, int item, bool is_h) {
+    GradTile t;
+    t.d = item % w.d_tiles;
+    const int rest = item / w.d_tiles;
+    if (is_h) {
+        t.m = rest % w.token_tiles;
+        t.split = rest / w.token_tiles;
+        t.kb0 = (int)((int64_t)w.kb_rows * t.split / w.splits);
+        t.kb1 = (int)((int64_t)w.kb_rows * (t.split + 1) / w.splits);
+    } else {
+        t.m = rest;
+        t.split = 0;
+        t.kb0 = 0;
+        t.kb1 = w.kb_tokens;
+    }
+    return t;
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+    k_xent_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_w,
+                 const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_dh,
+                 const __grid_constant__ CUtensorMap map_dw, GradWork w, int* err, uint64_t limit_ns) {
+    extern __shared__ uint8_t smem_raw[];
+    const Roles r = set_up(smem_raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int boxes = w.n / 64;
+    bool is_h;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            Ring ring;
+            for (int k = 0, item; (item = grad_item(w, k, is_h)) >= 0 && !*r.abort_flag; ++k) {
+                const GradTile t = grad_tile(w, item, is_h);
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++ring.it) {
+                    const int s = ring.slot();
+                    if (!mbar_wait(&r.empty[s], ring.phase() ^ 1u, r.abort_flag, err, limit_ns)) goto loads_done;
+                    mbar_expect_tx(&r.full[s], (2 + boxes) * BOX);
+                    uint8_t* a = r.sA + (size_t)s * A_BYTES;
+                    uint8_t* b = r.sB + (size_t)s * B_BYTES;
+                    if (is_h) {
+                        // A: 128 tokens x 64 chunk rows of G. B: 64 table rows x n columns.
+                        for (int i = 0; i < 2; ++i) tma_load_2d(a + i * BOX, &map_g, &r.full[s], kb * BK, t.m * BM + i * 64);
+                        for (int i = 0; i < boxes; ++i)
+                            tma_load_2d(b + i * BOX, &map_w, &r.full[s], t.d * w.n + i * 64, (int)(w.row0 + kb * BK));
+                    } else {
+                        // A: 64 tokens x 128 chunk rows of G. B: 64 tokens x n columns.
+                        for (int i = 0; i < 2; ++i) tma_load_2d(a + i * BOX, &map_g, &r.full[s], t.m * BM + i * 64, kb * BK);
+                        for (int i = 0; i < boxes; ++i)
+                            tma_load_2d(b + i * BOX, &map_h, &r.full[s], t.d * w.n + i * 64, kb * BK);
+                    }
+                }
+            }
+        loads_done:
+            if (*r.abort_flag) drain_loads(r.full, STAGES, ring.it);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            Ring ring;
+            uint32_t tile = 0;
+            for (int k = 0, item; (item = grad_item(w, k, is_h)) >= 0 && !*r.abort_flag; ++k) {
+                const GradTile t = grad_tile(w, item, is_h);
+                if (t.kb0 >= t.kb1) continue;
+                if (!mbar_wait(&r.tempty[tile & 1u], ((tile >> 1) & 1u) ^ 1u, r.abort_flag, err, limit_ns)) goto mma_done;
+                tc_fence_after();
+                const uint32_t d = r.tmem + (tile & 1u) * BN;
+                const uint32_t idesc = idesc_of(w.n, is_h ? 0 : 1, 1);
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++ring.it) {
+                    const int s = ring.slot();
+                    if (!mbar_wait(&r.full[s], ring.phase(), r.abort_flag, err, limit_ns)) goto mma_done;
+                    tc_fence_after();
+                    const uint32_t a0 = smem_u32(r.sA + (size_t)s * A_BYTES), b0 = smem_u32(r.sB + (size_t)s * B_BYTES);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mma_f16(d, is_h ? smem_desc(a0 + 32 * j) : smem_desc_mn(a0 + 2048 * j), smem_desc_mn(b0 + 2048 * j), idesc,
+                                (kb > t.kb0 || j) ? 1u : 0u);
+                    mma_commit(&r.empty[s]);
+                }
+                mma_commit(&r.tfull[tile & 1u]);
+                ++tile;
+            }
+        mma_done:
+            if (*r.abort_flag) {
+                mma_commit(r.dbar);
+                mbar_drain(r.dbar, 0u, kDrainLimitNs);
+            }
+        }
+    } else {
+        const int quarter = warp & 3;
+        uint8_t* piece = r.sE + (size_t)quarter * 2 * EPI_BYTES;
+        uint32_t tile = 0, pieces = 0;
+        bool both = false;  // the last store group read both pieces
+        for (int k = 0, item; (item = grad_item(w, k, is_h)) >= 0; ++k) {
+            const GradTile t = grad_tile(w, item, is_h);
+            if (t.kb0 >= t.kb1) continue;
+            if (!wait_accumulator(r, tile, lane, err, limit_ns)) break;
+            const uint32_t at = r.tmem + ((uint32_t)(quarter * 32) << 16) + (tile & 1u) * BN;
+            const int row = t.m * BM + quarter * 32;
+            for (int c = 0; c < boxes; ++c) {
+                uint32_t v[64];
+                tmem_ld64(at + 64 * c, v);
+                tmem_wait64(v);
+                if (c == boxes - 1) release_accumulator(r, tile, lane);
+                const int col = t.d * w.n + 64 * c;
+                if (is_h) {
+                    // Both pieces: 32 fp32 columns each.
+                    if (lane == 0) bulk_wait_read<0>();
+                    __syncwarp();
+                    both = true;
+#pragma unroll
+                    for (int u = 0; u < 16; ++u)
+                        stage_unit(piece + (u >> 3) * EPI_BYTES, lane, u & 7, make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]));
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        const int at_row = (int)(t.split * w.tokens_pad + row);
+                        for (int i = 0; i < 2; ++i) {
+                            if (col + 32 * i >= w.dim) break;
+                            if (w.first)
+                                tma_store_2d(&map_dh, piece + i * EPI_BYTES, col + 32 * i, at_row);
+                            else
+                                tma_add_2d(&map_dh, piece + i * EPI_BYTES, col + 32 * i, at_row);
+                        }
+                        bulk_commit();
+                    }
+                } else {
+                    uint8_t* p = piece + (pieces++ & 1u) * EPI_BYTES;
+                    if (lane == 0) {
+                        if (both)
+                            bulk_wait_read<0>();
+                        else
+                            bulk_wait_read<1>();
+                    }
+                    both = false;
+                    __syncwarp();
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        uint32_t b[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;"
+                                : "=r"(b[e])
+                                : "f"(__uint_as_float(v[u * 8 + 2 * e + 1])), "f"(__uint_as_float(v[u * 8 + 2 * e])));
+                        stage_unit(p, lane, u, make_uint4(b[0], b[1], b[2], b[3]));
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (col < w.dim && w.row0 + row < w.rows) tma_store_2d(&map_dw, p, col, (int)(w.row0 + row));
+                        bulk_commit();
+                    }
+                }
+            }
+            ++tile;
+        }
+        if (lane == 0) bulk_wait_all();
+    }
+    tear_down(r);
+}
+
+// ------------------------------------------------------------------------------------------------
+// The small kernels around them
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float dot8(uint4 a, uint4 b) {
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        s = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), s);
+        s = fmaf(__uint_as_float(x[i] & 0xFFFF0000u), __uint_as_float(y[i] & 0xFFFF0000u), s);
+    }
+    return s;
+}
+
+// One warp per token: joins the splits' (maximum, sum) pairs and forms the label's logit.
+__global__ void __launch_bounds__(128)
+    k_xent_join(const float2* __restrict__ part, int splits, int64_t pitch, const uint16_t* __restrict__ h,
+                int64_t h_stride, const uint16_t* __restrict__ table, int64_t w_stride, const int64_t* __restrict__ labels,
+                int64_t tokens, int64_t rows, int dim, float scale, float* __restrict__ loss, float* __restrict__ lse) {
+    const int lane = threadIdx.x & 31;
+    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (t >= tokens) return;
+    float top = -INFINITY, sum = 0.f;
+    for (int i = lane; i < splits; i += 32) {
+        const float2 p = part[i * pitch + t];
+        if (p.y == 0.f) continue;  // no finite logit there
+        const float m = fmaxf(top, p.x);
+        sum = (sum != 0.f ? sum * ex2(top - m) : 0.f) + p.y * ex2(p.x - m);
+        top = m;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const float ot = __shfl_xor_sync(0xFFFFFFFFu, top, o), os = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        const float m = fmaxf(top, ot);
+        sum = (sum != 0.f ? sum * ex2(top - m) : 0.f) + (os != 0.f ? os * ex2(ot - m) : 0.f);
+        top = m;
+    }
+    const int64_t label = labels[t];
+    const bool valid = label >= 0 && label < rows;
+    float dot = 0.f;
+    if (valid) {
+        const uint16_t* a = h + t * h_stride;
+        const uint16_t* b = table + label * w_stride;
+        for (int j = lane * 8; j < dim; j += 256)
+            dot += dot8(*reinterpret_cast<const uint4*>(a + j), *reinterpret_cast<const uint4*>(b + j));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+    if (lane == 0) {
+        const float l = sum != 0.f ? (top + log2f(sum)) * LN2 : -INFINITY;
+        lse[t] = l;
+        loss[t] = valid ? l - dot * scale : 0.f;
+    }
+}
+
+// One warp per token: what the backward pass needs of it, and its row of h with tokens without loss set to
+// zero (their rows may hold anything; 0 * NaN would reach the table's gradient).
+__global__ void __launch_bounds__(128)
+    k_xent_tokens(const uint16_t* __restrict__ h, int64_t h_stride, const int64_t* __restrict__ labels,
+                  const float* __restrict__ lse, const float* __restrict__ grad, int64_t tokens, int64_t rows, int dim,
+                  float scale, TokenGrad* __restrict__ tok, uint16_t* __restrict__ masked) {
+    const int lane = threadIdx.x & 31;
+    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (t >= tokens) return;
+    const int64_t label = labels[t];
+    const float g = label >= 0 && label < rows ? scale * (grad ? grad[t] : 1.f) : 0.f;
+    if (lane == 0) tok[t] = TokenGrad{lse[t] * LOG2E, g, g != 0.f ? label : -1};
+    for (int j = lane * 8; j < dim; j += 256)
+        *reinterpret_cast<uint4*>(masked + t * dim + j) =
+            g != 0.f ? *reinterpret_cast<const uint4*>(h + t * h_stride + j) : make_uint4(0u, 0u, 0u, 0u);
+}
+
+// Sums the K splits of dh in order and rounds.
+__global__ void __launch_bounds__(256) k_xent_finish(const float4* __restrict__ part, int splits, int64_t pitch, int64_t n,
+                                                     uint2* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        float4 v = part[i];
+        for (int s = 1; s < splits; ++s) {
+            const float4 u = part[i + s * pitch];
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        out[i] = make_uint2(va::f2bf_rn(v.x) | ((uint32_t)va::f2bf_rn(v.y) << 16),
+                            va::f2bf_rn(v.z) | ((uint32_t)va::f2bf_rn(v.w) << 16));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Host
+// ------------------------------------------------------------------------------------------------
+int make_map(CUtensorMap* map, const void* base, bool f32, int64_t cols, int64_t rows, int64_t pitch, int box_cols, int box_rows) {
+    const auto enc = get_encode_fn();
+    if (!enc) return va_set_error(VA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(pitch * (f32 ? 4 : 2))};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult r = enc(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                           const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return va_set_error(VA_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+    return VA_OK;
+}
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+struct ForwardPlan {
+    int token_tiles, row_tiles, splits;
+    size_t bytes;
+};
+
+ForwardPlan plan_forward(int sms, int64_t tokens, int64_t rows) {
+    ForwardPlan p;
+    p.token_tiles = (int)((tokens + BM - 1) / BM);
+    p.row_tiles = (int)((rows + BN - 1) / BN);
+    // Row splits: rounds of the grid x (tiles of an item + half a tile for its start and end).
+    double best = 0;
+    p.splits = 1;
+    for (int sp = 1; sp <= std::min(sms, p.row_tiles); ++sp) {
+        const double cost = (double)(((int64_t)p.token_tiles * sp + sms - 1) / sms) * ((p.row_tiles + sp - 1) / sp + 0.5);
+        if (sp == 1 || cost < best) {
+            best = cost;
+            p.splits = sp;
+        }
+    }
+    p.bytes = (size_t)p.splits * p.token_tiles * BM * sizeof(float2);
+    return p;
+}
+
+struct BackwardPlan {
+    int64_t chunk;  // table rows per chunk (a multiple of 256)
+    int token_tiles, d_tiles, n, splits;
+    size_t off_h, off_dh, off_g, bytes;
+};
+
+BackwardPlan plan_backward(int sms, int64_t tokens, int64_t rows, int dim) {
+    BackwardPlan p;
+    p.token_tiles = (int)((tokens + BM - 1) / BM);
+    const int64_t most = std::max<int64_t>(BN, G_ENTRIES / tokens / BN * BN);
+    const int64_t chunks = (rows + most - 1) / most;
+    p.chunk = up((rows + chunks - 1) / chunks, BN);
+    p.d_tiles = (dim + BN - 1) / BN;
+    p.n = (int)up((dim + p.d_tiles - 1) / p.d_tiles, 64);
+    // K splits of dh: items of at most half a block's share of the chunk's work (or 8 K blocks), while
+    // the fp32 buffers stay within 64 MB.
+    const int64_t chunk_rows = std::min(p.chunk, rows), kb_rows = (chunk_rows + BK - 1) / BK, kb_tokens = (tokens + BK - 1) / BK;
+    const int64_t work = p.d_tiles * (p.token_tiles * kb_rows + (chunk_rows + BM - 1) / BM * kb_tokens);
+    const int64_t item = std::max<int64_t>(8, work / (2 * sms));
+    const int64_t room = std::max<int64_t>(1, ((int64_t)64 << 20) / (p.token_tiles * BM * (int64_t)dim * 4));
+    p.splits = (int)std::min(std::min((kb_rows + item - 1) / item, room), kb_rows);
+    p.off_h = (size_t)up(tokens * (int64_t)sizeof(TokenGrad), 1024);
+    p.off_dh = p.off_h + (size_t)up(tokens * dim * 2, 1024);
+    p.off_g = p.off_dh + (size_t)up((int64_t)p.splits * p.token_tiles * BM * dim * 4, 1024);
+    p.bytes = p.off_g + (size_t)(tokens * p.chunk * 2);
+    return p;
+}
+
+int check_sizes(int64_t tokens, int64_t rows, int dim) {
+    VA_REQUIRE(tokens >= 0 && tokens <= (1 << 24), "tokens must be in 0..16777216, got %lld", (long long)tokens);
+    VA_REQUIRE(rows > 0 && rows <= (1 << 28), "rows must be in 1..268435456, got %lld", (long long)rows);
+    VA_REQUIRE(dim > 0 && dim <= VA_MAX_DIM && dim % 8 == 0, "dimension must be a multiple of 8 in 8..%d, got %d", VA_MAX_DIM,
+               dim);
+    VA_REQUIRE((tokens + BM - 1) / BM * ((rows + BM - 1) / BM) <= (1 << 30), "%lld tokens x %lld rows is too large for one call",
+               (long long)tokens, (long long)rows);
+    return VA_OK;
+}
+
+int check_inputs(va_context* ctx, const void* h, int64_t h_stride, const void* table, int64_t table_stride, int64_t tokens,
+                 int64_t rows, int dim, float scale) {
+    VA_TRY(check_sizes(tokens, rows, dim));
+    VA_REQUIRE(h_stride >= dim && h_stride % 8 == 0 && h_stride < ((int64_t)1 << 36),
+               "hidden_stride must be a multiple of 8 and at least the dimension %d, got %lld", dim, (long long)h_stride);
+    VA_REQUIRE(table_stride >= dim && table_stride % 8 == 0 && table_stride < ((int64_t)1 << 36),
+               "table_stride must be a multiple of 8 and at least the dimension %d, got %lld", dim, (long long)table_stride);
+    VA_REQUIRE((((uintptr_t)h | (uintptr_t)table) & 15) == 0, "hidden and table must be aligned to 16 bytes");
+    VA_REQUIRE(scale > 0.f && scale < INFINITY, "logit_scale must be positive and finite, got %g", (double)scale);
+    return VA_OK;
+}
+
+// The caller's workspace, or the context's scratch (which may grow, so never inside a capture).
+int workspace_of(va_context* ctx, void* workspace, size_t have, size_t need, void** out) {
+    if (workspace) {
+        VA_REQUIRE(((uintptr_t)workspace & 127) == 0, "workspace must be aligned to 128 bytes");
+        VA_REQUIRE(have >= need, "workspace of %zu bytes is too small: %zu bytes are needed", have, need);
+        *out = workspace;
+        return VA_OK;
+    }
+    cudaStreamCaptureStatus status;
+    VA_CUDA_TRY(cudaStreamIsCapturing(ctx->stream, &status));
+    if (status != cudaStreamCaptureStatusNone)
+        return va_set_error(VA_ERR_UNSUPPORTED, "a captured call needs a workspace of its own (%zu bytes)", need);
+    return va_workspace(ctx, need, out);
+}
+
+template <int MODE>
+int launch_scores(va_context* ctx, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& g, const ScoreWork& work) {
+    VA_CUDA_TRY(cudaFuncSetAttribute(k_xent_scores<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+    const int grid = std::min(ctx->sm_count, work.token_tiles * work.splits);
+    k_xent_scores<MODE><<<grid, THREADS, SMEM, ctx->stream>>>(h, w, g, work, ctx->d_error, wait_limit_ns(ctx->timeout_ms));
+    return va_check_launch("k_xent_scores");
+}
+
+}  // namespace
+
+extern "C" {
+
+int va_softmax_xent_workspace(va_context* ctx, int64_t tokens, int64_t rows, int dim, int backward, size_t* bytes) {
+    VA_REQUIRE(ctx && bytes, "ctx and bytes must not be NULL");
+    VA_TRY(check_sizes(tokens, rows, dim));
+    *bytes = !tokens ? 0 : backward ? plan_backward(ctx->sm_count, tokens, rows, dim).bytes
+                                    : plan_forward(ctx->sm_count, tokens, rows).bytes;
+    return VA_OK;
+}
+
+int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hidden_stride, const uint16_t* table,
+                            int64_t table_stride, const int64_t* labels, int64_t tokens, int64_t rows, int dim,
+                            float logit_scale, void* workspace, size_t workspace_bytes, float* loss, float* lse) {
+    VA_REQUIRE(ctx && (!tokens || (hidden && table && labels && loss && lse)),
+               "ctx, hidden, table, labels, loss and lse must not be NULL");
+    VA_TRY(check_inputs(ctx, hidden, hidden_stride, table, table_stride, tokens, rows, dim, logit_scale));
+    if (!tokens) return VA_OK;
+    VaDeviceGuard on(ctx->device);
+    VA_CUDA_TRY(on.err);
+    const ForwardPlan p = plan_forward(ctx->sm_count, tokens, rows);
+    void* ws;
+    VA_TRY(workspace_of(ctx, workspace, workspace_bytes, p.bytes, &ws));
+    CUtensorMap mh, mw;
+    VA_TRY(make_map(&mh, hidden, false, dim, tokens, hidden_stride, BK, BM));
+    VA_TRY(make_map(&mw, table, false, dim, rows, table_stride, BK, BN));
+    ScoreWork w{};
+    w.tokens = tokens;
+    w.rows = rows;
+    w.token_tiles = p.token_tiles;
+    w.row_tiles = p.row_tiles;
+    w.splits = p.splits;
+    w.k_blocks = (dim + BK - 1) / BK;
+    w.scale2 = logit_scale * LOG2E;
+    w.part = static_cast<float2*>(ws);
+    VA_TRY(launch_scores<FORWARD>(ctx, mh, mw, mh, w));
+    k_xent_join<<<(unsigned)((tokens + 3) / 4), 128, 0, ctx->stream>>>(w.part, p.splits, (int64_t)p.token_tiles * BM, hidden,
+                                                                     hidden_stride, table, table_stride, labels, tokens, rows,
+                                                                     dim, logit_scale, loss, lse);
+    return va_check_launch("k_xent_join");
+}
+
+int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hidden_stride, const uint16_t* table,
+                             int64_t table_stride, const int64_t* labels, const float* lse, const float* grad_loss,
+                             int64_t tokens, int64_t rows, int dim, float logit_scale, void* workspace,
+                             size_t workspace_bytes, uint16_t* grad_hidden, uint16_t* grad_table) {
+    VA_REQUIRE(ctx && table && grad_table && (!tokens || (hidden && labels && lse && grad_hidden)),
+               "ctx, hidden, table, labels, lse, grad_hidden and grad_table must not be NULL");
+    VA_TRY(check_inputs(ctx, hidden, hidden_stride, table, table_stride, tokens, rows, dim, logit_scale));
+    VA_REQUIRE((((uintptr_t)grad_hidden | (uintptr_t)grad_table) & 15) == 0,
+               "grad_hidden and grad_table must be aligned to 16 bytes");
+    VaDeviceGuard on(ctx->device);
+    VA_CUDA_TRY(on.err);
+    if (!tokens) {
+        VA_CUDA_TRY(cudaMemsetAsync(grad_table, 0, (size_t)rows * dim * 2, ctx->stream));
+        return VA_OK;
+    }
+    const BackwardPlan p = plan_backward(ctx->sm_count, tokens, rows, dim);
+    void* ws;
+    VA_TRY(workspace_of(ctx, workspace, workspace_bytes, p.bytes, &ws));
+    TokenGrad* tok = static_cast<TokenGrad*>(ws);
+    uint16_t* masked = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_h);
+    float* dh = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_dh);
+    uint16_t* g = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_g);
+    k_xent_tokens<<<(unsigned)((tokens + 3) / 4), 128, 0, ctx->stream>>>(hidden, hidden_stride, labels, lse, grad_loss, tokens,
+                                                                       rows, dim, logit_scale, tok, masked);
+    VA_TRY(va_check_launch("k_xent_tokens"));
+    VA_CUDA_TRY(cudaFuncSetAttribute(k_xent_grads, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+
+    const int64_t tokens_pad = (int64_t)p.token_tiles * BM;
+    CUtensorMap mh, mw, mw64, mh64, mdh, mdw;
+    VA_TRY(make_map(&mh, masked, false, dim, tokens, dim, BK, BM));
+    VA_TRY(make_map(&mw, table, false, dim, rows, table_stride, BK, BN));
+    VA_TRY(make_map(&mh64, masked, false, dim, tokens, dim, 64, 64));
+    VA_TRY(make_map(&mw64, table, false, dim, rows, table_stride, 64, 64));
+    VA_TRY(make_map(&mdh, dh, true, dim, p.splits * tokens_pad, dim, 32, 32));
+    VA_TRY(make_map(&mdw, grad_table, false, dim, rows, dim, 64, 32));
+    for (int64_t row0 = 0; row0 < rows; row0 += p.chunk) {
+        const int64_t count = std::min(p.chunk, rows - row0);
+        CUtensorMap mg_out, mg;
+        VA_TRY(make_map(&mg_out, g, false, count, tokens, p.chunk, 64, 32));
+        VA_TRY(make_map(&mg, g, false, count, tokens, p.chunk, 64, 64));
+        ScoreWork s{};
+        s.tokens = tokens;
+        s.rows = count;
+        s.row0 = row0;
+        s.token_tiles = p.token_tiles;
+        s.row_tiles = s.splits = (int)((count + BN - 1) / BN);
+        s.k_blocks = (dim + BK - 1) / BK;
+        s.scale2 = logit_scale * LOG2E;
+        s.tok = tok;
+        VA_TRY(launch_scores<GRADIENT>(ctx, mh, mw, mg_out, s));
+
+        GradWork w{};
+        w.row0 = row0;
+        w.rows = rows;
+        w.dim = dim;
+        w.tokens_pad = tokens_pad;
+        w.token_tiles = p.token_tiles;
+        w.row_tiles = (int)((count + BM - 1) / BM);
+        w.d_tiles = p.d_tiles;
+        w.splits = p.splits;
+        w.n = p.n;
+        w.kb_rows = (int)((count + BK - 1) / BK);
+        w.kb_tokens = (int)((tokens + BK - 1) / BK);
+        w.first = row0 == 0;
+        const int items_h = p.token_tiles * p.d_tiles * p.splits, items_w = w.row_tiles * p.d_tiles;
+        const int grid = std::min(ctx->sm_count, items_h + items_w);
+        const double cost_h = (double)w.kb_rows / p.splits, cost_w = w.kb_tokens;
+        w.long_h = cost_h >= cost_w;
+        w.extra = (int)std::lround(std::max(cost_h, cost_w) / std::max(1.0, std::min(cost_h, cost_w)));
+        k_xent_grads<<<grid, THREADS, SMEM, ctx->stream>>>(mg, mw64, mh64, mdh, mdw, w, ctx->d_error,
+                                                           wait_limit_ns(ctx->timeout_ms));
+        VA_TRY(va_check_launch("k_xent_grads"));
+    }
+    const int64_t n4 = tokens * dim / 4;
+    k_xent_finish<<<(unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)ctx->sm_count * 8), 256, 0, ctx->stream>>>(
+        reinterpret_cast<const float4*>(dh), p.splits, tokens_pad * dim / 4, n4, reinterpret_cast<uint2*>(grad_hidden));
+    return va_check_launch("k_xent_finish");
+}
+
+}  // extern "C"

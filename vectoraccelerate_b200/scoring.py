@@ -1,0 +1,353 @@
+"""The scoring head of an embedding model over libva_cuda: the norm that makes its queries, 4-bit tables
+and their products with queries, and the loss that trains both sides.
+
+The reference has neither of them (its int4 quantizer has one scale per array, its LogSumExp and
+MatrixVector kernels work on fp32 data in memory); the classes follow the kernel classes of
+``kernels.py``: constructed from a context, ``encode...`` methods over device memory, and methods that
+take and return host arrays.
+
+Device arguments are a ``DeviceBuffer``, an integer device address, or an object with ``data_ptr()``
+(a torch tensor) on the context's device, laid out as documented. Work is enqueued on the context's
+stream: a caller that has arrays from another stream makes that stream the context's
+(``Metal4Configuration(stream=...)``) or orders the two.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import numpy as np
+
+from . import _ffi
+from .context import DeviceBuffer, GPUContext
+from .errors import InvalidInput
+from .kernels import MAXIMUM, Database, TopKSelectionKernel, _f32, _Kernel
+
+_ITEM = {_ffi.DTYPE_F32: 4, _ffi.DTYPE_BF16: 2, _ffi.DTYPE_INT8: 1}
+
+
+def _address(context: GPUContext, x, nbytes: int, name: str):
+    """Device address of an argument; what knows its own size, device or layout is checked."""
+    if x is None or isinstance(x, int):
+        return x
+    if isinstance(x, DeviceBuffer):
+        if x.context.device != context.device:
+            raise InvalidInput(f"{name} is on device {x.context.device}, the context on device {context.device}")
+        if x.nbytes < nbytes:
+            raise InvalidInput(f"{name} holds {x.nbytes} bytes, {nbytes} are needed")
+        return x.ptr
+    if not hasattr(x, "data_ptr"):
+        raise InvalidInput(f"{name} must be a DeviceBuffer, a device address or have data_ptr(), got {type(x).__name__}")
+    device = x.device
+    if device.type != "cuda" or device.index != context.device:
+        raise InvalidInput(f"{name} is on {device}, the context on cuda:{context.device}")
+    return x.data_ptr()
+
+
+def _dense(context: GPUContext, x, nbytes: int, name: str):
+    """``_address`` of an array that must be contiguous and large enough."""
+    if hasattr(x, "data_ptr"):
+        if not x.is_contiguous():
+            raise InvalidInput(f"{name} must be contiguous")
+        if x.numel() * x.element_size() < nbytes:
+            raise InvalidInput(f"{name} holds {x.numel() * x.element_size()} bytes, {nbytes} are needed")
+    return _address(context, x, nbytes, name)
+
+
+def _strided(context: GPUContext, x, rows: int, dim: int, stride: int, item: int, name: str):
+    """``_address`` of rows that lie ``stride`` elements apart."""
+    nbytes = ((rows - 1) * stride + dim) * item if rows > 0 else 0
+    if hasattr(x, "data_ptr"):
+        if x.element_size() != item:
+            raise InvalidInput(f"{name} has elements of {x.element_size()} bytes, {item} expected")
+        if x.dim() == 2 and rows > 0 and (x.shape[0] < rows or x.shape[1] < dim or x.stride(1) != 1
+                                          or (rows > 1 and x.stride(0) != stride)):
+            raise InvalidInput(f"{name} of shape {tuple(x.shape)} and strides {x.stride()} does not hold {rows} rows of "
+                               f"{dim} elements {stride} apart")
+    return _address(context, x, nbytes, name)
+
+
+def _to_bf16(a) -> np.ndarray:
+    """fp32 -> bf16 bit patterns (round to nearest even), for the host-array methods."""
+    u = np.ascontiguousarray(a, np.float32).view(np.uint32)
+    nan = (u & 0x7FFFFFFF) > 0x7F800000
+    r = ((u + np.uint32(0x7FFF) + ((u >> np.uint32(16)) & np.uint32(1))) >> np.uint32(16)).astype(np.uint16)
+    return np.where(nan, ((u >> np.uint32(16)) | np.uint32(0x40)).astype(np.uint16), r)
+
+
+def _from_bf16(b) -> np.ndarray:
+    return (np.ascontiguousarray(b, np.uint16).astype(np.uint32) << np.uint32(16)).view(np.float32)
+
+
+def int4_row_bytes(dimension: int) -> int:
+    """Bytes of a coded row (VA_INT4_ROW_BYTES)."""
+    return (dimension + 31) // 32 * 16
+
+
+class RMSNormInt8Kernel(_Kernel):
+    """Root-mean-square norm with the residual's addition and int8 codes with scales (va_rms_norm_int8)."""
+
+    def encode(self, x, weight, rows: int, dimension: int, codes, scales, residual=None, residual_out=None,
+               dtype: int = _ffi.DTYPE_BF16, epsilon: float = 1e-6, group: int = 0, x_stride: int | None = None,
+               residual_stride: int | None = None) -> None:
+        """codes [rows x dimension] int8 and scales [rows x groups] fp32 (one group per row when ``group`` is 0) of
+        h = x + residual; ``residual_out`` receives h. Strides in elements; the dimension by default."""
+        ctx = self.context
+        if dtype not in (_ffi.DTYPE_F32, _ffi.DTYPE_BF16):
+            raise InvalidInput(f"dtype must be DTYPE_F32 or DTYPE_BF16, got {dtype}")
+        item = _ITEM[dtype]
+        xs = dimension if x_stride is None else x_stride
+        rs = dimension if residual_stride is None else residual_stride
+        groups = -(-dimension // group) if group > 0 else 1
+        _ffi.call("va_rms_norm_int8", self._h, _strided(ctx, x, rows, dimension, xs, item, "x"),
+                  _strided(ctx, residual, rows, dimension, rs, item, "residual") if residual is not None else None,
+                  _dense(ctx, weight, dimension * item, "weight"), rows, dimension, dtype, xs, rs, epsilon, group,
+                  _dense(ctx, residual_out, rows * dimension * item, "residual_out") if residual_out is not None else None,
+                  _dense(ctx, codes, rows * dimension, "codes"), _dense(ctx, scales, rows * groups * 4, "scales"))
+
+    def compute(self, x, weight, residual=None, epsilon: float = 1e-6, group: int = 0):
+        """fp32 host arrays -> (codes int8 [rows, dim], scales [rows, groups], h [rows, dim])."""
+        a, w = _f32(x), np.ascontiguousarray(weight, np.float32)
+        rows, dim = a.shape
+        if w.shape != (dim,):
+            raise InvalidInput(f"weight must have {dim} elements, got shape {w.shape}")
+        ctx = self.context
+        r = None
+        if residual is not None:
+            r = _f32(residual)
+            if r.shape != a.shape:
+                raise InvalidInput(f"residual shape {r.shape} differs from {a.shape}")
+        groups = -(-dim // group) if group > 0 else 1
+        dx, dw = ctx.get_buffer_for(a), ctx.get_buffer_for(w)
+        dr = ctx.get_buffer_for(r) if r is not None else None
+        codes = ctx.get_buffer(rows * dim, np.int8, (rows, dim))
+        scales = ctx.get_buffer(4 * rows * groups, np.float32, (rows, groups))
+        self.encode(dx, dw, rows, dim, codes, scales, dr, dr, _ffi.DTYPE_F32, epsilon, group)
+        return codes.download(), scales.download(), dr.download() if dr is not None else a
+
+
+@dataclass
+class Int4Rows:
+    """4-bit rows in device memory: codes [n x int4_row_bytes(dim)], scales and zero points [n x groups]."""
+
+    codes: DeviceBuffer
+    scales: DeviceBuffer
+    zero_points: DeviceBuffer | None
+    n: int
+    dim: int
+    group: int
+    scale_dtype: int
+
+
+class Int4GroupQuantizationKernel(_Kernel):
+    """4-bit codes with a scale, and optionally a zero point, per group of 32, 64 or 128 columns
+    (va_sq_quantize_int4_groups; the codes' format is ScalarQuantizationKernel's)."""
+
+    def encode(self, x, rows: int, dimension: int, group: int, codes, scales, zero_points=None,
+               dtype: int = _ffi.DTYPE_F32, scale_dtype: int = _ffi.DTYPE_BF16, x_stride: int | None = None) -> None:
+        ctx = self.context
+        _check_types(dtype, scale_dtype, group, (_ffi.DTYPE_F32, _ffi.DTYPE_BF16))
+        stride = dimension if x_stride is None else x_stride
+        groups = -(-dimension // group)
+        _ffi.call("va_sq_quantize_int4_groups", self._h, _strided(ctx, x, rows, dimension, stride, _ITEM[dtype], "x"), dtype,
+                  rows, dimension, stride, group, scale_dtype,
+                  _dense(ctx, codes, rows * int4_row_bytes(dimension), "codes"),
+                  _dense(ctx, scales, rows * groups * _ITEM[scale_dtype], "scales"),
+                  _dense(ctx, zero_points, rows * groups, "zero_points") if zero_points is not None else None)
+
+    def quantize(self, rows, group: int = 64, type: str = "symmetric",  # noqa: A002
+                 scale_dtype: int = _ffi.DTYPE_BF16) -> Int4Rows:
+        """Codes of fp32 host rows."""
+        a = _f32(rows)
+        if a.size == 0:
+            raise InvalidInput("Empty input")
+        if type not in ("symmetric", "asymmetric"):
+            raise InvalidInput(f"type must be 'symmetric' or 'asymmetric', got {type!r}")
+        _check_types(_ffi.DTYPE_F32, scale_dtype, group, (_ffi.DTYPE_F32,))
+        n, dim = a.shape
+        groups = -(-dim // group)
+        ctx = self.context
+        codes = ctx.get_buffer(n * int4_row_bytes(dim), np.uint8, (n, int4_row_bytes(dim)))
+        scales = ctx.get_buffer(n * groups * _ITEM[scale_dtype],
+                                np.uint16 if scale_dtype == _ffi.DTYPE_BF16 else np.float32, (n, groups))
+        zeros = ctx.get_buffer(n * groups, np.int8, (n, groups)) if type == "asymmetric" else None
+        dx = ctx.get_buffer_for(a)
+        self.encode(dx, n, dim, group, codes, scales, zeros, _ffi.DTYPE_F32, scale_dtype)
+        ctx.synchronize()
+        return Int4Rows(codes, scales, zeros, n, dim, group, scale_dtype)
+
+    def dequantize(self, rows: Int4Rows) -> np.ndarray:
+        """The fp32 values that the codes stand for."""
+        ctx = self.context
+        out = ctx.get_buffer(4 * rows.n * rows.dim, np.float32, (rows.n, rows.dim))
+        _ffi.call("va_sq_dequantize_int4_groups", self._h, rows.codes.ptr, rows.scales.ptr,
+                  rows.zero_points.ptr if rows.zero_points else None, rows.n, rows.dim, rows.group, rows.scale_dtype, out.ptr)
+        return out.download()
+
+
+def _check_types(dtype: int, scale_dtype: int, group: int, dtypes) -> None:
+    if dtype not in dtypes:
+        raise InvalidInput(f"dtype must be one of {dtypes}, got {dtype}")
+    if scale_dtype not in (_ffi.DTYPE_F32, _ffi.DTYPE_BF16):
+        raise InvalidInput(f"scale_dtype must be DTYPE_F32 or DTYPE_BF16, got {scale_dtype}")
+    if group not in (32, 64, 128):
+        raise InvalidInput(f"group must be 32, 64 or 128, got {group}")
+
+
+class Int4MatVecKernel(_Kernel):
+    """Products of a few queries with 4-bit rows (va_int4_matvec): fp32 scores [queries x rows]."""
+
+    def encode(self, queries, num_queries: int, codes, scales, rows: int, dimension: int, group: int, out,
+               zero_points=None, query_dtype: int = _ffi.DTYPE_F32, query_scales=None,
+               scale_dtype: int = _ffi.DTYPE_BF16, out_stride: int | None = None) -> None:
+        """Queries [num_queries x dimension] contiguous, of ``query_dtype``; int8 queries take a scale each from
+        ``query_scales``."""
+        ctx = self.context
+        _check_types(query_dtype, scale_dtype, group, (_ffi.DTYPE_F32, _ffi.DTYPE_BF16, _ffi.DTYPE_INT8))
+        stride = rows if out_stride is None else out_stride
+        groups = -(-dimension // group)
+        _ffi.call("va_int4_matvec", self._h, _dense(ctx, queries, num_queries * dimension * _ITEM[query_dtype], "queries"),
+                  query_dtype,
+                  _dense(ctx, query_scales, num_queries * 4, "query_scales") if query_scales is not None else None,
+                  num_queries, _dense(ctx, codes, rows * int4_row_bytes(dimension), "codes"),
+                  _dense(ctx, scales, rows * groups * _ITEM[scale_dtype], "scales"),
+                  _dense(ctx, zero_points, rows * groups, "zero_points") if zero_points is not None else None,
+                  rows, dimension, group, scale_dtype, _strided(ctx, out, num_queries, rows, stride, 4, "out"), stride)
+
+    def compute(self, queries, table: Int4Rows) -> np.ndarray:
+        """fp32 host queries -> scores [queries, rows]."""
+        q = _f32(queries)
+        if q.shape[1] != table.dim:
+            raise InvalidInput(f"query dimension {q.shape[1]} != table dimension {table.dim}")
+        ctx = self.context
+        dq = ctx.get_buffer_for(q)
+        out = ctx.get_buffer(4 * q.shape[0] * table.n, np.float32, (q.shape[0], table.n))
+        self.encode(dq, q.shape[0], table.codes, table.scales, table.n, table.dim, table.group, out, table.zero_points,
+                    _ffi.DTYPE_F32, None, table.scale_dtype)
+        return out.download()
+
+
+class Int4Database:
+    """Resident 4-bit rows searched by inner product: scores of every row (Int4MatVecKernel), then the
+    k largest (TopKSelectionKernel), ids by (score, id). The fp32 rows are not kept."""
+
+    def __init__(self, context: GPUContext, rows, group: int = 64, type: str = "symmetric",  # noqa: A002
+                 scale_dtype: int = _ffi.DTYPE_BF16):
+        self.context = context
+        self.table = Int4GroupQuantizationKernel(context).quantize(rows, group, type, scale_dtype)
+        self.n, self.dim = self.table.n, self.table.dim
+        self._matvec, self._select = Int4MatVecKernel(context), TopKSelectionKernel(context)
+
+    def scores(self, queries) -> np.ndarray:
+        return self._matvec.compute(queries, self.table)
+
+    def search(self, queries, k: int, query_scales=None):
+        """-> (values [Q, k], ids [Q, k]). Queries are fp32, or int8 codes with a scale per query (the output of
+        RMSNormInt8Kernel)."""
+        int8 = query_scales is not None
+        q = np.ascontiguousarray(queries, np.int8 if int8 else np.float32)
+        if q.ndim == 1:
+            q = q[None, :]
+        if q.shape[1] != self.dim:
+            raise InvalidInput(f"query dimension {q.shape[1]} != database dimension {self.dim}")
+        if not 0 < k <= TopKSelectionKernel.maxK:
+            raise InvalidInput(f"K must be between 1 and {TopKSelectionKernel.maxK}")
+        ctx, t, nq = self.context, self.table, q.shape[0]
+        ds = None
+        if int8:
+            s = np.ascontiguousarray(query_scales, np.float32).ravel()
+            if s.shape != (nq,):
+                raise InvalidInput(f"query_scales must have one entry per query ({nq}), got {s.size}")
+            ds = ctx.get_buffer_for(s)
+        dq = ctx.get_buffer_for(q)
+        scores = ctx.get_buffer(4 * nq * self.n, np.float32, (nq, self.n))
+        self._matvec.encode(dq, nq, t.codes, t.scales, self.n, self.dim, t.group, scores, t.zero_points,
+                            _ffi.DTYPE_INT8 if int8 else _ffi.DTYPE_F32, ds, t.scale_dtype)
+        vals, ids = self._select.execute(scores, nq, self.n, k, MAXIMUM)
+        return vals.download(), ids.download()
+
+    def close(self) -> None:
+        for b in (self.table.codes, self.table.scales, self.table.zero_points):
+            if b is not None:
+                b.free()
+
+
+class SoftmaxCrossEntropyKernel(_Kernel):
+    """Softmax cross entropy of tokens against all rows of a table, logits never kept, with the gradients
+    of both sides (va_softmax_xent_forward / _backward). The table is bf16: device memory or a bf16
+    ``Database``."""
+
+    def workspace_bytes(self, tokens: int, rows: int, dimension: int, backward: bool) -> int:
+        n = ctypes.c_size_t()
+        _ffi.call("va_softmax_xent_workspace", self._h, tokens, rows, dimension, int(backward), ctypes.byref(n))
+        return n.value
+
+    def _table(self, table, rows: int, dimension: int, stride: int):
+        if isinstance(table, Database):
+            if table.context.device != self.context.device:
+                raise InvalidInput(f"table is on device {table.context.device}, the context on device {self.context.device}")
+            if table.dtype != _ffi.DTYPE_BF16 or table.dim != dimension or stride != dimension or table.n < rows:
+                raise InvalidInput(f"table must be a bf16 database of at least {rows} rows x {dimension}")
+            return table.rows_ptr()
+        return _strided(self.context, table, rows, dimension, stride, 2, "table")
+
+    def _workspace(self, workspace, tokens, rows, dimension, backward):
+        if workspace is None:
+            return None, 0
+        if isinstance(workspace, int):
+            return workspace, self.workspace_bytes(tokens, rows, dimension, backward)
+        nbytes = workspace.nbytes if isinstance(workspace, DeviceBuffer) else workspace.numel() * workspace.element_size()
+        return _dense(self.context, workspace, 0, "workspace"), nbytes
+
+    def encode_forward(self, hidden, table, labels, tokens: int, rows: int, dimension: int, loss, lse,
+                       logit_scale: float = 1.0, hidden_stride: int | None = None, table_stride: int | None = None,
+                       workspace=None) -> None:
+        """hidden [tokens x dimension], table [rows x dimension] bf16; labels int64 (outside [0, rows): no
+        loss); loss and lse [tokens] fp32. An integer ``workspace`` address must hold workspace_bytes()."""
+        ctx = self.context
+        hs = dimension if hidden_stride is None else hidden_stride
+        ts = dimension if table_stride is None else table_stride
+        ws, nbytes = self._workspace(workspace, tokens, rows, dimension, False)
+        _ffi.call("va_softmax_xent_forward", self._h, _strided(ctx, hidden, tokens, dimension, hs, 2, "hidden"), hs,
+                  self._table(table, rows, dimension, ts), ts, _dense(ctx, labels, tokens * 8, "labels"), tokens, rows,
+                  dimension, logit_scale, ws, nbytes, _dense(ctx, loss, tokens * 4, "loss"), _dense(ctx, lse, tokens * 4, "lse"))
+
+    def encode_backward(self, hidden, table, labels, lse, grad_loss, tokens: int, rows: int, dimension: int, grad_hidden,
+                        grad_table, logit_scale: float = 1.0, hidden_stride: int | None = None,
+                        table_stride: int | None = None, workspace=None) -> None:
+        """Gradients of sum(grad_loss * loss) (``grad_loss`` None: 1), bf16 and contiguous, written whole."""
+        ctx = self.context
+        hs = dimension if hidden_stride is None else hidden_stride
+        ts = dimension if table_stride is None else table_stride
+        ws, nbytes = self._workspace(workspace, tokens, rows, dimension, True)
+        _ffi.call("va_softmax_xent_backward", self._h, _strided(ctx, hidden, tokens, dimension, hs, 2, "hidden"), hs,
+                  self._table(table, rows, dimension, ts), ts, _dense(ctx, labels, tokens * 8, "labels"),
+                  _dense(ctx, lse, tokens * 4, "lse"),
+                  _dense(ctx, grad_loss, tokens * 4, "grad_loss") if grad_loss is not None else None, tokens, rows, dimension,
+                  logit_scale, ws, nbytes, _dense(ctx, grad_hidden, tokens * dimension * 2, "grad_hidden"),
+                  _dense(ctx, grad_table, rows * dimension * 2, "grad_table"))
+
+    def compute(self, hidden, table, labels, logit_scale: float = 1.0, grad_loss=None):
+        """Host arrays (hidden and table are rounded to bf16) -> (loss [T], lse [T], grad_hidden [T, D],
+        grad_table [V, D]), fp32."""
+        h, w = _to_bf16(_f32(hidden)), _to_bf16(_f32(table))
+        y = np.ascontiguousarray(labels, np.int64).ravel()
+        if h.shape[1] != w.shape[1]:
+            raise InvalidInput("Dimension mismatch in input vectors")
+        if y.shape != (h.shape[0],):
+            raise InvalidInput(f"labels must have one entry per token ({h.shape[0]}), got {y.size}")
+        t, v, d = h.shape[0], w.shape[0], h.shape[1]
+        ctx = self.context
+        dh, dw, dy = ctx.get_buffer_for(h), ctx.get_buffer_for(w), ctx.get_buffer_for(y)
+        loss, lse = ctx.get_buffer(4 * t, np.float32, (t,)), ctx.get_buffer(4 * t, np.float32, (t,))
+        gh, gw = ctx.get_buffer(2 * t * d, np.uint16, (t, d)), ctx.get_buffer(2 * v * d, np.uint16, (v, d))
+        dg = None
+        if grad_loss is not None:
+            g = np.ascontiguousarray(grad_loss, np.float32).ravel()
+            if g.shape != (t,):
+                raise InvalidInput(f"grad_loss must have one entry per token ({t}), got {g.size}")
+            dg = ctx.get_buffer_for(g)
+        self.encode_forward(dh, dw, dy, t, v, d, loss, lse, logit_scale)
+        self.encode_backward(dh, dw, dy, lse, dg, t, v, d, gh, gw, logit_scale)
+        return loss.download(), lse.download(), _from_bf16(gh.download()), _from_bf16(gw.download())
