@@ -349,7 +349,7 @@ int va_sq_dequantize_int4_groups(va_context* ctx, const uint8_t* codes, const vo
  * [nq x dim] are fp32 or bf16, or int8 codes (VA_DTYPE_INT8) whose scale per query is x_scales (fp32;
  * NULL: 1), e.g. va_rms_norm_int8's rows. Products are exact (an fp32 query is used in full), sums
  * are fp32 per group and over the groups, in a fixed order. Zero points lie in [-8, 7]. The codes are
- * read once per pass of up to 32 bf16 / int8 or 8 fp32 queries (half of it above 2048 dimensions). No
+ * read once per pass of up to 32 bf16 / int8 or 8 fp32 queries (8 and 2 above 2048 dimensions). No
  * allocation and no wait: the call may be captured into a graph. */
 int va_int4_matvec(va_context* ctx, const void* x, int x_dtype, const float* x_scales, int nq, const uint8_t* codes,
                    const void* scales, const int8_t* zeros, int64_t n, int dim, int group, int scale_dtype,
@@ -365,7 +365,7 @@ int va_int4_matvec(va_context* ctx, const void* x, int x_dtype, const float* x_s
  * so that code * scale = z / rms(h) to 8 bits. x, residual and weight [dim] are fp32 or bf16
  * (dtype), x and residual with row strides in elements. residual_out (optional, [rows x dim]
  * contiguous; may be x or residual itself when that is contiguous) receives h. Codes are those of
- * exact arithmetic. A row or group of zeros has codes 0 and scale 0; a row whose sum of squares is not
+ * exact arithmetic (for a < 2^119). A row or group with a < 2^-80 has codes 0 and scale 0; a row whose sum of squares is not
  * finite, and a group whose a is not, has codes 0 and scale NaN. One launch; may be captured. */
 int va_rms_norm_int8(va_context* ctx, const void* x, const void* residual, const void* weight, int64_t rows, int dim,
                      int dtype, int64_t x_stride, int64_t residual_stride, float eps, int group, void* residual_out,

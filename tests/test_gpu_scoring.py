@@ -129,10 +129,22 @@ def test_norm_codes_at_borders(tctx):
     for row in range(3):
         codes, _, _ = run_norm(tctx, x[row:row + 1].contiguous(), w, None, "f32", 0)
         assert torch.equal(codes.double(), norm_reference(x[row:row + 1], w, 1e-6, 0)[0])
-    tiny = torch.full((1, 64), 1e-41, device="cuda")  # 127 / a overflows fp32
-    tiny[0, 3] = 3e-41
-    codes, _, _ = run_norm(tctx, tiny, torch.ones(64, device="cuda"), None, "f32", 0)
-    assert torch.equal(codes.double(), norm_reference(tiny, torch.ones(64, device="cuda"), 1e-6, 0)[0])
+    tiny = torch.full((2, 64), 2.0 ** -81, device="cuda")  # below 2^-80: counts as zero
+    tiny[1, 3] = 2.0 ** -80
+    codes, scales, _ = run_norm(tctx, tiny, torch.ones(64, device="cuda"), None, "f32", 0)
+    assert (codes[0] == 0).all() and scales[0, 0] == 0
+    assert torch.equal(codes[1].double(), norm_reference(tiny[1:], torch.ones(64, device="cuda"), 1e-6, 0)[0][0]) and scales[1, 0] > 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_norm_many_borders(tctx, dtype):
+    # few distinct values, so that quotients fall on and next to the borders between codes all the time
+    g = gen(8)
+    x = (torch.randint(-255, 256, (2000, 1024), generator=g, device="cuda") / 8).to(DT[dtype])
+    w = (torch.randint(1, 5, (1024,), generator=g, device="cuda") * (1.0 if dtype == "bf16" else 1.0 / 3)).to(DT[dtype])
+    for group in (0, 32):
+        codes, _, _ = run_norm(tctx, x, w, None, dtype, group)
+        assert torch.equal(codes.double(), norm_reference(x, w, 1e-6, group)[0])
 
 
 def test_norm_no_rows(tctx):

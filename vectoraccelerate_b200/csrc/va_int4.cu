@@ -30,7 +30,6 @@ namespace {
 
 using namespace va::tc;
 
-constexpr int WARPS = 8;           // warps per block
 constexpr int TR = 32;             // rows per warp tile
 constexpr int CHUNK = 256;         // codes per ring slot and row (128 bytes)
 constexpr int SLOT = TR * 128;     // bytes of a ring slot
@@ -43,7 +42,7 @@ struct MatvecArgs {
     const float* x_scales;
     float* out;
     int64_t n, out_stride;
-    int64_t row_tiles;
+    int row_tiles;
     int dim, group, groups, nq, x_dtype;
     int chunks;  // 256-code chunks per row
     int wk;      // warps sharing a row tile
@@ -105,8 +104,31 @@ __device__ __forceinline__ float scale_of(const S* p) {
         return __ldg(p);
 }
 
+// The scales (and 136 + zero point, as bf16 bits) that a lane holds of one chunk: of its four rows, groups t and
+// t + 4 of the chunk.
+template <typename S, bool ZERO, int GROUP>
+struct ChunkScales {
+    static constexpr int GPC = CHUNK / GROUP;           // groups per chunk
+    static constexpr int SPL = GPC > 4 ? GPC / 4 : 1;   // held per lane and row
+    float sc[4][SPL];
+    uint32_t zp[ZERO ? 4 : 1][ZERO ? SPL : 1];
+    __device__ __forceinline__ void load(const MatvecArgs& a, int64_t row0, int c, int g, int t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            // rows past the end repeat the last one: they are not stored
+            const int64_t base = min(row0 + g + 8 * r, a.n - 1) * a.groups;
+#pragma unroll
+            for (int p = 0; p < SPL; ++p) {
+                const int gi = min(c * GPC + (t & (GPC - 1)) + 4 * p, a.groups - 1);
+                sc[r][p] = scale_of(static_cast<const S*>(a.scales) + base + gi);
+                if constexpr (ZERO) zp[r][p] = 0x4308u + (uint32_t)(int)__ldg(a.zeros + base + gi);
+            }
+        }
+    }
+};
+
 // NT column tiles of 8; S = scale type (uint16_t: bf16); GROUP = 32, 64, 128.
-template <int NT, typename S, bool ZERO, int GROUP>
+template <int NT, int WARPS, typename S, bool ZERO, int GROUP>
 __global__ void __launch_bounds__(WARPS * 32, 1)
     k_int4_matvec(const __grid_constant__ CUtensorMap codes, MatvecArgs a, int* err, uint64_t limit_ns) {
     extern __shared__ uint8_t smem_raw[];
@@ -122,10 +144,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 
     const int teams = WARPS / a.wk, team = warp / a.wk, part = warp % a.wk;
     // Row tiles go round the blocks first, so that few tiles spread over all SMs.
-    const int64_t first = (int64_t)team * gridDim.x + blockIdx.x, step = (int64_t)gridDim.x * teams;
+    const int first = team * (int)gridDim.x + (int)blockIdx.x, step = (int)gridDim.x * teams;
     const int mine = (a.chunks - part + a.wk - 1) / a.wk;  // chunks of this warp per row tile
-    const int64_t tiles = first < a.row_tiles ? (a.row_tiles - first + step - 1) / step : 0;
-    const int64_t total = tiles * mine;
+    const int tiles = first < a.row_tiles ? (a.row_tiles - first + step - 1) / step : 0;
 
     if (lane == 0) {
         for (int s = 0; s < a.ring; ++s) mbar_init(&full[s], 1);
@@ -133,14 +154,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
     if (threadIdx.x == 0) *s_abort = 0;
     __syncwarp();
-    // Position of the next load to issue: row tile and chunk.
-    int64_t issue_tile = first, issued = 0;
-    int issue_chunk = part;
-    auto issue = [&]() {
-        const int s = (int)(issued % a.ring);
+    // Position of the next load to issue (lane 0): slot, row tile and chunk.
+    int64_t left = (int64_t)tiles * mine;
+    uint32_t issued = 0;  // counted to the ring's length only
+    int issue_tile = first, issue_chunk = part;
+    auto issue = [&](int s) {
         mbar_expect_tx(&full[s], SLOT);
-        tma_load_2d(ring + (size_t)s * SLOT, &codes, &full[s], issue_chunk * 128, (int)(issue_tile * TR));
-        ++issued;
+        tma_load_2d(ring + (size_t)s * SLOT, &codes, &full[s], issue_chunk * 128, issue_tile * TR);
+        --left;
         issue_chunk += a.wk;
         if (issue_chunk >= a.chunks) {
             issue_chunk = part;
@@ -148,7 +169,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         }
     };
     if (lane == 0)
-        while (issued < a.ring && issued < total) issue();
+        for (; issued < (uint32_t)a.ring && left > 0; ++issued) issue((int)issued);
+    using Scales = ChunkScales<S, ZERO, GROUP>;
+    Scales next;
+    if (tiles > 0) next.load(a, (int64_t)first * TR, part, g, t);
 
     // Query fragments. k16 step i of a chunk: half i & 1 of 32-code block i >> 1. Lane (g, t) reads word
     // t of the block, whose nibbles 0..7 are elements 8t..8t+7; half h pairs the nibbles (2h, 2h + 4) and
@@ -163,13 +187,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
     __syncthreads();
 
-    constexpr int GPC = CHUNK / GROUP;          // groups per chunk
-    constexpr int SPL = GPC > 4 ? GPC / 4 : 1;  // scales held per lane and row
-    const S* scales = static_cast<const S*>(a.scales);
+    const uint32_t slot0 = smem_u32(ring) + g * 128 + t * 4;
     bool dead = false;
-    int64_t it = 0;
-    for (int64_t k = 0; k < tiles; ++k) {
-        const int64_t tile = first + k * step, row0 = tile * TR;
+    int s = 0;
+    uint32_t phase = 0;
+    for (int k = 0; k < tiles; ++k) {
+        const int tile = first + k * step;
+        const int64_t row0 = (int64_t)tile * TR;
         float acc[NT][2][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -177,36 +201,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[n][m][i] = 0.f;
-        // Rows g, g + 8, g + 16, g + 24 of the tile (clamped: rows past the end are not stored).
-        int64_t base[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) base[r] = min(row0 + g + 8 * r, a.n - 1) * a.groups;
-        for (int c = part; c < a.chunks; c += a.wk, ++it) {
-            // Lane t holds the scales of groups t (and t + 4) of the chunk for its four rows.
-            float sc[4][SPL];
-            uint32_t zp[4][SPL];
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int p = 0; p < SPL; ++p) {
-                    const int gi = min(c * GPC + (t & (GPC - 1)) + 4 * p, a.groups - 1);
-                    sc[r][p] = scale_of(scales + base[r] + gi);
-                    if constexpr (ZERO) zp[r][p] = 0x4308u + (uint32_t)(int)__ldg(a.zeros + base[r] + gi);
-                }
-            const int s = (int)(it % a.ring);
-            if (!dead) {
-                int ok = 1;
-                if (lane == 0) ok = mbar_wait(&full[s], (uint32_t)((it / a.ring) & 1), s_abort, err, limit_ns) ? 1 : 0;
-                dead = !__shfl_sync(0xFFFFFFFFu, ok, 0);
-                // every lane observes the phase itself: the copy's bytes are visible to it
-                if (!dead) dead = !mbar_try_wait(&full[s], (uint32_t)((it / a.ring) & 1));
-                dead = __any_sync(0xFFFFFFFFu, dead);
-            }
+        for (int c = part; c < a.chunks; c += a.wk) {
+            // The next chunk's scales are on their way while this one is multiplied.
+            const Scales now = next;
+            const bool last = c + a.wk >= a.chunks;
+            if (!last || k + 1 < tiles) next.load(a, last ? row0 + (int64_t)step * TR : row0, last ? part : c + a.wk, g, t);
+            // Every lane waits: the phase it has seen is what makes the copy's bytes visible to it.
+            if (!dead) dead = __any_sync(0xFFFFFFFFu, !mbar_wait(&full[s], phase, s_abort, err, limit_ns));
             if (dead) break;
-            const uint32_t slot = smem_u32(ring + (size_t)s * SLOT) + g * 128;
+            const uint32_t slot = slot0 + s * SLOT;
             const uint2* fr = frag + (size_t)c * 16 * NT * 32 + lane;
 #pragma unroll
-            for (int gi = 0; gi < GPC; ++gi) {
+            for (int gi = 0; gi < Scales::GPC; ++gi) {
                 float grp[NT][2][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -218,9 +224,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 uint32_t bias[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    gs[r] = __shfl_sync(0xFFFFFFFFu, sc[r][gi >> 2 < SPL ? gi >> 2 : 0], (lane & ~3) | (gi & 3));
+                    const int from = (lane & ~3) | (gi & 3);
+                    gs[r] = __shfl_sync(0xFFFFFFFFu, now.sc[r][Scales::SPL > 1 ? gi >> 2 : 0], from);
                     if constexpr (ZERO) {
-                        const uint32_t z = __shfl_sync(0xFFFFFFFFu, zp[r][gi >> 2 < SPL ? gi >> 2 : 0], (lane & ~3) | (gi & 3));
+                        const uint32_t z = __shfl_sync(0xFFFFFFFFu, now.zp[r][Scales::SPL > 1 ? gi >> 2 : 0], from);
                         bias[r] = z | (z << 16);  // 136 + zero point, exact in bf16
                     } else {
                         bias[r] = 0x43084308u;  // 136
@@ -231,7 +238,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                     const int blk = gi * (GROUP / 32) + b;
                     uint32_t w[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) w[r] = lds32(slot + r * 1024 + ((blk ^ g) << 4) + t * 4);
+                    for (int r = 0; r < 4; ++r) w[r] = lds32(slot + r * 1024 + ((blk ^ g) << 4));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t f[2][4];
@@ -258,7 +265,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                         for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(gs[2 * m + (i >> 1)], grp[n][m][i], acc[n][m][i]);
             }
             __syncwarp();  // the slot is free: every lane has read it
-            if (lane == 0 && issued < total) issue();
+            if (lane == 0 && left > 0) issue(s);
+            if (++s == a.ring) {
+                s = 0;
+                phase ^= 1u;
+            }
         }
         if (a.wk > 1) {
             // Partial sums of the team's other warps, added in warp order.
@@ -311,15 +322,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                     }
         }
     }
-    // After an expired wait: copies still in flight write this block's shared memory.
-    if (dead && lane == 0) drain_loads(full, a.ring, (uint32_t)issued);
+    // After an expired wait: copies still in flight write this block's shared memory. Of slot i the last
+    // copy issued completes phase `phase` (slots from s on) or the next one (slots already reissued).
+    if (dead && lane == 0)
+        for (int i = 0; i < a.ring && i < (int)issued; ++i)
+            mbar_drain(&full[i], i >= s ? phase : phase ^ 1u, kDrainLimitNs);
 }
+
+// Warps per block: what the registers allow (128 a thread at 16 warps).
+constexpr int warps_of(int nt) { return nt == 4 ? 8 : 16; }
 
 template <int NT, typename S, bool ZERO, int GROUP>
 int launch_matvec(va_context* ctx, const CUtensorMap& codes, const MatvecArgs& a, int grid, size_t smem) {
-    auto kern = k_int4_matvec<NT, S, ZERO, GROUP>;
+    auto kern = k_int4_matvec<NT, warps_of(NT), S, ZERO, GROUP>;
     VA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kern<<<grid, WARPS * 32, smem, ctx->stream>>>(codes, a, ctx->d_error, wait_limit_ns(ctx->timeout_ms));
+    kern<<<grid, warps_of(NT) * 32, smem, ctx->stream>>>(codes, a, ctx->d_error, wait_limit_ns(ctx->timeout_ms));
     return va_check_launch("k_int4_matvec");
 }
 
@@ -515,29 +532,30 @@ int va_int4_matvec(va_context* ctx, const void* x, int x_dtype, const float* x_s
     a.zeros = zeros;
     a.n = n;
     a.out_stride = out_stride;
-    a.row_tiles = (n + TR - 1) / TR;
+    a.row_tiles = (int)((n + TR - 1) / TR);
     a.dim = dim;
     a.group = group;
     a.groups = (dim + group - 1) / group;
     a.x_dtype = x_dtype;
     a.chunks = (dim + CHUNK - 1) / CHUNK;
-    // Warps per row tile: more only while the row tiles leave warps of the grid idle.
-    a.wk = 1;
-    while (a.wk < WARPS && a.wk * 2 <= a.chunks && a.row_tiles * a.wk * 2 <= (int64_t)ctx->sm_count * WARPS) a.wk *= 2;
     const int cols_per_query = x_dtype == VA_DTYPE_F32 ? 4 : 1;
     for (int q0 = 0; q0 < nq;) {
-        // Column tiles of this pass: what the queries fill, within 128 KB of fragments.
+        // Column tiles of this pass: what the queries fill, within 64 KB of fragments (128 KB at 8 warps).
         int nt = 1;
-        while (nt < MAX_NT && nt * 8 < (nq - q0) * cols_per_query && 2 * nt * a.chunks <= 32) nt *= 2;
+        while (nt < MAX_NT && nt * 8 < (nq - q0) * cols_per_query && 2 * nt * a.chunks <= (nt == 2 ? 32 : 16)) nt *= 2;
         a.nq = std::min(nq - q0, nt * 8 / cols_per_query);
         a.x = static_cast<const uint8_t*>(x) + (size_t)q0 * dim * es;
         a.x_scales = x_scales ? x_scales + q0 : nullptr;
         a.out = out + (int64_t)q0 * out_stride;
+        const int warps = warps_of(nt);
+        // Warps per row tile: more only while the row tiles leave warps of the grid idle.
+        a.wk = 1;
+        while (a.wk < 8 && a.wk * 2 <= a.chunks && (int64_t)a.row_tiles * a.wk * 2 <= (int64_t)ctx->sm_count * warps) a.wk *= 2;
         const size_t frag = (size_t)a.chunks * 16 * nt * 32 * sizeof(uint2);
-        const size_t rest = 1024 + frag + 16 + (a.wk > 1 ? (size_t)WARPS * nt * 8 * 32 * 4 : 0);
-        a.ring = (int)std::min<size_t>(6, (227 * 1024 - rest) / (WARPS * (SLOT + 8)));
-        const size_t smem = rest + (size_t)a.ring * WARPS * (SLOT + 8);
-        const int grid = (int)std::min<int64_t>(ctx->sm_count, a.row_tiles);
+        const size_t rest = 1024 + frag + 16 + (a.wk > 1 ? (size_t)warps * nt * 8 * 32 * 4 : 0);
+        a.ring = (int)std::min<size_t>(6, (227 * 1024 - rest) / (warps * (SLOT + 8)));
+        const size_t smem = rest + (size_t)a.ring * warps * (SLOT + 8);
+        const int grid = std::min(ctx->sm_count, a.row_tiles);
         if (nt == 1)
             VA_TRY(launch_types<1>(ctx, map, a, scale_dtype, grid, smem));
         else if (nt == 2)

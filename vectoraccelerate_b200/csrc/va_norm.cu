@@ -7,19 +7,24 @@
 //   code_j = rint(127 z_j / a)
 //   scale  = a / (127 sqrt(mean(h^2) + eps)),   so that code_j * scale ~ z_j / rms(h)
 // The rms cancels from the codes, which are therefore exact: the fp32 quotient decides a code
-// except within 2^-12 of a border between two codes, where it is redone in fp64 (z has at most 48
-// bits), about one element in 2,000. The sum of squares and the scales are fp32. A zero row (or
-// group) has codes 0 and scale 0. A row whose sum of squares is not finite, and a group whose a is
+// except within 2^-12 of a border between two codes (one element in 2,000), where the exact
+// remainder does. The sum of squares and the scales are fp32. A row (or group) with
+// a < 2^-80 has codes 0 and scale 0. A row whose sum of squares is not finite, and a group whose a is
 // not finite, has codes 0 and scale NaN.
 //
-// The work is one read of x and residual, one write of residual_out and the codes: HBM-bound. A
-// row's elements stay in registers between the statistics and the codes (TPR threads x NV vectors of
-// 8 elements), so nothing is read twice; one block barrier per row.
+// The work is one read of x and residual, one write of residual_out and the codes: HBM-bound, with
+// ~20 instructions per element to hide. A thread holds 8 neighbouring elements of a row in registers between
+// the statistics and the codes, so nothing is read twice. Blocks are persistent: each thread's vectors of
+// the next rows come through cp.async into shared memory of its own (no barrier), the weights stay in
+// registers, and a row costs one block barrier.
 #include <algorithm>
 
 #include "va_internal.cuh"
 
 namespace {
+
+// A largest |z| below this counts as zero: fp32 squares and quotients have run out of range by then.
+constexpr float SMALLEST = 0x1p-80f;
 
 struct NormArgs {
     const void* x;
@@ -33,73 +38,81 @@ struct NormArgs {
     float eps;
 };
 
-// Eight elements starting at p (`n` of them inside the row) as fp32. W is the widest access in bytes
+// Eight elements as loaded: bf16 pairs, or fp32.
+template <typename T>
+struct Vec {
+    uint32_t w[sizeof(T) * 2];
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (sizeof(T) == 2)
+            return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+        else
+            return __uint_as_float(w[i]);
+    }
+};
+
+// Eight elements from p, `n` of them inside the row (the others read as 0). W is the widest access in bytes
 // that every row start allows: 16, or the element's size.
 template <typename T, int W>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+__device__ __forceinline__ Vec<T> load8(const T* p, int n) {
+    Vec<T> v;
     if constexpr (W == 16) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-            }
-        } else {
-            const float4 a = *reinterpret_cast<const float4*>(p);
-            const float4 b = *(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uint4 u = n > 0 ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0u, 0u, 0u, 0u);
+            v.w[4 * i] = u.x, v.w[4 * i + 1] = u.y, v.w[4 * i + 2] = u.z, v.w[4 * i + 3] = u.w;
+        }
+    } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = 2 * i < n ? p[2 * i] : (T)0, hi = 2 * i + 1 < n ? p[2 * i + 1] : (T)0;
+            v.w[i] = lo | (hi << 16);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (i >= n) {
-                v[i] = 0.f;
-            } else if constexpr (sizeof(T) == 2) {
-                v[i] = va::bf2f(reinterpret_cast<const uint16_t*>(p)[i]);
-            } else {
-                v[i] = reinterpret_cast<const float*>(p)[i];
-            }
-        }
+        for (int i = 0; i < 8; ++i) v.w[i] = i < n ? __float_as_uint(p[i]) : 0u;
     }
+    return v;
 }
 
 template <typename T, int W>
-__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
+__device__ __forceinline__ void store8(T* p, int n, const Vec<T>& v) {
     if constexpr (W == 16) {
-        if constexpr (sizeof(T) == 2) {
-            uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                w[i] = (__float_as_uint(v[2 * i]) >> 16) | (__float_as_uint(v[2 * i + 1]) & 0xFFFF0000u);
-            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-            *(reinterpret_cast<float4*>(p) + 1) = make_float4(v[4], v[5], v[6], v[7]);
-        }
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            reinterpret_cast<uint4*>(p)[i] = make_uint4(v.w[4 * i], v.w[4 * i + 1], v.w[4 * i + 2], v.w[4 * i + 3]);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < n) {
                 if constexpr (sizeof(T) == 2)
-                    reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(__float_as_uint(v[i]) >> 16);
+                    p[i] = (T)(i & 1 ? v.w[i >> 1] >> 16 : v.w[i >> 1]);
                 else
-                    reinterpret_cast<float*>(p)[i] = v[i];
+                    p[i] = __uint_as_float(v.w[i]);
             }
     }
 }
 
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 // The largest |z| so far, exactly: z = hi + lo with hi = fl(z). Rounding is monotonic, so hi decides
-// and lo only breaks ties of hi. Products of two bf16 values fit fp32: lo stays 0.
+// and lo only breaks ties of hi. Products of two bf16 values fit fp32: lo stays 0. A NaN stays in hi (and
+// is then reported through the scale).
 template <typename T>
 struct Top {
     float hi = 0.f, lo = 0.f;
     __device__ __forceinline__ void take(float h, float l) {
-        // !(h <= hi): a NaN stays in hi (and is then reported through the scale)
         if constexpr (sizeof(T) == 2) {
-            hi = !(h <= hi) ? h : hi;
+            hi = max_nan(hi, h);
         } else {
             const bool more = !(h <= hi) || (h == hi && l > lo);
             lo = more ? l : lo;
@@ -134,152 +147,191 @@ struct Top {
     }
 };
 
-// rint(127 z / a): the fp32 quotient (within 127 * 4 * 2^-24 < 2^-15 of the exact one) unless it is
-// within 2^-12 of a border or not finite (127 / a overflowed), then fp64.
+// rint(127 z / a) of eight elements, packed. t = z (127 / a) in fp32 is within 127 * 4 * 2^-24 < 2^-15 of the
+// quotient; adding 1.5 * 2^23 rounds it (to even) into the low byte. Where some t is within 2^-12 of the border
+// b between two codes, the sign of 127 z - b a decides: for bf16 both products are exact in fp32 (7 + 16 and 8 + 16
+// bits); for fp32 their rounding errors and the low parts are added (48 bits).
 template <typename T>
-__device__ __forceinline__ int code_of(float h, float w, float inv, const Top<T>& a) {
-    const float t = h * w * inv;
-    const float r = rintf(t);
-    if (fabsf(fabsf(t - r) - 0.5f) >= 0x1p-12f) return (int)r;
-    const double z = (double)h * (double)w;
-    return (int)rint(z * 127.0 / ((double)a.hi + (double)a.lo));
-}
-
-// TPR threads per row, NV vectors of 8 elements per thread; NV * 8 * TPR >= dim. 32-thread rows
-// share a block of 128 threads; wider rows take a block each.
-template <typename T, int W, int TPR, int NV>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) k_rms_norm_int8(NormArgs a) {
-    constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
-    constexpr int WARPS = TPR / 32;
-    __shared__ float s_sum[ROWS][WARPS], s_hi[ROWS][WARPS], s_lo[ROWS][WARPS];
-    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-    const int64_t row_id = (int64_t)blockIdx.x * ROWS + slot;
-    const bool live = row_id < a.rows;
-    const int64_t row = live ? row_id : a.rows - 1;  // a spare slot repeats the last row, without stores
-    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
-    const T* weight = static_cast<const T*>(a.weight);
-
-    float h[NV][8];
+__device__ __forceinline__ uint2 codes_of(const Vec<T>& h, const Vec<T>& w, const Top<T>& a) {
+    uint32_t m[8];
+    constexpr float SHIFT = 12582912.f;
+    const float inv = 127.f / a.hi;
+    float off = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int j = (i * TPR + t) * 8;
-        if (j < a.dim) {
-            load8<T, W>(x + j, a.dim - j, h[i]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) h[i][k] = 0.f;
-        }
+    for (int k = 0; k < 8; ++k) {
+        const float t = h[k] * w[k] * inv, r = t + SHIFT;
+        m[k] = __float_as_uint(r);
+        off = fmaxf(off, fabsf(t - (r - SHIFT)));
     }
-    float w[NV][8];
+    if (off > 0.5f - 0x1p-12f) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int j = (i * TPR + t) * 8;
-        if (j < a.dim) {
-            load8<T, W>(weight + j, a.dim - j, w[i]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[i][k] = 0.f;
-        }
-    }
-    if (res) {
-        // Every load precedes the stores: residual_out may be x's or residual's own rows.
-        float r[NV][8];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = (i * TPR + t) * 8;
-            if (j < a.dim) load8<T, W>(res + j, a.dim - j, r[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = (i * TPR + t) * 8;
-            if (j < a.dim) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    h[i][k] += r[i][k];
-                    if constexpr (sizeof(T) == 2) h[i][k] = va::bf2f(va::f2bf_rn(h[i][k]));
-                }
-                if (live && a.residual_out)
-                    store8<T, W>(static_cast<T*>(a.residual_out) + row * a.dim + j, a.dim - j, h[i]);
+        for (int k = 0; k < 8; ++k) {
+            const float z = h[k] * w[k], t = z * inv, r = __uint_as_float(m[k]) - SHIFT, d = t - r;
+            if (fabsf(d) > 0.5f - 0x1p-12f) {
+                const float b = r + copysignf(0.5f, d), p = b * a.hi, q = 127.f * z;
+                float diff = q - p;
+                if constexpr (sizeof(T) == 4)
+                    diff += (fmaf(127.f, z, -q) - fmaf(b, a.hi, -p)) + (127.f * fmaf(h[k], w[k], -z) - b * a.lo);
+                const float past = copysignf(diff, 1.f) == 0.f ? ((m[k] & 1u) ? 1.f : -1.f) : (d > 0.f ? diff : -diff);
+                if (past > 0.f) m[k] += d > 0.f ? 1u : 0xFFFFFFFFu;
             }
         }
     }
-    float sum = 0.f;
-    Top<T> top[NV];
+    uint2 p;
+    p.x = __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410);
+    p.y = __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410);
+    return p;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Rows on their way per thread (16-byte accesses only).
+template <typename T>
+constexpr int stages_of() { return sizeof(T) == 2 ? 3 : 2; }
+
+// TPR threads per row, 8 elements each; 8 * TPR >= dim. Narrow rows share a block of 128 threads.
+template <typename T, int W, int TPR>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR < 512 ? 1024 / (TPR < 128 ? 128 : TPR) : 2)
+    k_rms_norm_int8(NormArgs a) {
+    constexpr int THREADS = TPR < 128 ? 128 : TPR, ROWS = THREADS / TPR, WARPS = TPR / 32, STAGES = stages_of<T>();
+    constexpr int HALVES = sizeof(T) / 2;  // 16-byte pieces of a vector
+    extern __shared__ uint4 s_in[];        // [stage][x, residual][piece][thread]
+    __shared__ float s_sum[2][ROWS][WARPS], s_hi[2][ROWS][WARPS], s_lo[2][ROWS][WARPS];
+    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR, j = t * 8;
+    const Vec<T> w = load8<T, W>(static_cast<const T*>(a.weight) + j, a.dim - j);
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    // Every thread of a block makes the same number of turns (barriers); rows past the end repeat the last one.
+    const int64_t row0 = (int64_t)blockIdx.x * ROWS;
+    const auto mine = [&](int64_t r) { return min(r + slot, a.rows - 1); };
+    const auto fetch = [&](int64_t r, int stage) {
+        if constexpr (W == 16) {
+            if (r < a.rows && j < a.dim) {
+                const T* px = static_cast<const T*>(a.x) + mine(r) * a.x_stride + j;
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(s_in + (size_t)stage * 2 * HALVES * THREADS + threadIdx.x);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
+                for (int i = 0; i < HALVES; ++i) cp_async16(dst + i * THREADS * 16, reinterpret_cast<const uint4*>(px) + i);
+                if (a.residual) {
+                    const T* pr = static_cast<const T*>(a.residual) + mine(r) * a.residual_stride + j;
+#pragma unroll
+                    for (int i = 0; i < HALVES; ++i)
+                        cp_async16(dst + (HALVES + i) * THREADS * 16, reinterpret_cast<const uint4*>(pr) + i);
+                }
+            }
+            cp_async_commit();
+        }
+    };
+    const auto take = [&](int64_t r, int stage, bool residual) {
+        if constexpr (W == 16) {
+            Vec<T> v;
+            const uint4* from = s_in + ((size_t)stage * 2 + (residual ? 1 : 0)) * HALVES * THREADS + threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < HALVES; ++i) {
+                const uint4 u = j < a.dim ? from[i * THREADS] : make_uint4(0u, 0u, 0u, 0u);
+                v.w[4 * i] = u.x, v.w[4 * i + 1] = u.y, v.w[4 * i + 2] = u.z, v.w[4 * i + 3] = u.w;
+            }
+            return v;
+        } else {
+            const T* p = residual ? static_cast<const T*>(a.residual) + mine(r) * a.residual_stride
+                                  : static_cast<const T*>(a.x) + mine(r) * a.x_stride;
+            return load8<T, W>(p + j, a.dim - j);
+        }
+    };
+    for (int s = 0; s < STAGES - 1; ++s) fetch(row0 + s * step, s);
+    int stage = 0, turn = 0;
+    for (int64_t r = row0; r < a.rows; r += step, turn ^= 1) {
+        // (residual_out may be x's or residual's own rows: a row is stored only after its loads.)
+        fetch(r + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+        cp_async_wait<STAGES - 1>();
+        const int64_t row = mine(r);
+        const bool live = r + slot < a.rows;
+        Vec<T> h = take(r, stage, false);
+        if (a.residual) {
+            const Vec<T> v = take(r, stage, true);
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) h.w[k] = pack_bf16(h[2 * k] + v[2 * k], h[2 * k + 1] + v[2 * k + 1]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) h.w[k] = __float_as_uint(h[k] + v[k]);
+            }
+            if (a.residual_out && live && j < a.dim)
+                store8<T, W>(static_cast<T*>(a.residual_out) + row * a.dim + j, a.dim - j, h);
+        }
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        float sum = 0.f;
+        Top<T> top;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            sum = fmaf(h[i][k], h[i][k], sum);
-            top[i].element(h[i][k], w[i][k]);
+            sum = fmaf(h[k], h[k], sum);
+            top.element(h[k], w[k]);
         }
-    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if (a.group) {
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (a.group)
+            top.lanes(a.group / 8);
+        else
+            top.template lanes<32>();
+        if constexpr (WARPS > 1) {
+            // Two sets of slots in turn: one barrier per row.
+            if ((t & 31) == 0) {
+                s_sum[turn][slot][t >> 5] = sum;
+                s_hi[turn][slot][t >> 5] = top.hi;
+                s_lo[turn][slot][t >> 5] = top.lo;
+            }
+            __syncthreads();
+            sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) top[i].lanes(a.group / 8);
-    } else {
+            for (int k = 0; k < WARPS; ++k) sum += s_sum[turn][slot][k];
+            if (!a.group) {
 #pragma unroll
-        for (int i = 1; i < NV; ++i) top[0].take(top[i].hi, top[i].lo);
-        top[0].template lanes<32>();
-    }
-    if constexpr (WARPS > 1) {
-        const int warp = t >> 5;
-        if ((t & 31) == 0) {
-            s_sum[slot][warp] = sum;
-            s_hi[slot][warp] = top[0].hi;
-            s_lo[slot][warp] = top[0].lo;
+                for (int k = 0; k < WARPS; ++k) top.take(s_hi[turn][slot][k], s_lo[turn][slot][k]);
+            }
         }
-        __syncthreads();
-        sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < WARPS; ++k) sum += s_sum[slot][k];
-        if (!a.group) {
-#pragma unroll
-            for (int k = 0; k < WARPS; ++k) top[0].take(s_hi[slot][k], s_lo[slot][k]);
+        if (!live || j >= a.dim) continue;
+        const bool ok = sum < INFINITY && top.hi < INFINITY;  // false for NaN too
+        if (a.group ? j % a.group == 0 : j == 0) {
+            const float per = rsqrtf(sum / (float)a.dim + a.eps) / 127.f;
+            a.scales[row * a.groups + (a.group ? j / a.group : 0)] =
+                !ok ? __int_as_float(0x7FC00000) : top.hi >= SMALLEST ? top.hi * per : 0.f;
         }
-    }
-    if (!live) return;
-    const bool finite = sum < INFINITY;  // false for NaN too
-    const float per = rsqrtf(sum / (float)a.dim + a.eps) / 127.f;
-    int8_t* codes = a.codes + row * a.dim;
-    float* scales = a.scales + row * a.groups;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int j = (i * TPR + t) * 8;
-        if (j >= a.dim) continue;
-        const Top<T> top_i = a.group ? top[i] : top[0];
-        const bool ok = finite && top_i.hi < INFINITY;
-        if (a.group ? j % a.group == 0 : j == 0)
-            scales[a.group ? j / a.group : 0] = ok ? top_i.hi * per : __int_as_float(0x7FC00000);
-        const float inv = 127.f / top_i.hi;
-        uint32_t packed[2] = {0u, 0u};
-        if (ok && top_i.hi > 0.f) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                packed[k >> 2] |= ((uint32_t)code_of<T>(h[i][k], w[i][k], inv, top_i) & 0xFFu) << (8 * (k & 3));
-        }
+        uint2 packed = make_uint2(0u, 0u);
+        if (ok && top.hi >= SMALLEST) packed = codes_of<T>(h, w, top);
+        int8_t* codes = a.codes + row * a.dim + j;
         if constexpr (W == 16) {
-            *reinterpret_cast<uint2*>(codes + j) = make_uint2(packed[0], packed[1]);
+            *reinterpret_cast<uint2*>(codes) = packed;
         } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (j + k < a.dim) codes[j + k] = (int8_t)(packed[k >> 2] >> (8 * (k & 3)));
+                if (j + k < a.dim) codes[k] = (int8_t)((k < 4 ? packed.x : packed.y) >> (8 * (k & 3)));
         }
     }
+}
+
+template <typename T, int W, int TPR>
+int launch_rows(va_context* ctx, const NormArgs& a) {
+    constexpr int THREADS = TPR < 128 ? 128 : TPR, ROWS = THREADS / TPR, BLOCKS = TPR < 512 ? 1024 / THREADS : 2;
+    constexpr size_t SMEM = W == 16 ? (size_t)stages_of<T>() * 2 * (sizeof(T) / 2) * THREADS * 16 : 0;
+    if (SMEM > 47 * 1024)  // (with the static part over the 48 KB that need no asking)
+        VA_CUDA_TRY(cudaFuncSetAttribute(k_rms_norm_int8<T, W, TPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+    const int64_t grid = std::min<int64_t>((a.rows + ROWS - 1) / ROWS, (int64_t)ctx->sm_count * BLOCKS);
+    k_rms_norm_int8<T, W, TPR><<<(unsigned)grid, THREADS, SMEM, ctx->stream>>>(a);
+    return va_check_launch("k_rms_norm_int8");
 }
 
 template <typename T, int W>
 int launch_norm(va_context* ctx, const NormArgs& a) {
-    const int vecs = (a.dim + 7) / 8;
-    if (vecs <= 64)
-        k_rms_norm_int8<T, W, 32, 2><<<(unsigned)((a.rows + 3) / 4), 128, 0, ctx->stream>>>(a);
-    else if (vecs <= 256)
-        k_rms_norm_int8<T, W, 128, 2><<<(unsigned)a.rows, 128, 0, ctx->stream>>>(a);
-    else
-        k_rms_norm_int8<T, W, 256, 2><<<(unsigned)a.rows, 256, 0, ctx->stream>>>(a);
-    return va_check_launch("k_rms_norm_int8");
+    if (a.dim <= 256) return launch_rows<T, W, 32>(ctx, a);
+    if (a.dim <= 512) return launch_rows<T, W, 64>(ctx, a);
+    if (a.dim <= 1024) return launch_rows<T, W, 128>(ctx, a);
+    if (a.dim <= 2048) return launch_rows<T, W, 256>(ctx, a);
+    return launch_rows<T, W, 512>(ctx, a);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
