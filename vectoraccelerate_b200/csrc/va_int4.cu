@@ -7,19 +7,25 @@
 // scale * (c - zero).
 //
 // Scores: out[q, r] = xs_q * sum_g scale[r, g] * sum_{j in g} (c[r, j] - zero[r, g]) x[q, j].
-// The codes are read once per pass of up to 32 columns, 4 bits for 2 to 32 operations: HBM-bound, if
-// unpacking keeps pace. So the products run on the tensor cores through mma.sync m16n8k16 (codes are A, 16
-// rows; queries are B, 8 columns): a code costs 1.4 integer instructions to become an exact bf16 and
-// nothing more for 1..8 columns, where fp32 FMAs would take 1.5 + columns. tcgen05 would need the
-// unpacked codes written to shared memory (4 bytes of traffic per byte read) to use a 128-row tile
-// whose columns stay mostly empty.
-//   * The codes enter as integers in [-15, 15] (exact in bf16), the scale multiplies the fp32 group sum.
-//   * bf16 and int8 queries are exact as one bf16 column; an fp32 query is split by truncation into
-//     three bf16 columns of 8 mantissa bits each, exact again, and the three sums are added at the end.
+// The codes are read once per pass of queries, 4 bits for 2 to 64 operations: HBM-bound, if unpacking keeps
+// pace: the logic pipe takes half an instruction per clock and scheduler. The products run on the tensor cores
+// through mma.sync (codes are A, 16 rows; queries are B, 8 columns). tcgen05 would need the unpacked codes written
+// to shared memory to use a 128-row tile whose columns stay mostly empty. Two forms:
+//   * DIGITS, integer m16n8k32: three logic instructions turn 8 codes into 8 bytes c + 8. An int8 query is one
+//     column; an fp32 or bf16 query becomes, per group, fixed-point numbers of 31 bits below the power of two above
+//     the group's largest |x| (an error of at most 2^-30 of that |x|), in four columns of signed 8-bit digits. Group
+//     sums are exact integers below 2^22; they start at 1.5 * 2^23 as a bit pattern, less (8 + zero) times the digits'
+//     sum, so that the finished accumulator read as fp32 and less 1.5 * 2^23 is the group's sum.
+//   * PIECES, bf16 m16n8k16: 11 instructions turn 8 codes into 8 exact bf16 values c - zero. A bf16 query is one
+//     column, exact; an fp32 query is split by truncation into three bf16 values of 8 mantissa bits each, exact, that
+//     are multiplied in turn into the same sum.
+//   Digits cost four columns and their recombination per group and query, pieces cost more per code: digits serve int8
+//   queries and up to two others, pieces the rest (TIMES).
+//   * Group scales and query scales are applied and the groups summed in fp32.
 //   * A warp owns 32 rows. Its tiles of 32 rows x 128 bytes arrive by TMA in a ring of its own (one
 //     lane issues, the warp waits; no other warp is involved), 128B-swizzled, so that the four words
 //     of a 32-code block of 8 rows are one conflict-free access.
-//   * The query fragments are laid out once per block in shared memory in the order the mma reads.
+//   * The queries are laid out once per block in shared memory in the order the mma reads.
 //   * Few rows: WK warps share a row tile, each takes every WK-th 256-code chunk, and the first adds
 //     the partial sums in order.
 #include <algorithm>
@@ -33,7 +39,6 @@ using namespace va::tc;
 constexpr int TR = 32;             // rows per warp tile
 constexpr int CHUNK = 256;         // codes per ring slot and row (128 bytes)
 constexpr int SLOT = TR * 128;     // bytes of a ring slot
-constexpr int MAX_NT = 4;          // column tiles of 8 per pass
 
 struct MatvecArgs {
     const void* x;
@@ -43,11 +48,21 @@ struct MatvecArgs {
     float* out;
     int64_t n, out_stride;
     int row_tiles;
-    int dim, group, groups, nq, x_dtype;
+    int dim, groups, nq, x_dtype;
     int chunks;  // 256-code chunks per row
     int wk;      // warps sharing a row tile
     int ring;    // slots per warp
 };
+
+// What a column of B holds: an int8 query; a digit of a query; a query (bf16) or its three pieces in turn (fp32).
+enum Mode { DIGITS_INT8, DIGITS_WIDE, BF16, BF16X3 };
+constexpr int pieces_of(int mode) { return mode == BF16X3 ? 3 : 1; }
+constexpr bool is_bf16(int mode) { return mode == BF16 || mode == BF16X3; }
+// Bytes of shared memory that one chunk's queries take per column tile.
+constexpr int frag_bytes(int mode) { return 32 * 8 * (is_bf16(mode) ? 16 * pieces_of(mode) : 8); }
+
+constexpr uint32_t MAGIC = 0x4B400000u;  // 1.5 * 2^23 as fp32 bits
+constexpr float MAGIC_F = 12582912.f;
 
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     uint32_t v;
@@ -55,92 +70,186 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     return v;
 }
 
-// (w & 0x000F000F) ^ 0x43084308: the two nibbles at bits 0 and 16 as bf16 values 128 + (c + 8).
-__device__ __forceinline__ uint32_t nibbles(uint32_t w) { return (w & 0x000F000Fu) ^ 0x43084308u; }
+// The low nibbles of four bytes as c + 8.
+__device__ __forceinline__ uint32_t nibbles(uint32_t w) { return (w & 0x0F0F0F0Fu) ^ 0x08080808u; }
 
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+// d = a b + c
+__device__ __forceinline__ void mma_u8s8(uint32_t (&d)[4], const uint32_t (&a)[4], uint2 b, const uint32_t (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+
+// (w & 0x000F000F) ^ 0x43084308: the nibbles at bits 0 and 16 as bf16 values 128 + (c + 8); less 136 + zero.
+__device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t bias) {
     uint32_t d;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"((w & 0x000F000Fu) ^ 0x43084308u), "r"(bias));
     return d;
 }
 
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint2 b, const float (&c)[4]) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Column `col` of the query operand at element j: the query's value, or piece col & 3 of an fp32
-// query (three pieces of 8 mantissa bits, the fourth column is zero). bf16 bit pattern.
-__device__ __forceinline__ uint16_t query_bits(const MatvecArgs& a, int col, int j) {
-    if (j >= a.dim) return 0;
-    if (a.x_dtype == VA_DTYPE_F32) {
-        const int q = col >> 2, piece = col & 3;
-        if (q >= a.nq || piece == 3) return 0;
-        float v = static_cast<const float*>(a.x)[(int64_t)q * a.dim + j];
-        uint32_t u = __float_as_uint(v) & 0xFFFF0000u;
-        if ((u & 0x7F800000u) == 0x7F800000u) {  // infinity or NaN: all of it in the first piece
-            if (v != v) u |= 0x00400000u;
-            return piece == 0 ? (uint16_t)(u >> 16) : (uint16_t)0;
-        }
-        for (int p = 0; p < piece; ++p) {
-            v -= __uint_as_float(u);
-            u = __float_as_uint(v) & 0xFFFF0000u;
-        }
-        return (uint16_t)(u >> 16);
-    }
-    if (col >= a.nq) return 0;
-    const int64_t at = (int64_t)col * a.dim + j;
-    if (a.x_dtype == VA_DTYPE_BF16) return static_cast<const uint16_t*>(a.x)[at];
-    return (uint16_t)(__float_as_uint((float)static_cast<const int8_t*>(a.x)[at]) >> 16);
+// Loads that stay where they are written (ahead of the chunk they are for), as the wait and the products do.
+__device__ __forceinline__ uint32_t load_ahead(const uint16_t* p) {
+    uint16_t v;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t load_ahead(const float* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ int load_ahead(const int8_t* p) {
+    int v;
+    asm volatile("ld.global.nc.s8 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
 }
 
-template <typename S>
-__device__ __forceinline__ float scale_of(const S* p) {
-    if constexpr (sizeof(S) == 2)
-        return va::bf2f(__ldg(p));
-    else
-        return __ldg(p);
-}
-
-// The scales (and 136 + zero point, as bf16 bits) that a lane holds of one chunk: of its four rows, groups t and
-// t + 4 of the chunk.
+// The scales and zero points that a lane holds of one chunk: of its four rows, groups t and t + 4 of the chunk.
 template <typename S, bool ZERO, int GROUP>
 struct ChunkScales {
     static constexpr int GPC = CHUNK / GROUP;           // groups per chunk
     static constexpr int SPL = GPC > 4 ? GPC / 4 : 1;   // held per lane and row
-    float sc[4][SPL];
-    uint32_t zp[ZERO ? 4 : 1][ZERO ? SPL : 1];
-    __device__ __forceinline__ void load(const MatvecArgs& a, int64_t row0, int c, int g, int t) {
+    uint32_t sc[4][SPL];  // as stored
+    int zp[ZERO ? 4 : 1][ZERO ? SPL : 1];
+    __device__ __forceinline__ void load(const MatvecArgs& a, const int64_t (&base)[4], int c, int t) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            // rows past the end repeat the last one: they are not stored
-            const int64_t base = min(row0 + g + 8 * r, a.n - 1) * a.groups;
+        for (int p = 0; p < SPL; ++p) {
+            const int gi = min(c * GPC + (t & (GPC - 1)) + 4 * p, a.groups - 1);
 #pragma unroll
-            for (int p = 0; p < SPL; ++p) {
-                const int gi = min(c * GPC + (t & (GPC - 1)) + 4 * p, a.groups - 1);
-                sc[r][p] = scale_of(static_cast<const S*>(a.scales) + base + gi);
-                if constexpr (ZERO) zp[r][p] = 0x4308u + (uint32_t)(int)__ldg(a.zeros + base + gi);
+            for (int r = 0; r < 4; ++r) {
+                sc[r][p] = load_ahead(static_cast<const S*>(a.scales) + base[r] + gi);
+                if constexpr (ZERO) zp[r][p] = load_ahead(a.zeros + base[r] + gi);
             }
         }
     }
 };
 
+// First scales of a lane's four rows in a row tile; rows past the end repeat the last one (they are not stored).
+__device__ __forceinline__ void row_bases(const MatvecArgs& a, int tile, int g, int64_t (&base)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) base[r] = min((int64_t)tile * TR + g + 8 * r, a.n - 1) * a.groups;
+}
+
+// What a block keeps of the queries in shared memory.
+struct QueryShared {
+    uint2* frag;    // [chunk][block 8][step 2 of bf16][NT][piece][lane]: in the mma's order
+    int* start;     // [group][NT * 8]: MAGIC - 8 * sum of the column's digits
+    float* weight;  // [group][NT * 4]: of a pair of columns (DIGITS_WIDE)
+};
+
+// One warp lays out group `grp` of query q (absent queries and elements are zeros). The 32-code block's word t has
+// the nibbles of elements 8t..8t + 7: the even ones are k = 4t.. of the mma, the odd ones k = 16 + 4t...
+template <int NT, int GROUP, int MODE>
+__device__ __forceinline__ void lay_out(const MatvecArgs& a, const QueryShared& sh, int q, int grp, int lane) {
+    constexpr int E = GROUP / 32;
+    if constexpr (is_bf16(MODE)) {
+        // k16 step h of a block pairs the nibbles (2h, 2h + 4) and (2h + 1, 2h + 5) of each word.
+        constexpr int P = pieces_of(MODE);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int blk = grp * E + e, j = blk * 32 + lane, r = lane & 7;
+            const int64_t at = (int64_t)q * a.dim + j;
+            const bool there = q < a.nq && j < a.dim;
+            uint16_t* to = reinterpret_cast<uint16_t*>(
+                               sh.frag + (((size_t)blk * 2 + ((r >> 1) & 1)) * NT + (q >> 3)) * P * 32 + (q & 7) * 4 + (lane >> 3)) +
+                           (r & 1) * 2 + (r >> 2);
+            if constexpr (P == 1) {
+                *to = there ? static_cast<const uint16_t*>(a.x)[at] : (uint16_t)0;
+            } else {
+                float v = there ? static_cast<const float*>(a.x)[at] : 0.f;
+                const bool finite = fabsf(v) < INFINITY;
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    // an infinity or a NaN stays in the first piece
+                    const uint32_t u = v != v ? 0x7FC00000u : __float_as_uint(v) & 0xFFFF0000u;
+                    to[(size_t)p * 32 * 4] = (uint16_t)(u >> 16);
+                    v = finite ? v - __uint_as_float(u) : 0.f;
+                }
+            }
+        }
+        return;
+    }
+    constexpr bool wide = MODE == DIGITS_WIDE;
+    int v[E];
+    float w = 0.f;
+    if constexpr (!wide) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int j = grp * GROUP + e * 32 + lane;
+            v[e] = q < a.nq && j < a.dim ? static_cast<const int8_t*>(a.x)[(int64_t)q * a.dim + j] : 0;
+        }
+    } else {
+        float f[E], top = 0.f;
+        bool finite = true;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int j = grp * GROUP + e * 32 + lane;
+            const int64_t at = (int64_t)q * a.dim + j;
+            f[e] = q >= a.nq || j >= a.dim ? 0.f
+                   : a.x_dtype == VA_DTYPE_F32 ? static_cast<const float*>(a.x)[at]
+                                               : va::bf2f(static_cast<const uint16_t*>(a.x)[at]);
+            finite = finite && fabsf(f[e]) < INFINITY;
+            top = fmaxf(top, fabsf(f[e]));
+        }
+        finite = __all_sync(0xFFFFFFFFu, finite);
+        top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));
+        // 2^e > top; the fixed point's unit is 2^(e - 30), not below the smallest fp32.
+        const int e = max((int)(__float_as_uint(top) >> 23) - 126, -119);
+        w = finite ? ldexpf(1.f, e - 30) : __int_as_float(0x7FC00000);
+        // (two steps: the factor alone may exceed fp32)
+        const float up = ldexpf(1.f, (30 - e) / 2), up2 = ldexpf(1.f, 30 - e - (30 - e) / 2);
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = finite ? __float2int_rn(f[i] * up * up2) : 0;
+    }
+    constexpr int planes = wide ? 4 : 1;
+#pragma unroll
+    for (int p = planes - 1; p >= 0; --p) {  // digits from the lowest; column p = 0 has the highest
+        const int col = q * planes + p;
+        int sum = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int d = (int)(int8_t)v[e];
+            v[e] = (v[e] - d) >> 8;
+            sum += d;
+            const int blk = grp * E + e;
+            int8_t* to = reinterpret_cast<int8_t*>(sh.frag + ((size_t)blk * NT + (col >> 3)) * 32 + (col & 7) * 4 + (lane >> 3));
+            to[(lane & 1) * 4 + ((lane & 7) >> 1)] = (int8_t)d;
+        }
+        sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+        if (lane == 0) sh.start[(size_t)grp * NT * 8 + col] = (int)(MAGIC - 8u * (uint32_t)sum);
+    }
+    if (wide && lane < 2) sh.weight[(size_t)grp * NT * 4 + q * 2 + lane] = lane == 0 ? w * 65536.f : w;
+}
+
 // NT column tiles of 8; S = scale type (uint16_t: bf16); GROUP = 32, 64, 128.
-template <int NT, int WARPS, typename S, bool ZERO, int GROUP>
+template <int MODE, int NT, int WARPS, typename S, bool ZERO, int GROUP>
 __global__ void __launch_bounds__(WARPS * 32, 1)
     k_int4_matvec(const __grid_constant__ CUtensorMap codes, MatvecArgs a, int* err, uint64_t limit_ns) {
     extern __shared__ uint8_t smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
+    using Scales = ChunkScales<S, ZERO, GROUP>;
+    constexpr int GPC = Scales::GPC, P = pieces_of(MODE);
+    constexpr bool WIDE = MODE == DIGITS_WIDE;
+    const int groups_pad = a.chunks * GPC;
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* ring = smem + (size_t)warp * a.ring * SLOT;
-    uint2* frag = (uint2*)(smem + (size_t)WARPS * a.ring * SLOT);  // [chunk][step 16][NT][lane]
-    uint64_t* bars = (uint64_t*)(frag + (size_t)a.chunks * 16 * NT * 32);
+    QueryShared sh;
+    sh.frag = (uint2*)(smem + (size_t)WARPS * a.ring * SLOT);
+    sh.start = (int*)(sh.frag + (size_t)a.chunks * NT * (frag_bytes(MODE) / 8));
+    sh.weight = (float*)(sh.start + (is_bf16(MODE) ? 0 : (size_t)groups_pad * NT * 8));
+    uint64_t* bars = (uint64_t*)(sh.weight + (is_bf16(MODE) ? 0 : (size_t)groups_pad * NT * 4));
     uint64_t* full = bars + warp * a.ring;
     volatile int* s_abort = (volatile int*)(bars + WARPS * a.ring);
-    float* join = (float*)(bars + WARPS * a.ring + 1);  // [WARPS][NT][2][4][32], only with wk > 1
+    float* join = (float*)(bars + WARPS * a.ring + 1);  // [WARPS][NT * 8][32], only with wk > 1
 
     const int teams = WARPS / a.wk, team = warp / a.wk, part = warp % a.wk;
     // Row tiles go round the blocks first, so that few tiles spread over all SMs.
@@ -170,99 +279,150 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     };
     if (lane == 0)
         for (; issued < (uint32_t)a.ring && left > 0; ++issued) issue((int)issued);
-    using Scales = ChunkScales<S, ZERO, GROUP>;
     Scales next;
-    if (tiles > 0) next.load(a, (int64_t)first * TR, part, g, t);
+    int64_t base[4];
+    row_bases(a, min(first, a.row_tiles - 1), g, base);
+    next.load(a, base, part, t);
 
-    // Query fragments. k16 step i of a chunk: half i & 1 of 32-code block i >> 1. Lane (g, t) reads word
-    // t of the block, whose nibbles 0..7 are elements 8t..8t+7; half h pairs the nibbles (2h, 2h + 4) and
-    // (2h + 1, 2h + 5), which B's registers must match for column g.
-    for (int e = threadIdx.x; e < a.chunks * 16 * NT * 32; e += WARPS * 32) {
-        const int l = e & 31, nt = (e >> 5) % NT, i = (e >> 5) / NT;
-        const int j = (i >> 1) * 32 + (l & 3) * 8 + 2 * (i & 1), col = nt * 8 + (l >> 2);
-        uint2 f;
-        f.x = query_bits(a, col, j) | ((uint32_t)query_bits(a, col, j + 4) << 16);
-        f.y = query_bits(a, col, j + 1) | ((uint32_t)query_bits(a, col, j + 5) << 16);
-        frag[e] = f;
-    }
+    constexpr int QUERIES = WIDE ? NT * 2 : NT * 8;
+    for (int i = warp; i < groups_pad * QUERIES; i += WARPS) lay_out<NT, GROUP, MODE>(a, sh, i % QUERIES, i / QUERIES, lane);
     __syncthreads();
 
-    const uint32_t slot0 = smem_u32(ring) + g * 128 + t * 4;
+    // (the 16-byte unit b of row r lies at unit b ^ (r & 7) of its 128 bytes)
+    const uint32_t slot0 = smem_u32(ring) + g * 128 + g * 16 + t * 4;
+    const uint2* const frag0 = sh.frag + lane;
     bool dead = false;
     int s = 0;
     uint32_t phase = 0;
+    constexpr int ACC = WIDE ? 2 : 4;  // sums per row tile half: rows g and g + 8, of a pair of columns each or added up
     for (int k = 0; k < tiles; ++k) {
         const int tile = first + k * step;
-        const int64_t row0 = (int64_t)tile * TR;
-        float acc[NT][2][4];
+        float acc[NT][2][ACC];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[n][m][i] = 0.f;
+                for (int i = 0; i < ACC; ++i) acc[n][m][i] = 0.f;
         for (int c = part; c < a.chunks; c += a.wk) {
             // The next chunk's scales are on their way while this one is multiplied.
             const Scales now = next;
-            const bool last = c + a.wk >= a.chunks;
-            if (!last || k + 1 < tiles) next.load(a, last ? row0 + (int64_t)step * TR : row0, last ? part : c + a.wk, g, t);
+            if (c + a.wk < a.chunks) {
+                next.load(a, base, c + a.wk, t);
+            } else if (k + 1 < tiles) {
+                row_bases(a, tile + step, g, base);
+                next.load(a, base, part, t);
+            }
             // Every lane waits: the phase it has seen is what makes the copy's bytes visible to it.
             if (!dead) dead = __any_sync(0xFFFFFFFFu, !mbar_wait(&full[s], phase, s_abort, err, limit_ns));
             if (dead) break;
             const uint32_t slot = slot0 + s * SLOT;
-            const uint2* fr = frag + (size_t)c * 16 * NT * 32 + lane;
+            const uint2* fr = frag0 + (size_t)c * NT * (frag_bytes(MODE) / 8);
+            const int2* starts = reinterpret_cast<const int2*>(sh.start + (size_t)c * GPC * NT * 8) + t;
+            const float* weight = sh.weight + (size_t)c * GPC * NT * 4 + t;
 #pragma unroll
-            for (int gi = 0; gi < Scales::GPC; ++gi) {
-                float grp[NT][2][4];
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) grp[n][m][i] = 0.f;
+            for (int gi = 0; gi < GPC; ++gi) {
                 float gs[4];
-                uint32_t bias[4];
+                int zero[4];
+                const int from = (lane & ~3) | (gi & 3);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int from = (lane & ~3) | (gi & 3);
-                    gs[r] = __shfl_sync(0xFFFFFFFFu, now.sc[r][Scales::SPL > 1 ? gi >> 2 : 0], from);
-                    if constexpr (ZERO) {
-                        const uint32_t z = __shfl_sync(0xFFFFFFFFu, now.zp[r][Scales::SPL > 1 ? gi >> 2 : 0], from);
-                        bias[r] = z | (z << 16);  // 136 + zero point, exact in bf16
-                    } else {
-                        bias[r] = 0x43084308u;  // 136
-                    }
+                    gs[r] = __uint_as_float(__shfl_sync(0xFFFFFFFFu, now.sc[r][Scales::SPL > 1 ? gi >> 2 : 0], from)
+                                            << (sizeof(S) == 2 ? 16 : 0));
+                    zero[r] = 0;
+                    if constexpr (ZERO) zero[r] = __shfl_sync(0xFFFFFFFFu, now.zp[r][Scales::SPL > 1 ? gi >> 2 : 0], from);
                 }
+                if constexpr (is_bf16(MODE)) {
+                    float grp[NT][2][4];
+                    uint32_t bias[4];
 #pragma unroll
-                for (int b = 0; b < GROUP / 32; ++b) {
-                    const int blk = gi * (GROUP / 32) + b;
-                    uint32_t w[4];
+                    for (int r = 0; r < 4; ++r) bias[r] = (0x4308u + (uint32_t)zero[r]) * 0x10001u;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) w[r] = lds32(slot + r * 1024 + ((blk ^ g) << 4));
+                    for (int b = 0; b < GROUP / 32; ++b) {
+                        const int blk = gi * (GROUP / 32) + b;
+                        uint32_t w[4];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                        for (int r = 0; r < 4; ++r) w[r] = lds32((slot ^ (blk << 4)) + r * 1024);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t f[2][4];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                f[r >> 1][r & 1] = pair(w[r] >> (8 * h), bias[r]);
+                                f[r >> 1][2 + (r & 1)] = pair(w[r] >> (8 * h + 4), bias[r]);
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int p = 0; p < P; ++p) {
+                                    const uint2 q = fr[(((blk * 2 + h) * NT + n) * P + p) * 32];
+                                    const float none[4] = {0.f, 0.f, 0.f, 0.f};
+                                    if (b + h + p == 0) {
+                                        mma_bf16(grp[n][0], f[0], q, none);
+                                        mma_bf16(grp[n][1], f[1], q, none);
+                                    } else {
+                                        mma_bf16(grp[n][0], f[0], q, grp[n][0]);
+                                        mma_bf16(grp[n][1], f[1], q, grp[n][1]);
+                                    }
+                                }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int m = 0; m < 2; ++m)
+#pragma unroll
+                            for (int i = 0; i < ACC; ++i) acc[n][m][i] = fmaf(gs[2 * m + (i >> 1)], grp[n][m][i], acc[n][m][i]);
+                } else {
+                    uint32_t grp[NT][2][4];
+#pragma unroll
+                    for (int b = 0; b < GROUP / 32; ++b) {
+                        const int blk = gi * (GROUP / 32) + b;
                         uint32_t f[2][4];
 #pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            f[m][0] = sub_bf16x2(nibbles(w[2 * m] >> (8 * h)), bias[2 * m]);
-                            f[m][1] = sub_bf16x2(nibbles(w[2 * m + 1] >> (8 * h)), bias[2 * m + 1]);
-                            f[m][2] = sub_bf16x2(nibbles(w[2 * m] >> (8 * h + 4)), bias[2 * m]);
-                            f[m][3] = sub_bf16x2(nibbles(w[2 * m + 1] >> (8 * h + 4)), bias[2 * m + 1]);
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t w = lds32((slot ^ (blk << 4)) + r * 1024);
+                            f[r >> 1][r & 1] = nibbles(w);
+                            f[r >> 1][2 + (r & 1)] = nibbles(w >> 4);
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            const uint2 q = fr[((blk * 2 + h) * NT + n) * 32];
-                            mma_bf16(grp[n][0], f[0], q.x, q.y);
-                            mma_bf16(grp[n][1], f[1], q.x, q.y);
+                            const uint2 q = fr[(blk * NT + n) * 32];
+                            if (b == 0) {
+                                const int2 d = starts[(gi * NT + n) * 4];
+                                uint32_t start[2][4];
+#pragma unroll
+                                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        start[m][i] = (uint32_t)(i & 1 ? d.y : d.x) -
+                                                      (ZERO ? (uint32_t)(zero[2 * m + (i >> 1)] * ((int)(MAGIC - (uint32_t)(i & 1 ? d.y : d.x)) >> 3)) : 0u);
+                                mma_u8s8(grp[n][0], f[0], q, start[0]);
+                                mma_u8s8(grp[n][1], f[1], q, start[1]);
+                            } else {
+                                mma_u8s8(grp[n][0], f[0], q, grp[n][0]);
+                                mma_u8s8(grp[n][1], f[1], q, grp[n][1]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float w = WIDE ? weight[(gi * NT + n) * 4] : 0.f;
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            float v[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(grp[n][m][i]) - MAGIC_F;
+#pragma unroll
+                            for (int i = 0; i < ACC; ++i) {
+                                if constexpr (WIDE)
+                                    acc[n][m][i] = fmaf(gs[2 * m + i], fmaf(v[2 * i], 256.f, v[2 * i + 1]) * w, acc[n][m][i]);
+                                else
+                                    acc[n][m][i] = fmaf(gs[2 * m + (i >> 1)], v[i], acc[n][m][i]);
+                            }
                         }
                     }
                 }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(gs[2 * m + (i >> 1)], grp[n][m][i], acc[n][m][i]);
             }
             __syncwarp();  // the slot is free: every lane has read it
             if (lane == 0 && left > 0) issue(s);
@@ -280,7 +440,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
                     for (int m = 0; m < 2; ++m)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) at[((n * 2 + m) * 4 + i) * 32] = acc[n][m][i];
+                        for (int i = 0; i < ACC; ++i) at[((n * 2 + m) * ACC + i) * 32] = acc[n][m][i];
             }
             asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(a.wk * 32) : "memory");
             if (part == 0) {
@@ -291,7 +451,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
                         for (int m = 0; m < 2; ++m)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[n][m][i] += from[((n * 2 + m) * 4 + i) * 32];
+                            for (int i = 0; i < ACC; ++i) acc[n][m][i] += from[((n * 2 + m) * ACC + i) * 32];
                 }
             }
             asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(a.wk * 32) : "memory");
@@ -303,20 +463,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int hi = 0; hi < 2; ++hi) {
-                        const int64_t row = row0 + g + 16 * m + 8 * hi;
-                        const float v0 = acc[n][m][2 * hi], v1 = acc[n][m][2 * hi + 1];
-                        if (a.x_dtype == VA_DTYPE_F32) {
-                            // Columns 4q..4q+3 are pieces of query q: lanes t = 0, 1 hold query 2n, t = 2, 3 query 2n + 1.
-                            float v = v0 + v1;
-                            v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+                        const int64_t row = (int64_t)tile * TR + g + 16 * m + 8 * hi;
+                        if constexpr (WIDE) {
+                            // Lanes t = 0, 1 hold query 2n (high and low digits), t = 2, 3 query 2n + 1.
+                            const float v = acc[n][m][hi] + __shfl_xor_sync(0xFFFFFFFFu, acc[n][m][hi], 1);
                             const int q = n * 2 + (t >> 1);
                             if ((t & 1) == 0 && row < a.n && q < a.nq) a.out[(int64_t)q * a.out_stride + row] = v;
                         } else {
-                            const int q = n * 8 + 2 * t;
-                            if (row < a.n) {
-                                if (q < a.nq) a.out[(int64_t)q * a.out_stride + row] = a.x_scales ? v0 * __ldg(a.x_scales + q) : v0;
-                                if (q + 1 < a.nq)
-                                    a.out[(int64_t)(q + 1) * a.out_stride + row] = a.x_scales ? v1 * __ldg(a.x_scales + q + 1) : v1;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const int q = n * 8 + 2 * t + i;
+                                if (row < a.n && q < a.nq)
+                                    a.out[(int64_t)q * a.out_stride + row] =
+                                        a.x_scales ? acc[n][m][2 * hi + i] * __ldg(a.x_scales + q) : acc[n][m][2 * hi + i];
                             }
                         }
                     }
@@ -332,28 +491,74 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 // Warps per block: what the registers allow (128 a thread at 16 warps).
 constexpr int warps_of(int nt) { return nt == 4 ? 8 : 16; }
 
-template <int NT, typename S, bool ZERO, int GROUP>
-int launch_matvec(va_context* ctx, const CUtensorMap& codes, const MatvecArgs& a, int grid, size_t smem) {
-    auto kern = k_int4_matvec<NT, warps_of(NT), S, ZERO, GROUP>;
-    VA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kern<<<grid, warps_of(NT) * 32, smem, ctx->stream>>>(codes, a, ctx->d_error, wait_limit_ns(ctx->timeout_ms));
+struct Launch {
+    CUtensorMap codes;
+    MatvecArgs a;
+    int group, scale_dtype, grid;
+    size_t smem;
+};
+
+template <int MODE, int NT, typename S, bool ZERO, int GROUP>
+int launch_matvec(va_context* ctx, const Launch& l) {
+    auto kern = k_int4_matvec<MODE, NT, warps_of(NT), S, ZERO, GROUP>;
+    VA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)l.smem));
+    kern<<<l.grid, warps_of(NT) * 32, l.smem, ctx->stream>>>(l.codes, l.a, ctx->d_error, wait_limit_ns(ctx->timeout_ms));
     return va_check_launch("k_int4_matvec");
 }
 
-template <int NT, typename S, bool ZERO>
-int launch_group(va_context* ctx, const CUtensorMap& codes, const MatvecArgs& a, int grid, size_t smem) {
-    if (a.group == 32) return launch_matvec<NT, S, ZERO, 32>(ctx, codes, a, grid, smem);
-    if (a.group == 64) return launch_matvec<NT, S, ZERO, 64>(ctx, codes, a, grid, smem);
-    return launch_matvec<NT, S, ZERO, 128>(ctx, codes, a, grid, smem);
+template <int MODE, int NT, typename S, bool ZERO>
+int launch_group(va_context* ctx, const Launch& l) {
+    if (l.group == 32) return launch_matvec<MODE, NT, S, ZERO, 32>(ctx, l);
+    if (l.group == 64) return launch_matvec<MODE, NT, S, ZERO, 64>(ctx, l);
+    return launch_matvec<MODE, NT, S, ZERO, 128>(ctx, l);
 }
 
-template <int NT>
-int launch_types(va_context* ctx, const CUtensorMap& codes, const MatvecArgs& a, int scale_dtype, int grid, size_t smem) {
-    if (scale_dtype == VA_DTYPE_BF16)
-        return a.zeros ? launch_group<NT, uint16_t, true>(ctx, codes, a, grid, smem)
-                       : launch_group<NT, uint16_t, false>(ctx, codes, a, grid, smem);
-    return a.zeros ? launch_group<NT, float, true>(ctx, codes, a, grid, smem)
-                   : launch_group<NT, float, false>(ctx, codes, a, grid, smem);
+template <int MODE, int NT>
+int launch_types(va_context* ctx, const Launch& l) {
+    if (l.scale_dtype == VA_DTYPE_BF16)
+        return l.a.zeros ? launch_group<MODE, NT, uint16_t, true>(ctx, l) : launch_group<MODE, NT, uint16_t, false>(ctx, l);
+    return l.a.zeros ? launch_group<MODE, NT, float, true>(ctx, l) : launch_group<MODE, NT, float, false>(ctx, l);
+}
+
+// A pass: its mode, column tiles and queries.
+struct Pass {
+    int mode, nt, nq;
+};
+
+// fp32 and bf16 queries: up to two as digits (one column tile), more as pieces, 8 queries a column tile; three
+// pieces of 8 queries leave the ring two slots up to 1536 dimensions, beyond which fp32 queries go as digits in up to
+// four column tiles. int8 queries: 8 a column tile, up to four. Two tiles of bf16 pieces take twice the memory
+// of one, which is left to the ring above 2048 dimensions.
+Pass pass_of(int x_dtype, int left, int chunks) {
+    if (x_dtype == VA_DTYPE_INT8) {
+        const int nt = left > 16 ? 4 : left > 8 ? 2 : 1;
+        return Pass{DIGITS_INT8, nt, std::min(left, nt * 8)};
+    }
+    if (left <= 2) return Pass{DIGITS_WIDE, 1, left};
+    if (x_dtype == VA_DTYPE_BF16) {
+        const int nt = left > 8 && chunks <= 8 ? 2 : 1;
+        return Pass{BF16, nt, std::min(left, nt * 8)};
+    }
+    if (chunks <= 6) return Pass{BF16X3, 1, std::min(left, 8)};
+    const int nt = left > 4 ? 4 : 2;
+    return Pass{DIGITS_WIDE, nt, std::min(left, nt * 2)};
+}
+
+int launch_pass(va_context* ctx, const Pass& p, const Launch& l) {
+    switch (p.mode) {
+        case DIGITS_INT8:
+            return p.nt == 1   ? launch_types<DIGITS_INT8, 1>(ctx, l)
+                   : p.nt == 2 ? launch_types<DIGITS_INT8, 2>(ctx, l)
+                               : launch_types<DIGITS_INT8, 4>(ctx, l);
+        case DIGITS_WIDE:
+            return p.nt == 1   ? launch_types<DIGITS_WIDE, 1>(ctx, l)
+                   : p.nt == 2 ? launch_types<DIGITS_WIDE, 2>(ctx, l)
+                               : launch_types<DIGITS_WIDE, 4>(ctx, l);
+        case BF16:
+            return p.nt == 1 ? launch_types<BF16, 1>(ctx, l) : launch_types<BF16, 2>(ctx, l);
+        default:
+            return launch_types<BF16X3, 1>(ctx, l);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -518,51 +723,50 @@ int va_int4_matvec(va_context* ctx, const void* x, int x_dtype, const float* x_s
 
     const auto enc = get_encode_fn();
     if (!enc) return va_set_error(VA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
-    CUtensorMap map;
+    Launch l{};
     const cuuint64_t dims[2] = {(cuuint64_t)VA_INT4_ROW_BYTES(dim), (cuuint64_t)n};
     const cuuint64_t strides[1] = {(cuuint64_t)VA_INT4_ROW_BYTES(dim)};
     const cuuint32_t box[2] = {128, TR}, estr[2] = {1, 1};
-    const CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, estr,
+    const CUresult r = enc(&l.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return va_set_error(VA_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
-
-    MatvecArgs a{};
+    l.group = group;
+    l.scale_dtype = scale_dtype;
+    MatvecArgs& a = l.a;
     a.scales = scales;
     a.zeros = zeros;
     a.n = n;
     a.out_stride = out_stride;
     a.row_tiles = (int)((n + TR - 1) / TR);
     a.dim = dim;
-    a.group = group;
     a.groups = (dim + group - 1) / group;
     a.x_dtype = x_dtype;
     a.chunks = (dim + CHUNK - 1) / CHUNK;
-    const int cols_per_query = x_dtype == VA_DTYPE_F32 ? 4 : 1;
-    for (int q0 = 0; q0 < nq;) {
-        // Column tiles of this pass: what the queries fill, within 64 KB of fragments (128 KB at 8 warps).
-        int nt = 1;
-        while (nt < MAX_NT && nt * 8 < (nq - q0) * cols_per_query && 2 * nt * a.chunks <= (nt == 2 ? 32 : 16)) nt *= 2;
-        a.nq = std::min(nq - q0, nt * 8 / cols_per_query);
+    l.grid = std::min(ctx->sm_count, a.row_tiles);
+    for (int q0 = 0; q0 < nq; q0 += a.nq) {
+        const Pass p = pass_of(x_dtype, nq - q0, a.chunks);
+        a.nq = p.nq;
         a.x = static_cast<const uint8_t*>(x) + (size_t)q0 * dim * es;
         a.x_scales = x_scales ? x_scales + q0 : nullptr;
         a.out = out + (int64_t)q0 * out_stride;
-        const int warps = warps_of(nt);
-        // Warps per row tile: more only while the row tiles leave warps of the grid idle.
-        a.wk = 1;
-        while (a.wk < 8 && a.wk * 2 <= a.chunks && (int64_t)a.row_tiles * a.wk * 2 <= (int64_t)ctx->sm_count * warps) a.wk *= 2;
-        const size_t frag = (size_t)a.chunks * 16 * nt * 32 * sizeof(uint2);
-        const size_t rest = 1024 + frag + 16 + (a.wk > 1 ? (size_t)warps * nt * 8 * 32 * 4 : 0);
+        // Warps per row tile: what leaves the busiest warp the least to do, a tile's end counted as half a chunk and a
+        // join as one and a half.
+        const int warps = warps_of(p.nt);
+        double best = 0;
+        for (int wk = 1; wk <= 8 && wk <= a.chunks; wk *= 2) {
+            const int64_t slots = (int64_t)l.grid * (warps / wk);
+            const double cost = (double)((a.row_tiles + slots - 1) / slots) * ((a.chunks + wk - 1) / wk + (wk > 1 ? 2.0 : 0.5));
+            if (wk == 1 || cost < best) {
+                best = cost;
+                a.wk = wk;
+            }
+        }
+        const size_t queries = (size_t)p.nt * a.chunks * (frag_bytes(p.mode) + (is_bf16(p.mode) ? 0 : CHUNK / group * (8 + 4) * 4));
+        const size_t rest = 1024 + queries + 16 + (a.wk > 1 ? (size_t)warps * p.nt * 8 * 32 * 4 : 0);
         a.ring = (int)std::min<size_t>(6, (227 * 1024 - rest) / (warps * (SLOT + 8)));
-        const size_t smem = rest + (size_t)a.ring * warps * (SLOT + 8);
-        const int grid = std::min(ctx->sm_count, a.row_tiles);
-        if (nt == 1)
-            VA_TRY(launch_types<1>(ctx, map, a, scale_dtype, grid, smem));
-        else if (nt == 2)
-            VA_TRY(launch_types<2>(ctx, map, a, scale_dtype, grid, smem));
-        else
-            VA_TRY(launch_types<4>(ctx, map, a, scale_dtype, grid, smem));
-        q0 += a.nq;
+        l.smem = rest + (size_t)a.ring * warps * (SLOT + 8);
+        VA_TRY(launch_pass(ctx, p, l));
     }
     return VA_OK;
 }
