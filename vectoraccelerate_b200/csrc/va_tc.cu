@@ -659,59 +659,6 @@ constexpr int PB_BYTES = P_ROWS * BKB;       // 16 KB of database rows
 constexpr int PSTAGE_BYTES = PA_BYTES + PB_BYTES;
 constexpr int PBM = 256;                     // queries per pair tile
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_index() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_count() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%nclusterid.x;" : "=r"(r));
-    return r;
-}
-// Address of the same shared-memory location in CTA `rank` of this cluster.
-__device__ __forceinline__ uint32_t map_rank(uint32_t smem_addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int c0,
-                                                 int c1) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
-        "[%2];" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(bar_cluster_addr), "r"(c0), "r"(c1)
-        : "memory");
-}
-__device__ __forceinline__ void mma_commit_pair(uint32_t bar_cluster_addr) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster_addr)
-                 : "memory");
-}
-// An abort in one CTA of a pair stops both: its flag is also set in the peer CTA.
-__device__ __forceinline__ void abort_peer(volatile int* s_abort, uint32_t rank) {
-    *s_abort = 1;
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_rank(smem_u32((const void*)s_abort), rank ^ 1u)), "r"(1)
-                 : "memory");
-}
-// Teardown of a pair after an abort: a CTA's TMA loads signal the leader's barriers, so the peer
-// cannot wait for its own loads; both CTAs let in-flight copies land (a fixed settle time, far
-// above a copy's latency) before the cluster barrier that precedes TMEM release and exit.
-__device__ __forceinline__ void settle_ns(uint64_t ns) {
-    const uint64_t t0 = va::globaltimer_ns();
-    while (va::globaltimer_ns() - t0 < ns) __nanosleep(1000);
-}
-
 template <int ELEM>
 struct PairKind;
 template <>

@@ -6,17 +6,21 @@
 //   G_tv = c g_t (exp(z_tv - lse_t) - [v = label_t])           dh = G w        dw = G^T h
 // with g_t the gradient of loss_t. A token whose label is outside [0, V) has no loss: loss 0, G row 0.
 //
-// Forward, 2TVD operations: k_xent_scores<FORWARD> walks 128-token x 256-row tiles (TMA ring, one
-// thread issuing tcgen05.mma, two TMEM accumulators) and its epilogue keeps each token's running
-// maximum and sum of exponentials (in powers of two) in registers; the partial pairs of the row splits
-// are joined by k_xent_join, which also forms the label's logit.
+// Forward, 2TVD operations: k_xent_scores<FORWARD> walks tiles of tokens x 256 rows (TMA ring, one thread issuing
+// tcgen05.mma, two TMEM accumulators) and its epilogue keeps each token's running maximum and sum of
+// exponentials (in powers of two) in registers; the partial pairs of the row splits are joined by k_xent_join, which
+// also forms the label's logit.
 // Backward, 6TVD: the table is taken in chunks of rows so that G of a chunk (bf16) is at most 256 MB.
 // k_xent_scores<GRADIENT> recomputes the chunk's logits and stores G; k_xent_grads multiplies it both
 // ways, with operands that are contiguous along the wrong axis read as MN-major tiles instead of being
 // transposed in memory: dw tiles (M = rows, K = tokens) are finished in one go; dh tiles (M = tokens, K = the
 // chunk's rows) add into an fp32 buffer per K split, which k_xent_finish sums and rounds.
-// Both directions are compute-bound once T and V pass a few hundred: the tensor pipe is the limit and
-// the exponentials (16 per clock and SM) hide behind it above D = 256.
+// Both directions are compute-bound once T and V pass a few hundred: the tensor pipe and its operand feed are the
+// limit, and the exponentials (16 per clock and SM) hide behind it above D = 256.
+//
+// Tiles: a CTA's 128 x 256 tile takes 48 KB of operands per 64 of K, more than shared memory and L2 feed at the
+// full rate; a pair of CTAs (cta_group::2) works on 256 x 256 and loads 32 KB each. Pairs serve problems that
+// fill the GPU with 128-row tiles twice over; smaller ones keep single CTAs, which spread wider (PAIR_TIMES).
 //
 // Roundings: G to bf16 once (its products with w and h are summed in fp32, so the error of a gradient
 // stays near that of its own rounding to bf16); everything else fp32. All orders of summation are fixed.
@@ -29,56 +33,117 @@ namespace {
 
 using namespace va::tc;
 
-constexpr int BM = 128;                   // tile rows (TMEM lanes)
+constexpr int BM = 128;                   // tile rows of a CTA (TMEM lanes)
 constexpr int BN = 256;                   // columns of an accumulator
 constexpr int BK = 64;                    // elements of K per stage (128 bytes)
 constexpr int BOX = 64 * 128;             // bytes of a 64-row box of 128-byte rows
 constexpr int A_BYTES = 2 * BOX;
-constexpr int B_BYTES = 4 * BOX;
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int STAGES = 4;
+constexpr int RING_BYTES = 4 * 6 * BOX;   // 4 stages of 6 boxes, or 6 stages of 4 (pairs)
 constexpr int EPI_BYTES = 32 * 128;       // one staged 32-row x 128-byte piece of an epilogue warp
 constexpr int THREADS = 192;              // TMA warp, MMA warp, four epilogue warps
 constexpr int TMEM_COLS = 512;
-constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 4 * 2 * EPI_BYTES + (2 * STAGES + 5) * 8 + 16;
+constexpr size_t SMEM = 1024 + RING_BYTES + 4 * 2 * EPI_BYTES + (2 * 6 + 5) * 8 + 16;
 constexpr int64_t G_ENTRIES = 1 << 27;    // gradient entries of a chunk (256 MB of bf16)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
-enum { FORWARD = 0, GRADIENT = 1 };
-
-// Per token of the backward pass: lse in powers of two, c * g (0: no loss) and the label.
-struct TokenGrad {
-    float lse2, scale;
-    int64_t label;
+template <bool PAIR>
+struct Tile {
+    static constexpr int CTAS = PAIR ? 2 : 1;
+    static constexpr int M = CTAS * BM;
+    static constexpr int STAGES = PAIR ? 6 : 4;
+    static constexpr int B_BYTES = (PAIR ? 2 : 4) * BOX;  // a CTA's share of B at the full width
 };
 
+enum { FORWARD = 0, GRADIENT = 1 };
+
+// Per token of the backward pass: lse in powers of two, c * g (0: no loss), log2 |c g| - lse2 and the label.
+struct TokenGrad {
+    float lse2, scale, shift;
+    int label;
+};
+
+// What the roles of a CTA share. In a pair, CTA 0 leads: its full barriers count both CTAs' bytes, it issues the
+// MMAs, and its tempty barriers collect both CTAs' epilogue warps; empty and tfull are signalled in both CTAs.
+template <bool PAIR>
 struct Roles {
     uint8_t *sA, *sB, *sE;
     uint64_t *full, *empty, *tfull, *tempty, *dbar;
     volatile int* abort_flag;
     uint32_t tmem;
+    uint32_t rank;      // in the pair
+    int worker, workers;
+
+    __device__ __forceinline__ bool leader() const { return !PAIR || rank == 0; }
+    // A bounded wait; one that expires stops the other CTA of the pair too.
+    __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, uint64_t limit_ns) const {
+        if (mbar_wait(bar, parity, abort_flag, err, limit_ns)) return true;
+        if constexpr (PAIR) abort_peer(abort_flag, rank);
+        return false;
+    }
+    // Arms stage s for `bytes` of each CTA.
+    __device__ __forceinline__ void arm(int s, uint32_t bytes) const {
+        if (leader()) mbar_expect_tx(&full[s], bytes * Tile<PAIR>::CTAS);
+    }
+    __device__ __forceinline__ void load(int s, void* dst, const CUtensorMap* map, int c0, int c1) const {
+        if constexpr (PAIR)
+            tma_load_2d_pair(dst, map, map_rank(smem_u32(&full[s]), 0), c0, c1);
+        else
+            tma_load_2d(dst, map, &full[s], c0, c1);
+    }
+    // Signals a barrier of every CTA once the MMAs issued so far are done.
+    __device__ __forceinline__ void commit(uint64_t* bar) const {
+        if constexpr (PAIR) {
+            mma_commit_pair(map_rank(smem_u32(bar), 0));
+            mma_commit_pair(map_rank(smem_u32(bar), 1));
+        } else {
+            mma_commit(bar);
+        }
+    }
+    // After an abort, before the CTAs rejoin: copies in flight have landed, MMAs issued are done.
+    __device__ __forceinline__ void settle_loads(uint32_t issued) const {
+        if (!*abort_flag) return;
+        if (leader()) drain_loads(full, Tile<PAIR>::STAGES, issued);
+        if constexpr (PAIR) settle_ns(1000000ull);
+    }
+    __device__ __forceinline__ void settle_mmas() const {
+        if (!*abort_flag) return;
+        if constexpr (PAIR)
+            mma_commit_pair(map_rank(smem_u32(dbar), 0));
+        else
+            mma_commit(dbar);
+        mbar_drain(dbar, 0u, kDrainLimitNs);
+    }
 };
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    // (.ftz: terms below 2^-126 of the largest count as zero)
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(a), "l"(b), "r"(idesc), "r"(acc));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
 
-// Instruction descriptor: fp32 accumulator, bf16 operands, M = 128, N columns; an operand is K-major (0)
+// Instruction descriptor: fp32 accumulator, bf16 operands, M rows, N columns; an operand is K-major (0)
 // or MN-major (1).
-__host__ __device__ constexpr uint32_t idesc_of(int n, int a_mn, int b_mn) {
+__host__ __device__ constexpr uint32_t idesc_of(int m, int n, int a_mn, int b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 // MN-major operand, 128B swizzle: boxes of 64 (MN) x 64 (K), 128 bytes per K row. Groups of 8 K rows are
@@ -111,12 +176,14 @@ __device__ __forceinline__ void bulk_wait_read() {
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Shared set-up of the two kernels: barriers, TMEM.
-__device__ __forceinline__ Roles set_up(uint8_t* smem_raw) {
-    Roles r;
+template <bool PAIR>
+__device__ __forceinline__ Roles<PAIR> set_up(uint8_t* smem_raw) {
+    constexpr int STAGES = Tile<PAIR>::STAGES;
+    Roles<PAIR> r;
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     r.sA = smem;
     r.sB = smem + (size_t)STAGES * A_BYTES;
-    r.sE = r.sB + (size_t)STAGES * B_BYTES;
+    r.sE = smem + RING_BYTES;
     r.full = (uint64_t*)(r.sE + 4 * 2 * EPI_BYTES);
     r.empty = r.full + STAGES;
     r.tfull = r.empty + STAGES;
@@ -124,6 +191,9 @@ __device__ __forceinline__ Roles set_up(uint8_t* smem_raw) {
     r.dbar = r.tempty + 2;
     uint32_t* s_tmem = (uint32_t*)(r.dbar + 1);
     r.abort_flag = (volatile int*)(s_tmem + 1);
+    r.rank = PAIR ? cluster_rank() : 0u;
+    r.worker = PAIR ? (int)cluster_index() : (int)blockIdx.x;
+    r.workers = PAIR ? (int)cluster_count() : (int)gridDim.x;
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&r.full[s], 1);
@@ -131,16 +201,24 @@ __device__ __forceinline__ Roles set_up(uint8_t* smem_raw) {
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&r.tfull[b], 1);
-            mbar_init(&r.tempty[b], 4);
+            mbar_init(&r.tempty[b], 4 * Tile<PAIR>::CTAS);
         }
         mbar_init(r.dbar, 1);
         *r.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // Both CTAs' barriers exist before either CTA signals the other's.
+    if constexpr (PAIR) cluster_sync();
     if (threadIdx.x >> 5 == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
-                     "r"(TMEM_COLS));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
+                         "r"(TMEM_COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
+                         "r"(TMEM_COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -149,36 +227,49 @@ __device__ __forceinline__ Roles set_up(uint8_t* smem_raw) {
     return r;
 }
 
-// Every role rejoins; TMEM is freed after the last read and the last MMA.
-__device__ __forceinline__ void tear_down(const Roles& r) {
+// Every role of every CTA rejoins; TMEM is freed after the last read and the last MMA.
+template <bool PAIR>
+__device__ __forceinline__ void tear_down(const Roles<PAIR>& r) {
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();
     if (threadIdx.x >> 5 == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(r.tmem), "r"(TMEM_COLS));
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(r.tmem), "r"(TMEM_COLS));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(r.tmem), "r"(TMEM_COLS));
     }
 }
 
 // A ring position shared by the producer and the MMA issuer.
+template <bool PAIR>
 struct Ring {
     uint32_t it = 0;
-    __device__ __forceinline__ int slot() const { return (int)(it % STAGES); }
-    __device__ __forceinline__ uint32_t phase() const { return (it / STAGES) & 1u; }
+    __device__ __forceinline__ int slot() const { return (int)(it % Tile<PAIR>::STAGES); }
+    __device__ __forceinline__ uint32_t phase() const { return (it / Tile<PAIR>::STAGES) & 1u; }
 };
 
 // Waits for accumulator `tile`; the whole warp follows lane 0's verdict.
-__device__ __forceinline__ bool wait_accumulator(const Roles& r, uint32_t tile, int lane, int* err, uint64_t limit_ns) {
+template <bool PAIR>
+__device__ __forceinline__ bool wait_accumulator(const Roles<PAIR>& r, uint32_t tile, int lane, int* err, uint64_t limit_ns) {
     int ok = 1;
-    if (lane == 0) ok = mbar_wait(&r.tfull[tile & 1u], (tile >> 1) & 1u, r.abort_flag, err, limit_ns) ? 1 : 0;
+    if (lane == 0) ok = r.wait(&r.tfull[tile & 1u], (tile >> 1) & 1u, err, limit_ns) ? 1 : 0;
     ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
     tc_fence_after();
     return ok != 0;
 }
-__device__ __forceinline__ void release_accumulator(const Roles& r, uint32_t tile, int lane) {
+template <bool PAIR>
+__device__ __forceinline__ void release_accumulator(const Roles<PAIR>& r, uint32_t tile, int lane) {
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&r.tempty[tile & 1u]);
+    if (lane == 0) {
+        if constexpr (PAIR)
+            mbar_arrive_remote(map_rank(smem_u32(&r.tempty[tile & 1u]), 0));
+        else
+            mbar_arrive(&r.tempty[tile & 1u]);
+    }
 }
 
 // One lane's 128 bytes of a staged piece: row `lane` of 32, 16-byte units in the 128B swizzle order.
@@ -193,8 +284,9 @@ struct ScoreWork {
     int64_t tokens, rows;  // rows: of this launch (the whole table, or one chunk), from row0
     int64_t row0;
     int token_tiles, row_tiles, splits, k_blocks;
+    int n;                 // table rows of a tile: 256, or 128 (single CTAs)
     float scale2;          // c * log2(e)
-    float2* part;          // forward: (maximum, sum) per [split][token_tiles * 128]
+    float2* part;          // forward: (maximum, sum) per [split][token_tiles * tile rows]
     const TokenGrad* tok;  // gradient
 };
 
@@ -229,153 +321,150 @@ __device__ __forceinline__ void lse_chunk(uint32_t (&r)[64], float scale2, int v
     sum += (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-// Gradient entries of 64 columns of a token, staged as 128 bytes of bf16. `label` is the label's
-// column in the chunk (outside [0, 64): not here).
-__device__ __forceinline__ void grad_chunk(const uint32_t (&r)[64], float scale2, float lse2, float scale, int label,
-                                           uint8_t* piece, int lane) {
-    const bool here = (unsigned)label < 64u;
-    const bool any = __any_sync(0xFFFFFFFFu, here);
+// Gradient entries c g p of 64 columns of a token, staged as 128 bytes of bf16: |c g| is part of the exponent, its
+// sign (and the zeros of a token without loss, whatever its logits are) are put on the bits. `label` is the label's
+// column in the chunk (outside [0, 64): not here); its entry c g (p - 1) is formed in fp32 and replaces the staged one.
+__device__ __forceinline__ void grad_chunk(const uint32_t (&r)[64], float scale2, const TokenGrad& tg, int label, uint8_t* piece,
+                                           int lane) {
+    const uint32_t keep = tg.scale == 0.f ? 0u : 0xFFFFFFFFu, sign = tg.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
         uint32_t p[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            float v[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int i = u * 8 + k * 2 + e;
-                // a token without loss has exact zeros, whatever its logits are
-                v[e] = scale == 0.f ? 0.f : ex2(fmaf(__uint_as_float(r[i]), scale2, -lse2)) * scale;
-                if (any && label == i) v[e] -= scale;
-            }
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[k]) : "f"(v[1]), "f"(v[0]));
+            const float lo = ex2(fmaf(__uint_as_float(r[u * 8 + k * 2]), scale2, tg.shift));
+            const float hi = ex2(fmaf(__uint_as_float(r[u * 8 + k * 2 + 1]), scale2, tg.shift));
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[k]) : "f"(hi), "f"(lo));
+            p[k] = (p[k] & keep) ^ sign;
         }
         stage_unit(piece, lane, u, make_uint4(p[0], p[1], p[2], p[3]));
     }
+    if ((unsigned)label < 64u) {
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+            if (i == label) z = __uint_as_float(r[i]);
+        const float g = (ex2(fmaf(z, scale2, -tg.lse2)) - 1.f) * tg.scale;
+        *reinterpret_cast<uint16_t*>(piece + lane * 128 + ((((unsigned)label >> 3) ^ (lane & 7)) << 4) + (label & 7) * 2) =
+            va::f2bf_rn(g);
+    }
 }
 
-template <int MODE>
+template <int MODE, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
     k_xent_scores(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
                   const __grid_constant__ CUtensorMap map_g, ScoreWork w, int* err, uint64_t limit_ns) {
     extern __shared__ uint8_t smem_raw[];
-    const Roles r = set_up(smem_raw);
+    const Roles<PAIR> r = set_up<PAIR>(smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n_items = w.token_tiles * w.splits;
+    constexpr int TM = Tile<PAIR>::M;
+    const int share = w.n / Tile<PAIR>::CTAS;  // table rows of a tile that this CTA loads
     int tt, split, r0, r1;
 
     if (warp == 0) {
         if (lane == 0) {
-            Ring ring;
-            for (int item = blockIdx.x; item < n_items && !*r.abort_flag; item += gridDim.x) {
+            Ring<PAIR> ring;
+            for (int item = r.worker; item < n_items && !*r.abort_flag; item += r.workers) {
                 score_item(w, item, tt, split, r0, r1);
                 for (int t = r0; t < r1; ++t)
                     for (int kb = 0; kb < w.k_blocks; ++kb, ++ring.it) {
                         const int s = ring.slot();
-                        if (!mbar_wait(&r.empty[s], ring.phase() ^ 1u, r.abort_flag, err, limit_ns)) goto loads_done;
-                        mbar_expect_tx(&r.full[s], STAGE_BYTES);
-                        tma_load_2d(r.sA + (size_t)s * A_BYTES, &map_h, &r.full[s], kb * BK, tt * BM);
-                        tma_load_2d(r.sB + (size_t)s * B_BYTES, &map_w, &r.full[s], kb * BK, (int)(w.row0 + (int64_t)t * BN));
+                        if (!r.wait(&r.empty[s], ring.phase() ^ 1u, err, limit_ns)) goto loads_done;
+                        r.arm(s, A_BYTES + share * 128);
+                        r.load(s, r.sA + (size_t)s * A_BYTES, &map_h, kb * BK, tt * TM + (int)r.rank * BM);
+                        r.load(s, r.sB + (size_t)s * Tile<PAIR>::B_BYTES, &map_w, kb * BK,
+                               (int)(w.row0 + (int64_t)t * w.n) + (int)r.rank * share);
                     }
             }
         loads_done:
-            if (*r.abort_flag) drain_loads(r.full, STAGES, ring.it);
+            r.settle_loads(ring.it);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            Ring ring;
+        if (lane == 0 && r.leader()) {
+            Ring<PAIR> ring;
             uint32_t tile = 0;
-            constexpr uint32_t idesc = idesc_of(BN, 0, 0);
-            for (int item = blockIdx.x; item < n_items && !*r.abort_flag; item += gridDim.x) {
+            const uint32_t idesc = idesc_of(TM, w.n, 0, 0);
+            for (int item = r.worker; item < n_items && !*r.abort_flag; item += r.workers) {
                 score_item(w, item, tt, split, r0, r1);
                 for (int t = r0; t < r1; ++t, ++tile) {
-                    if (!mbar_wait(&r.tempty[tile & 1u], ((tile >> 1) & 1u) ^ 1u, r.abort_flag, err, limit_ns)) goto mma_done;
+                    if (!r.wait(&r.tempty[tile & 1u], ((tile >> 1) & 1u) ^ 1u, err, limit_ns)) goto mma_done;
                     tc_fence_after();
                     const uint32_t d = r.tmem + (tile & 1u) * BN;
                     for (int kb = 0; kb < w.k_blocks; ++kb, ++ring.it) {
                         const int s = ring.slot();
-                        if (!mbar_wait(&r.full[s], ring.phase(), r.abort_flag, err, limit_ns)) goto mma_done;
+                        if (!r.wait(&r.full[s], ring.phase(), err, limit_ns)) goto mma_done;
                         tc_fence_after();
-                        const uint32_t a0 = smem_u32(r.sA + (size_t)s * A_BYTES), b0 = smem_u32(r.sB + (size_t)s * B_BYTES);
+                        const uint32_t a0 = smem_u32(r.sA + (size_t)s * A_BYTES), b0 = smem_u32(r.sB + (size_t)s * Tile<PAIR>::B_BYTES);
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            mma_f16(d, smem_desc(a0 + 32 * j), smem_desc(b0 + 32 * j), idesc, (kb | j) ? 1u : 0u);
-                        mma_commit(&r.empty[s]);
+                            mma_f16<PAIR>(d, smem_desc(a0 + 32 * j), smem_desc(b0 + 32 * j), idesc, (kb | j) ? 1u : 0u);
+                        r.commit(&r.empty[s]);
                     }
-                    mma_commit(&r.tfull[tile & 1u]);
+                    r.commit(&r.tfull[tile & 1u]);
                 }
             }
         mma_done:
-            if (*r.abort_flag) {
-                mma_commit(r.dbar);
-                mbar_drain(r.dbar, 0u, kDrainLimitNs);
-            }
+            r.settle_mmas();
         }
     } else {
-        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const int quarter = warp & 3;
         uint8_t* piece = r.sE + (size_t)quarter * 2 * EPI_BYTES;
         uint32_t tile = 0;
-        for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+        for (int item = r.worker; item < n_items; item += r.workers) {
             score_item(w, item, tt, split, r0, r1);
-            const int64_t token = (int64_t)tt * BM + row;
+            const int64_t token0 = (int64_t)tt * TM + r.rank * BM + quarter * 32, token = token0 + lane;
             float top = -INFINITY, nb = 0.f, sum = 0.f;
-            TokenGrad tg{0.f, 0.f, -1};
+            TokenGrad tg{0.f, 0.f, 0.f, -1};
             if constexpr (MODE == GRADIENT) {
                 if (token < w.tokens) tg = w.tok[token];
             }
             for (int t = r0; t < r1; ++t, ++tile) {
                 if (!wait_accumulator(r, tile, lane, err, limit_ns)) goto epilogue_done;
                 const uint32_t at = r.tmem + ((uint32_t)(quarter * 32) << 16) + (tile & 1u) * BN;
-                const int64_t col0 = (int64_t)t * BN;
-                const int valid = (int)min((int64_t)BN, w.rows - col0);
-                uint32_t ra[64], rb[64];
-                if constexpr (MODE == FORWARD) {
-                    tmem_ld64(at, ra);
-                    tmem_wait64(ra);
-                    tmem_ld64(at + 64, rb);
-                    lse_chunk(ra, w.scale2, valid, top, nb, sum);
-                    tmem_wait64(rb);
-                    tmem_ld64(at + 128, ra);
-                    lse_chunk(rb, w.scale2, valid - 64, top, nb, sum);
-                    tmem_wait64(ra);
-                    tmem_ld64(at + 192, rb);
-                    lse_chunk(ra, w.scale2, valid - 128, top, nb, sum);
-                    tmem_wait64(rb);
-                    release_accumulator(r, tile, lane);
-                    lse_chunk(rb, w.scale2, valid - 192, top, nb, sum);
-                } else {
-                    const int64_t lab = tg.label - w.row0 - col0;
-                    const int label = lab >= 0 && lab < BN ? (int)lab : -BN;
-                    const int64_t token0 = (int64_t)tt * BM + quarter * 32;
-                    auto put = [&](int c, const uint32_t(&v)[64]) {
+                const int64_t col0 = (int64_t)t * w.n;
+                const int valid = (int)min((int64_t)w.n, w.rows - col0);
+                int64_t label = -1;
+                if constexpr (MODE == GRADIENT) label = (int64_t)tg.label - w.row0 - col0;
+                // 64 columns at a time, the next ones on their way from TMEM meanwhile.
+                const auto use = [&](int c, uint32_t(&v)[64]) {
+                    if constexpr (MODE == FORWARD) {
+                        lse_chunk(v, w.scale2, valid - 64 * c, top, nb, sum);
+                    } else {
                         uint8_t* p = piece + (c & 1) * EPI_BYTES;
                         // the store that last used this piece has read it
                         if (lane == 0) bulk_wait_read<1>();
                         __syncwarp();
-                        grad_chunk(v, w.scale2, tg.lse2, tg.scale, label - 64 * c, p, lane);
+                        grad_chunk(v, w.scale2, tg, (int)max(min(label, (int64_t)BN) - 64 * c, (int64_t)-1), p, lane);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) {
-                            if (token0 < w.tokens && col0 + 64 * c < w.rows) tma_store_2d(&map_g, p, (int)(col0 + 64 * c), (int)token0);
+                            if (token0 < w.tokens && 64 * c < valid) tma_store_2d(&map_g, p, (int)(col0 + 64 * c), (int)token0);
                             bulk_commit();
                         }
-                    };
-                    tmem_ld64(at, ra);
-                    tmem_wait64(ra);
-                    tmem_ld64(at + 64, rb);
-                    put(0, ra);
-                    tmem_wait64(rb);
+                    }
+                };
+                uint32_t ra[64], rb[64];
+                tmem_ld64(at, ra);
+                tmem_wait64(ra);
+                tmem_ld64(at + 64, rb);
+                use(0, ra);
+                tmem_wait64(rb);
+                if (w.n > 128) {
                     tmem_ld64(at + 128, ra);
-                    put(1, rb);
+                    use(1, rb);
                     tmem_wait64(ra);
                     tmem_ld64(at + 192, rb);
-                    put(2, ra);
+                    use(2, ra);
                     tmem_wait64(rb);
                     release_accumulator(r, tile, lane);
-                    put(3, rb);
+                    use(3, rb);
+                } else {
+                    release_accumulator(r, tile, lane);
+                    use(1, rb);
                 }
             }
-            if constexpr (MODE == FORWARD) w.part[(int64_t)split * w.token_tiles * BM + token] = make_float2(-nb, sum);
+            if constexpr (MODE == FORWARD) w.part[(int64_t)split * w.token_tiles * TM + token] = make_float2(-nb, sum);
         }
     epilogue_done:
         if (MODE == GRADIENT && lane == 0) bulk_wait_all();
@@ -387,26 +476,26 @@ __global__ void __launch_bounds__(THREADS, 1)
 // The two products of a chunk's G
 // ------------------------------------------------------------------------------------------------
 // Items: n_h = token_tiles * d_tiles * splits of dh (K = a split of the chunk's rows) and n_w = row_tiles *
-// d_tiles of dw (K = the tokens).
+// d_tiles of dw (K = the tokens). A worker is a CTA or a pair.
 struct GradWork {
     int64_t row0;           // first table row of the chunk
     int64_t rows;           // rows of the whole table
     int dim;
-    int64_t tokens_pad;     // token_tiles * 128: rows of one split's dh buffer
+    int64_t tokens_pad;     // token_tiles * tile rows: of one split's dh buffer
     int token_tiles, row_tiles, d_tiles, splits;
-    int n;                  // columns of a tile: 64, 128, 192 or 256
+    int n;                  // columns of a tile: 64, 128, 192 or 256 (pairs: 128 or 256)
     int kb_rows, kb_tokens; // K blocks of 64: chunk rows, tokens
     int first;              // first chunk: dh is stored, else added
     int long_h;             // dh items are the longer ones and go out first
-    int extra;              // shorter items given first to the blocks that got one longer item less
+    int extra;              // shorter items given first to the workers that got one longer item less
 };
 
-// The k-th item of this block, or -1. The longer items go round the blocks first; then `extra` shorter
-// ones to each block left with one longer item less (as many as make up for it), then the rest to all.
-__device__ __forceinline__ int grad_item(const GradWork& w, int k, bool& is_h) {
+// The k-th item of worker b, or -1. The longer items go round the workers first; then `extra` shorter
+// ones to each worker left with one longer item less (as many as make up for it), then the rest to all.
+__device__ __forceinline__ int grad_item(const GradWork& w, int b, int grid, int k, bool& is_h) {
     const int n_h = w.token_tiles * w.d_tiles * w.splits, n_w = w.row_tiles * w.d_tiles;
     const int n_long = w.long_h ? n_h : n_w, n_short = w.long_h ? n_w : n_h;
-    const int grid = gridDim.x, b = blockIdx.x, over = n_long % grid;
+    const int over = n_long % grid;
     const int longs = n_long / grid + (b < over ? 1 : 0);
     if (k < longs) {
         is_h = w.long_h;
@@ -414,7 +503,7 @@ __device__ __forceinline__ int grad_item(const GradWork& w, int k, bool& is_h) {
     }
     is_h = !w.long_h;
     k -= longs;
-    const int late = over ? grid - over : 0;  // blocks with one longer item less
+    const int late = over ? grid - over : 0;  // workers with one longer item less
     const int given = min(late * w.extra, n_short);
     if (b >= over && late) {
         const int j = (b - over) + k * late;
@@ -449,90 +538,88 @@ __device__ __forceinline__ GradTile grad_tile(const GradWork& w, int item, bool 
     return t;
 }
 
+template <bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
     k_xent_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_w,
                  const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_dh,
                  const __grid_constant__ CUtensorMap map_dw, GradWork w, int* err, uint64_t limit_ns) {
     extern __shared__ uint8_t smem_raw[];
-    const Roles r = set_up(smem_raw);
+    const Roles<PAIR> r = set_up<PAIR>(smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int boxes = w.n / 64;
+    constexpr int TM = Tile<PAIR>::M;
+    const int boxes = w.n / 64 / Tile<PAIR>::CTAS;  // of B that this CTA loads
     bool is_h;
 
     if (warp == 0) {
         if (lane == 0) {
-            Ring ring;
-            for (int k = 0, item; (item = grad_item(w, k, is_h)) >= 0 && !*r.abort_flag; ++k) {
+            Ring<PAIR> ring;
+            for (int k = 0, item; (item = grad_item(w, r.worker, r.workers, k, is_h)) >= 0 && !*r.abort_flag; ++k) {
                 const GradTile t = grad_tile(w, item, is_h);
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++ring.it) {
                     const int s = ring.slot();
-                    if (!mbar_wait(&r.empty[s], ring.phase() ^ 1u, r.abort_flag, err, limit_ns)) goto loads_done;
-                    mbar_expect_tx(&r.full[s], (2 + boxes) * BOX);
+                    if (!r.wait(&r.empty[s], ring.phase() ^ 1u, err, limit_ns)) goto loads_done;
+                    r.arm(s, (2 + boxes) * BOX);
                     uint8_t* a = r.sA + (size_t)s * A_BYTES;
-                    uint8_t* b = r.sB + (size_t)s * B_BYTES;
+                    uint8_t* b = r.sB + (size_t)s * Tile<PAIR>::B_BYTES;
+                    const int m0 = t.m * TM + (int)r.rank * BM, d0 = t.d * w.n + (int)r.rank * boxes * 64;
                     if (is_h) {
-                        // A: 128 tokens x 64 chunk rows of G. B: 64 table rows x n columns.
-                        for (int i = 0; i < 2; ++i) tma_load_2d(a + i * BOX, &map_g, &r.full[s], kb * BK, t.m * BM + i * 64);
-                        for (int i = 0; i < boxes; ++i)
-                            tma_load_2d(b + i * BOX, &map_w, &r.full[s], t.d * w.n + i * 64, (int)(w.row0 + kb * BK));
+                        // A: 128 tokens x 64 chunk rows of G. B: 64 table rows x this CTA's columns.
+                        for (int i = 0; i < 2; ++i) r.load(s, a + i * BOX, &map_g, kb * BK, m0 + i * 64);
+                        for (int i = 0; i < boxes; ++i) r.load(s, b + i * BOX, &map_w, d0 + i * 64, (int)(w.row0 + kb * BK));
                     } else {
-                        // A: 64 tokens x 128 chunk rows of G. B: 64 tokens x n columns.
-                        for (int i = 0; i < 2; ++i) tma_load_2d(a + i * BOX, &map_g, &r.full[s], t.m * BM + i * 64, kb * BK);
-                        for (int i = 0; i < boxes; ++i)
-                            tma_load_2d(b + i * BOX, &map_h, &r.full[s], t.d * w.n + i * 64, kb * BK);
+                        // A: 64 tokens x 128 chunk rows of G. B: 64 tokens x this CTA's columns.
+                        for (int i = 0; i < 2; ++i) r.load(s, a + i * BOX, &map_g, m0 + i * 64, kb * BK);
+                        for (int i = 0; i < boxes; ++i) r.load(s, b + i * BOX, &map_h, d0 + i * 64, kb * BK);
                     }
                 }
             }
         loads_done:
-            if (*r.abort_flag) drain_loads(r.full, STAGES, ring.it);
+            r.settle_loads(ring.it);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            Ring ring;
+        if (lane == 0 && r.leader()) {
+            Ring<PAIR> ring;
             uint32_t tile = 0;
-            for (int k = 0, item; (item = grad_item(w, k, is_h)) >= 0 && !*r.abort_flag; ++k) {
+            for (int k = 0, item; (item = grad_item(w, r.worker, r.workers, k, is_h)) >= 0 && !*r.abort_flag; ++k) {
                 const GradTile t = grad_tile(w, item, is_h);
                 if (t.kb0 >= t.kb1) continue;
-                if (!mbar_wait(&r.tempty[tile & 1u], ((tile >> 1) & 1u) ^ 1u, r.abort_flag, err, limit_ns)) goto mma_done;
+                if (!r.wait(&r.tempty[tile & 1u], ((tile >> 1) & 1u) ^ 1u, err, limit_ns)) goto mma_done;
                 tc_fence_after();
                 const uint32_t d = r.tmem + (tile & 1u) * BN;
-                const uint32_t idesc = idesc_of(w.n, is_h ? 0 : 1, 1);
+                const uint32_t idesc = idesc_of(TM, w.n, is_h ? 0 : 1, 1);
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++ring.it) {
                     const int s = ring.slot();
-                    if (!mbar_wait(&r.full[s], ring.phase(), r.abort_flag, err, limit_ns)) goto mma_done;
+                    if (!r.wait(&r.full[s], ring.phase(), err, limit_ns)) goto mma_done;
                     tc_fence_after();
-                    const uint32_t a0 = smem_u32(r.sA + (size_t)s * A_BYTES), b0 = smem_u32(r.sB + (size_t)s * B_BYTES);
+                    const uint32_t a0 = smem_u32(r.sA + (size_t)s * A_BYTES), b0 = smem_u32(r.sB + (size_t)s * Tile<PAIR>::B_BYTES);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        mma_f16(d, is_h ? smem_desc(a0 + 32 * j) : smem_desc_mn(a0 + 2048 * j), smem_desc_mn(b0 + 2048 * j), idesc,
+                        mma_f16<PAIR>(d, is_h ? smem_desc(a0 + 32 * j) : smem_desc_mn(a0 + 2048 * j), smem_desc_mn(b0 + 2048 * j), idesc,
                                 (kb > t.kb0 || j) ? 1u : 0u);
-                    mma_commit(&r.empty[s]);
+                    r.commit(&r.empty[s]);
                 }
-                mma_commit(&r.tfull[tile & 1u]);
+                r.commit(&r.tfull[tile & 1u]);
                 ++tile;
             }
         mma_done:
-            if (*r.abort_flag) {
-                mma_commit(r.dbar);
-                mbar_drain(r.dbar, 0u, kDrainLimitNs);
-            }
+            r.settle_mmas();
         }
     } else {
         const int quarter = warp & 3;
         uint8_t* piece = r.sE + (size_t)quarter * 2 * EPI_BYTES;
         uint32_t tile = 0, pieces = 0;
         bool both = false;  // the last store group read both pieces
-        for (int k = 0, item; (item = grad_item(w, k, is_h)) >= 0; ++k) {
+        for (int k = 0, item; (item = grad_item(w, r.worker, r.workers, k, is_h)) >= 0; ++k) {
             const GradTile t = grad_tile(w, item, is_h);
             if (t.kb0 >= t.kb1) continue;
             if (!wait_accumulator(r, tile, lane, err, limit_ns)) break;
             const uint32_t at = r.tmem + ((uint32_t)(quarter * 32) << 16) + (tile & 1u) * BN;
-            const int row = t.m * BM + quarter * 32;
-            for (int c = 0; c < boxes; ++c) {
+            const int row = t.m * TM + (int)r.rank * BM + quarter * 32, pieces_n = w.n / 64;
+            for (int c = 0; c < pieces_n; ++c) {
                 uint32_t v[64];
                 tmem_ld64(at + 64 * c, v);
                 tmem_wait64(v);
-                if (c == boxes - 1) release_accumulator(r, tile, lane);
+                if (c == pieces_n - 1) release_accumulator(r, tile, lane);
                 const int col = t.d * w.n + 64 * c;
                 if (is_h) {
                     // Both pieces: 32 fp32 columns each.
@@ -656,7 +743,10 @@ __global__ void __launch_bounds__(128)
     if (t >= tokens) return;
     const int64_t label = labels[t];
     const float g = label >= 0 && label < rows ? scale * (grad ? grad[t] : 1.f) : 0.f;
-    if (lane == 0) tok[t] = TokenGrad{lse[t] * LOG2E, g, g != 0.f ? label : -1};
+    if (lane == 0) {
+        const float lse2 = lse[t] * LOG2E;
+        tok[t] = TokenGrad{lse2, g, g != 0.f ? log2f(fabsf(g)) - lse2 : 0.f, g != 0.f ? (int)label : -1};
+    }
     for (int j = lane * 8; j < dim; j += 256)
         *reinterpret_cast<uint4*>(masked + t * dim + j) =
             g != 0.f ? *reinterpret_cast<const uint4*>(h + t * h_stride + j) : make_uint4(0u, 0u, 0u, 0u);
@@ -694,53 +784,68 @@ int make_map(CUtensorMap* map, const void* base, bool f32, int64_t cols, int64_t
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
+// A pair's 256-row tiles are worth it when single CTAs would have two tiles each.
+bool use_pairs(int sms, int64_t tokens, int64_t rows) {
+    return tokens > BM && (tokens + BM - 1) / BM * ((rows + BN - 1) / BN) >= 2 * sms;
+}
+
 struct ForwardPlan {
-    int token_tiles, row_tiles, splits;
+    bool pair;
+    int n, token_tiles, row_tiles, splits;
     size_t bytes;
 };
 
 ForwardPlan plan_forward(int sms, int64_t tokens, int64_t rows) {
     ForwardPlan p;
-    p.token_tiles = (int)((tokens + BM - 1) / BM);
-    p.row_tiles = (int)((rows + BN - 1) / BN);
+    p.pair = use_pairs(sms, tokens, rows);
+    const int tm = p.pair ? 2 * BM : BM, workers = p.pair ? sms / 2 : sms;
+    p.token_tiles = (int)((tokens + tm - 1) / tm);
+    // Half as wide tiles where whole ones leave CTAs without work.
+    p.n = !p.pair && p.token_tiles * ((rows + BN - 1) / BN) < sms ? BN / 2 : BN;
+    p.row_tiles = (int)((rows + p.n - 1) / p.n);
     // Row splits: rounds of the grid x (tiles of an item + half a tile for its start and end).
     double best = 0;
     p.splits = 1;
-    for (int sp = 1; sp <= std::min(sms, p.row_tiles); ++sp) {
-        const double cost = (double)(((int64_t)p.token_tiles * sp + sms - 1) / sms) * ((p.row_tiles + sp - 1) / sp + 0.5);
+    for (int sp = 1; sp <= std::min(workers, p.row_tiles); ++sp) {
+        const double cost = (double)(((int64_t)p.token_tiles * sp + workers - 1) / workers) * ((p.row_tiles + sp - 1) / sp + 0.5);
         if (sp == 1 || cost < best) {
             best = cost;
             p.splits = sp;
         }
     }
-    p.bytes = (size_t)p.splits * p.token_tiles * BM * sizeof(float2);
+    p.bytes = (size_t)p.splits * p.token_tiles * tm * sizeof(float2);
     return p;
 }
 
 struct BackwardPlan {
+    bool pair;
     int64_t chunk;  // table rows per chunk (a multiple of 256)
+    int n_scores;   // tile width of the logits
     int token_tiles, d_tiles, n, splits;
     size_t off_h, off_dh, off_g, bytes;
 };
 
 BackwardPlan plan_backward(int sms, int64_t tokens, int64_t rows, int dim) {
     BackwardPlan p;
-    p.token_tiles = (int)((tokens + BM - 1) / BM);
+    p.pair = use_pairs(sms, tokens, rows);
+    const int tm = p.pair ? 2 * BM : BM, workers = p.pair ? sms / 2 : sms;
+    p.token_tiles = (int)((tokens + tm - 1) / tm);
+    p.n_scores = !p.pair && p.token_tiles * ((rows + BN - 1) / BN) < sms ? BN / 2 : BN;
     const int64_t most = std::max<int64_t>(BN, G_ENTRIES / tokens / BN * BN);
     const int64_t chunks = (rows + most - 1) / most;
     p.chunk = up((rows + chunks - 1) / chunks, BN);
     p.d_tiles = (dim + BN - 1) / BN;
-    p.n = (int)up((dim + p.d_tiles - 1) / p.d_tiles, 64);
-    // K splits of dh: items of at most half a block's share of the chunk's work (or 8 K blocks), while
+    p.n = (int)up((dim + p.d_tiles - 1) / p.d_tiles, p.pair ? 128 : 64);
+    // K splits of dh: items of at most half a worker's share of the chunk's work (or 8 K blocks), while
     // the fp32 buffers stay within 64 MB.
     const int64_t chunk_rows = std::min(p.chunk, rows), kb_rows = (chunk_rows + BK - 1) / BK, kb_tokens = (tokens + BK - 1) / BK;
-    const int64_t work = p.d_tiles * (p.token_tiles * kb_rows + (chunk_rows + BM - 1) / BM * kb_tokens);
-    const int64_t item = std::max<int64_t>(8, work / (2 * sms));
-    const int64_t room = std::max<int64_t>(1, ((int64_t)64 << 20) / (p.token_tiles * BM * (int64_t)dim * 4));
+    const int64_t work = p.d_tiles * (p.token_tiles * kb_rows + (chunk_rows + tm - 1) / tm * kb_tokens);
+    const int64_t item = std::max<int64_t>(8, work / (2 * workers));
+    const int64_t room = std::max<int64_t>(1, ((int64_t)64 << 20) / (p.token_tiles * tm * (int64_t)dim * 4));
     p.splits = (int)std::min(std::min((kb_rows + item - 1) / item, room), kb_rows);
     p.off_h = (size_t)up(tokens * (int64_t)sizeof(TokenGrad), 1024);
     p.off_dh = p.off_h + (size_t)up(tokens * dim * 2, 1024);
-    p.off_g = p.off_dh + (size_t)up((int64_t)p.splits * p.token_tiles * BM * dim * 4, 1024);
+    p.off_g = p.off_dh + (size_t)up((int64_t)p.splits * p.token_tiles * tm * dim * 4, 1024);
     p.bytes = p.off_g + (size_t)(tokens * p.chunk * 2);
     return p;
 }
@@ -782,12 +887,31 @@ int workspace_of(va_context* ctx, void* workspace, size_t have, size_t need, voi
     return va_workspace(ctx, need, out);
 }
 
+// `items` workers of one or two CTAs, at most one CTA per SM.
+template <typename... Args>
+int launch_tiles(va_context* ctx, bool pair, int items, const char* name, void (*kern)(Args...), Args... args) {
+    VA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(pair ? 2 * std::min(ctx->sm_count / 2, items) : std::min(ctx->sm_count, items)));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pair ? 1 : 0;
+    VA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+    return va_check_launch(name);
+}
+
 template <int MODE>
-int launch_scores(va_context* ctx, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& g, const ScoreWork& work) {
-    VA_CUDA_TRY(cudaFuncSetAttribute(k_xent_scores<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
-    const int grid = std::min(ctx->sm_count, work.token_tiles * work.splits);
-    k_xent_scores<MODE><<<grid, THREADS, SMEM, ctx->stream>>>(h, w, g, work, ctx->d_error, wait_limit_ns(ctx->timeout_ms));
-    return va_check_launch("k_xent_scores");
+int launch_scores(va_context* ctx, bool pair, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& g,
+                  const ScoreWork& work) {
+    return launch_tiles(ctx, pair, work.token_tiles * work.splits, "k_xent_scores",
+                        pair ? k_xent_scores<MODE, true> : k_xent_scores<MODE, false>, h, w, g, work, ctx->d_error,
+                        wait_limit_ns(ctx->timeout_ms));
 }
 
 }  // namespace
@@ -816,8 +940,9 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
     VA_TRY(workspace_of(ctx, workspace, workspace_bytes, p.bytes, &ws));
     CUtensorMap mh, mw;
     VA_TRY(make_map(&mh, hidden, false, dim, tokens, hidden_stride, BK, BM));
-    VA_TRY(make_map(&mw, table, false, dim, rows, table_stride, BK, BN));
+    VA_TRY(make_map(&mw, table, false, dim, rows, table_stride, BK, p.pair ? BN / 2 : p.n));
     ScoreWork w{};
+    w.n = p.n;
     w.tokens = tokens;
     w.rows = rows;
     w.token_tiles = p.token_tiles;
@@ -826,8 +951,8 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
     w.k_blocks = (dim + BK - 1) / BK;
     w.scale2 = logit_scale * LOG2E;
     w.part = static_cast<float2*>(ws);
-    VA_TRY(launch_scores<FORWARD>(ctx, mh, mw, mh, w));
-    k_xent_join<<<(unsigned)((tokens + 3) / 4), 128, 0, ctx->stream>>>(w.part, p.splits, (int64_t)p.token_tiles * BM, hidden,
+    VA_TRY(launch_scores<FORWARD>(ctx, p.pair, mh, mw, mh, w));
+    k_xent_join<<<(unsigned)((tokens + 3) / 4), 128, 0, ctx->stream>>>(w.part, p.splits, (int64_t)p.token_tiles * (p.pair ? 2 * BM : BM), hidden,
                                                                      hidden_stride, table, table_stride, labels, tokens, rows,
                                                                      dim, logit_scale, loss, lse);
     return va_check_launch("k_xent_join");
@@ -858,12 +983,12 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
     k_xent_tokens<<<(unsigned)((tokens + 3) / 4), 128, 0, ctx->stream>>>(hidden, hidden_stride, labels, lse, grad_loss, tokens,
                                                                        rows, dim, logit_scale, tok, masked);
     VA_TRY(va_check_launch("k_xent_tokens"));
-    VA_CUDA_TRY(cudaFuncSetAttribute(k_xent_grads, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
 
-    const int64_t tokens_pad = (int64_t)p.token_tiles * BM;
+    const int tm = p.pair ? 2 * BM : BM;
+    const int64_t tokens_pad = (int64_t)p.token_tiles * tm;
     CUtensorMap mh, mw, mw64, mh64, mdh, mdw;
     VA_TRY(make_map(&mh, masked, false, dim, tokens, dim, BK, BM));
-    VA_TRY(make_map(&mw, table, false, dim, rows, table_stride, BK, BN));
+    VA_TRY(make_map(&mw, table, false, dim, rows, table_stride, BK, p.pair ? BN / 2 : p.n_scores));
     VA_TRY(make_map(&mh64, masked, false, dim, tokens, dim, 64, 64));
     VA_TRY(make_map(&mw64, table, false, dim, rows, table_stride, 64, 64));
     VA_TRY(make_map(&mdh, dh, true, dim, p.splits * tokens_pad, dim, 32, 32));
@@ -878,11 +1003,12 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
         s.rows = count;
         s.row0 = row0;
         s.token_tiles = p.token_tiles;
-        s.row_tiles = s.splits = (int)((count + BN - 1) / BN);
+        s.n = p.n_scores;
+        s.row_tiles = s.splits = (int)((count + s.n - 1) / s.n);
         s.k_blocks = (dim + BK - 1) / BK;
         s.scale2 = logit_scale * LOG2E;
         s.tok = tok;
-        VA_TRY(launch_scores<GRADIENT>(ctx, mh, mw, mg_out, s));
+        VA_TRY(launch_scores<GRADIENT>(ctx, p.pair, mh, mw, mg_out, s));
 
         GradWork w{};
         w.row0 = row0;
@@ -890,7 +1016,7 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
         w.dim = dim;
         w.tokens_pad = tokens_pad;
         w.token_tiles = p.token_tiles;
-        w.row_tiles = (int)((count + BM - 1) / BM);
+        w.row_tiles = (int)((count + tm - 1) / tm);
         w.d_tiles = p.d_tiles;
         w.splits = p.splits;
         w.n = p.n;
@@ -898,13 +1024,11 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
         w.kb_tokens = (int)((tokens + BK - 1) / BK);
         w.first = row0 == 0;
         const int items_h = p.token_tiles * p.d_tiles * p.splits, items_w = w.row_tiles * p.d_tiles;
-        const int grid = std::min(ctx->sm_count, items_h + items_w);
         const double cost_h = (double)w.kb_rows / p.splits, cost_w = w.kb_tokens;
         w.long_h = cost_h >= cost_w;
         w.extra = (int)std::lround(std::max(cost_h, cost_w) / std::max(1.0, std::min(cost_h, cost_w)));
-        k_xent_grads<<<grid, THREADS, SMEM, ctx->stream>>>(mg, mw64, mh64, mdh, mdw, w, ctx->d_error,
-                                                           wait_limit_ns(ctx->timeout_ms));
-        VA_TRY(va_check_launch("k_xent_grads"));
+        VA_TRY(launch_tiles(ctx, p.pair, items_h + items_w, "k_xent_grads", p.pair ? k_xent_grads<true> : k_xent_grads<false>, mg, mw64,
+                            mh64, mdh, mdw, w, ctx->d_error, wait_limit_ns(ctx->timeout_ms)));
     }
     const int64_t n4 = tokens * dim / 4;
     k_xent_finish<<<(unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)ctx->sm_count * 8), 256, 0, ctx->stream>>>(

@@ -21,51 +21,77 @@ import numpy as np
 
 from . import _ffi
 from .context import DeviceBuffer, GPUContext
-from .errors import InvalidInput
+from .errors import InvalidInput, raise_for_status
 from .kernels import MAXIMUM, Database, TopKSelectionKernel, _f32, _Kernel
 
 _ITEM = {_ffi.DTYPE_F32: 4, _ffi.DTYPE_BF16: 2, _ffi.DTYPE_INT8: 1}
 
 
-def _address(context: GPUContext, x, nbytes: int, name: str):
-    """Device address of an argument; what knows its own size, device or layout is checked."""
-    if x is None or isinstance(x, int):
+class _ScoringKernel(_Kernel):
+    """A kernel whose calls take device memory: keeps the device and the library's functions at hand, as a call
+    for one token costs little else."""
+
+    def __init__(self, context: GPUContext):
+        super().__init__(context)
+        self._device = context.device
+        self._lib = _ffi.load()
+
+
+def _checked(status: int, name: str) -> None:
+    if status != _ffi.VA_OK:
+        raise_for_status(status, f"{name}: {_ffi.last_error()}")
+
+
+def _dense(device: int, x, nbytes: int, name: str):
+    """Device address of a contiguous array of at least ``nbytes``; what knows its own size, device or layout is
+    checked."""
+    if x.__class__ is int:
         return x
-    if isinstance(x, DeviceBuffer):
-        if x.context.device != context.device:
-            raise InvalidInput(f"{name} is on device {x.context.device}, the context on device {context.device}")
-        if x.nbytes < nbytes:
-            raise InvalidInput(f"{name} holds {x.nbytes} bytes, {nbytes} are needed")
-        return x.ptr
-    if not hasattr(x, "data_ptr"):
-        raise InvalidInput(f"{name} must be a DeviceBuffer, a device address or have data_ptr(), got {type(x).__name__}")
-    device = x.device
-    if device.type != "cuda" or device.index != context.device:
-        raise InvalidInput(f"{name} is on {device}, the context on cuda:{context.device}")
-    return x.data_ptr()
-
-
-def _dense(context: GPUContext, x, nbytes: int, name: str):
-    """``_address`` of an array that must be contiguous and large enough."""
     if hasattr(x, "data_ptr"):
+        if x.get_device() == device and x.is_contiguous() and x.nbytes >= nbytes:
+            return x.data_ptr()
         if not x.is_contiguous():
             raise InvalidInput(f"{name} must be contiguous")
-        if x.numel() * x.element_size() < nbytes:
-            raise InvalidInput(f"{name} holds {x.numel() * x.element_size()} bytes, {nbytes} are needed")
-    return _address(context, x, nbytes, name)
+        if x.nbytes < nbytes:
+            raise InvalidInput(f"{name} holds {x.nbytes} bytes, {nbytes} are needed")
+        _device_of(device, x, name)
+    return _buffer(device, x, nbytes, name)
 
 
-def _strided(context: GPUContext, x, rows: int, dim: int, stride: int, item: int, name: str):
-    """``_address`` of rows that lie ``stride`` elements apart."""
-    nbytes = ((rows - 1) * stride + dim) * item if rows > 0 else 0
+def _strided(device: int, x, rows: int, dim: int, stride: int, item: int, name: str):
+    """Device address of rows of ``dim`` elements that lie ``stride`` elements apart."""
+    if x.__class__ is int:
+        return x
     if hasattr(x, "data_ptr"):
+        if (stride == dim and x.get_device() == device and x.is_contiguous() and x.itemsize == item
+                and x.nbytes >= rows * dim * item):
+            return x.data_ptr()
         if x.element_size() != item:
             raise InvalidInput(f"{name} has elements of {x.element_size()} bytes, {item} expected")
-        if x.dim() == 2 and rows > 0 and (x.shape[0] < rows or x.shape[1] < dim or x.stride(1) != 1
-                                          or (rows > 1 and x.stride(0) != stride)):
-            raise InvalidInput(f"{name} of shape {tuple(x.shape)} and strides {x.stride()} does not hold {rows} rows of "
-                               f"{dim} elements {stride} apart")
-    return _address(context, x, nbytes, name)
+        if x.dim() != 2 or x.shape[0] < rows or x.shape[1] < dim or (dim > 1 and x.stride(1) != 1) or (
+                rows > 1 and x.stride(0) != stride):
+            if rows > 0 and not (stride == dim and x.is_contiguous() and x.numel() >= rows * dim):
+                raise InvalidInput(f"{name} of shape {tuple(x.shape)} and strides {x.stride()} does not hold {rows} rows of "
+                                   f"{dim} elements {stride} apart")
+        if x.get_device() != device:
+            _device_of(device, x, name)
+        return x.data_ptr()
+    return _buffer(device, x, ((rows - 1) * stride + dim) * item if rows > 0 else 0, name)
+
+
+def _device_of(device: int, x, name: str) -> None:
+    if x.get_device() != device:
+        raise InvalidInput(f"{name} is on {x.device}, the context on cuda:{device}")
+
+
+def _buffer(device: int, x, nbytes: int, name: str):
+    if not isinstance(x, DeviceBuffer):
+        raise InvalidInput(f"{name} must be a DeviceBuffer, a device address or have data_ptr(), got {type(x).__name__}")
+    if x.context.device != device:
+        raise InvalidInput(f"{name} is on device {x.context.device}, the context on device {device}")
+    if x.nbytes < nbytes:
+        raise InvalidInput(f"{name} holds {x.nbytes} bytes, {nbytes} are needed")
+    return x.ptr
 
 
 def _to_bf16(a) -> np.ndarray:
@@ -85,7 +111,7 @@ def int4_row_bytes(dimension: int) -> int:
     return (dimension + 31) // 32 * 16
 
 
-class RMSNormInt8Kernel(_Kernel):
+class RMSNormInt8Kernel(_ScoringKernel):
     """Root-mean-square norm with the residual's addition and int8 codes with scales (va_rms_norm_int8)."""
 
     def encode(self, x, weight, rows: int, dimension: int, codes, scales, residual=None, residual_out=None,
@@ -93,18 +119,19 @@ class RMSNormInt8Kernel(_Kernel):
                residual_stride: int | None = None) -> None:
         """codes [rows x dimension] int8 and scales [rows x groups] fp32 (one group per row when ``group`` is 0) of
         h = x + residual; ``residual_out`` receives h. Strides in elements; the dimension by default."""
-        ctx = self.context
         if dtype not in (_ffi.DTYPE_F32, _ffi.DTYPE_BF16):
             raise InvalidInput(f"dtype must be DTYPE_F32 or DTYPE_BF16, got {dtype}")
-        item = _ITEM[dtype]
+        dev, item = self._device, _ITEM[dtype]
         xs = dimension if x_stride is None else x_stride
         rs = dimension if residual_stride is None else residual_stride
         groups = -(-dimension // group) if group > 0 else 1
-        _ffi.call("va_rms_norm_int8", self._h, _strided(ctx, x, rows, dimension, xs, item, "x"),
-                  _strided(ctx, residual, rows, dimension, rs, item, "residual") if residual is not None else None,
-                  _dense(ctx, weight, dimension * item, "weight"), rows, dimension, dtype, xs, rs, epsilon, group,
-                  _dense(ctx, residual_out, rows * dimension * item, "residual_out") if residual_out is not None else None,
-                  _dense(ctx, codes, rows * dimension, "codes"), _dense(ctx, scales, rows * groups * 4, "scales"))
+        n = rows * dimension
+        _checked(self._lib.va_rms_norm_int8(
+            self.context.handle, _strided(dev, x, rows, dimension, xs, item, "x"),
+            None if residual is None else _strided(dev, residual, rows, dimension, rs, item, "residual"),
+            _dense(dev, weight, dimension * item, "weight"), rows, dimension, dtype, xs, rs, epsilon, group,
+            None if residual_out is None else _dense(dev, residual_out, n * item, "residual_out"),
+            _dense(dev, codes, n, "codes"), _dense(dev, scales, rows * groups * 4, "scales")), "va_rms_norm_int8")
 
     def compute(self, x, weight, residual=None, epsilon: float = 1e-6, group: int = 0):
         """fp32 host arrays -> (codes int8 [rows, dim], scales [rows, groups], h [rows, dim])."""
@@ -140,21 +167,22 @@ class Int4Rows:
     scale_dtype: int
 
 
-class Int4GroupQuantizationKernel(_Kernel):
+class Int4GroupQuantizationKernel(_ScoringKernel):
     """4-bit codes with a scale, and optionally a zero point, per group of 32, 64 or 128 columns
     (va_sq_quantize_int4_groups; the codes' format is ScalarQuantizationKernel's)."""
 
     def encode(self, x, rows: int, dimension: int, group: int, codes, scales, zero_points=None,
                dtype: int = _ffi.DTYPE_F32, scale_dtype: int = _ffi.DTYPE_BF16, x_stride: int | None = None) -> None:
-        ctx = self.context
         _check_types(dtype, scale_dtype, group, (_ffi.DTYPE_F32, _ffi.DTYPE_BF16))
+        dev = self._device
         stride = dimension if x_stride is None else x_stride
         groups = -(-dimension // group)
-        _ffi.call("va_sq_quantize_int4_groups", self._h, _strided(ctx, x, rows, dimension, stride, _ITEM[dtype], "x"), dtype,
-                  rows, dimension, stride, group, scale_dtype,
-                  _dense(ctx, codes, rows * int4_row_bytes(dimension), "codes"),
-                  _dense(ctx, scales, rows * groups * _ITEM[scale_dtype], "scales"),
-                  _dense(ctx, zero_points, rows * groups, "zero_points") if zero_points is not None else None)
+        _checked(self._lib.va_sq_quantize_int4_groups(
+            self.context.handle, _strided(dev, x, rows, dimension, stride, _ITEM[dtype], "x"), dtype, rows, dimension, stride,
+            group, scale_dtype, _dense(dev, codes, rows * int4_row_bytes(dimension), "codes"),
+            _dense(dev, scales, rows * groups * _ITEM[scale_dtype], "scales"),
+            None if zero_points is None else _dense(dev, zero_points, rows * groups, "zero_points")),
+            "va_sq_quantize_int4_groups")
 
     def quantize(self, rows, group: int = 64, type: str = "symmetric",  # noqa: A002
                  scale_dtype: int = _ffi.DTYPE_BF16) -> Int4Rows:
@@ -195,7 +223,7 @@ def _check_types(dtype: int, scale_dtype: int, group: int, dtypes) -> None:
         raise InvalidInput(f"group must be 32, 64 or 128, got {group}")
 
 
-class Int4MatVecKernel(_Kernel):
+class Int4MatVecKernel(_ScoringKernel):
     """Products of a few queries with 4-bit rows (va_int4_matvec): fp32 scores [queries x rows]."""
 
     def encode(self, queries, num_queries: int, codes, scales, rows: int, dimension: int, group: int, out,
@@ -203,17 +231,17 @@ class Int4MatVecKernel(_Kernel):
                scale_dtype: int = _ffi.DTYPE_BF16, out_stride: int | None = None) -> None:
         """Queries [num_queries x dimension] contiguous, of ``query_dtype``; int8 queries take a scale each from
         ``query_scales``."""
-        ctx = self.context
-        _check_types(query_dtype, scale_dtype, group, (_ffi.DTYPE_F32, _ffi.DTYPE_BF16, _ffi.DTYPE_INT8))
+        _check_types(query_dtype, scale_dtype, group, _ITEM)
+        dev = self._device
         stride = rows if out_stride is None else out_stride
         groups = -(-dimension // group)
-        _ffi.call("va_int4_matvec", self._h, _dense(ctx, queries, num_queries * dimension * _ITEM[query_dtype], "queries"),
-                  query_dtype,
-                  _dense(ctx, query_scales, num_queries * 4, "query_scales") if query_scales is not None else None,
-                  num_queries, _dense(ctx, codes, rows * int4_row_bytes(dimension), "codes"),
-                  _dense(ctx, scales, rows * groups * _ITEM[scale_dtype], "scales"),
-                  _dense(ctx, zero_points, rows * groups, "zero_points") if zero_points is not None else None,
-                  rows, dimension, group, scale_dtype, _strided(ctx, out, num_queries, rows, stride, 4, "out"), stride)
+        _checked(self._lib.va_int4_matvec(
+            self.context.handle, _dense(dev, queries, num_queries * dimension * _ITEM[query_dtype], "queries"), query_dtype,
+            None if query_scales is None else _dense(dev, query_scales, num_queries * 4, "query_scales"), num_queries,
+            _dense(dev, codes, rows * int4_row_bytes(dimension), "codes"),
+            _dense(dev, scales, rows * groups * _ITEM[scale_dtype], "scales"),
+            None if zero_points is None else _dense(dev, zero_points, rows * groups, "zero_points"), rows, dimension, group,
+            scale_dtype, _strided(dev, out, num_queries, rows, stride, 4, "out"), stride), "va_int4_matvec")
 
     def compute(self, queries, table: Int4Rows) -> np.ndarray:
         """fp32 host queries -> scores [queries, rows]."""
@@ -273,7 +301,7 @@ class Int4Database:
                 b.free()
 
 
-class SoftmaxCrossEntropyKernel(_Kernel):
+class SoftmaxCrossEntropyKernel(_ScoringKernel):
     """Softmax cross entropy of tokens against all rows of a table, logits never kept, with the gradients
     of both sides (va_softmax_xent_forward / _backward). The table is bf16: device memory or a bf16
     ``Database``."""
@@ -285,48 +313,49 @@ class SoftmaxCrossEntropyKernel(_Kernel):
 
     def _table(self, table, rows: int, dimension: int, stride: int):
         if isinstance(table, Database):
-            if table.context.device != self.context.device:
-                raise InvalidInput(f"table is on device {table.context.device}, the context on device {self.context.device}")
+            if table.context.device != self._device:
+                raise InvalidInput(f"table is on device {table.context.device}, the context on device {self._device}")
             if table.dtype != _ffi.DTYPE_BF16 or table.dim != dimension or stride != dimension or table.n < rows:
                 raise InvalidInput(f"table must be a bf16 database of at least {rows} rows x {dimension}")
             return table.rows_ptr()
-        return _strided(self.context, table, rows, dimension, stride, 2, "table")
+        return _strided(self._device, table, rows, dimension, stride, 2, "table")
 
     def _workspace(self, workspace, tokens, rows, dimension, backward):
         if workspace is None:
             return None, 0
         if isinstance(workspace, int):
             return workspace, self.workspace_bytes(tokens, rows, dimension, backward)
-        nbytes = workspace.nbytes if isinstance(workspace, DeviceBuffer) else workspace.numel() * workspace.element_size()
-        return _dense(self.context, workspace, 0, "workspace"), nbytes
+        return _dense(self._device, workspace, 0, "workspace"), workspace.nbytes
 
     def encode_forward(self, hidden, table, labels, tokens: int, rows: int, dimension: int, loss, lse,
                        logit_scale: float = 1.0, hidden_stride: int | None = None, table_stride: int | None = None,
                        workspace=None) -> None:
         """hidden [tokens x dimension], table [rows x dimension] bf16; labels int64 (outside [0, rows): no
         loss); loss and lse [tokens] fp32. An integer ``workspace`` address must hold workspace_bytes()."""
-        ctx = self.context
+        dev = self._device
         hs = dimension if hidden_stride is None else hidden_stride
         ts = dimension if table_stride is None else table_stride
         ws, nbytes = self._workspace(workspace, tokens, rows, dimension, False)
-        _ffi.call("va_softmax_xent_forward", self._h, _strided(ctx, hidden, tokens, dimension, hs, 2, "hidden"), hs,
-                  self._table(table, rows, dimension, ts), ts, _dense(ctx, labels, tokens * 8, "labels"), tokens, rows,
-                  dimension, logit_scale, ws, nbytes, _dense(ctx, loss, tokens * 4, "loss"), _dense(ctx, lse, tokens * 4, "lse"))
+        _checked(self._lib.va_softmax_xent_forward(
+            self.context.handle, _strided(dev, hidden, tokens, dimension, hs, 2, "hidden"), hs,
+            self._table(table, rows, dimension, ts), ts, _dense(dev, labels, tokens * 8, "labels"), tokens, rows, dimension,
+            logit_scale, ws, nbytes, _dense(dev, loss, tokens * 4, "loss"), _dense(dev, lse, tokens * 4, "lse")),
+            "va_softmax_xent_forward")
 
     def encode_backward(self, hidden, table, labels, lse, grad_loss, tokens: int, rows: int, dimension: int, grad_hidden,
                         grad_table, logit_scale: float = 1.0, hidden_stride: int | None = None,
                         table_stride: int | None = None, workspace=None) -> None:
         """Gradients of sum(grad_loss * loss) (``grad_loss`` None: 1), bf16 and contiguous, written whole."""
-        ctx = self.context
+        dev = self._device
         hs = dimension if hidden_stride is None else hidden_stride
         ts = dimension if table_stride is None else table_stride
         ws, nbytes = self._workspace(workspace, tokens, rows, dimension, True)
-        _ffi.call("va_softmax_xent_backward", self._h, _strided(ctx, hidden, tokens, dimension, hs, 2, "hidden"), hs,
-                  self._table(table, rows, dimension, ts), ts, _dense(ctx, labels, tokens * 8, "labels"),
-                  _dense(ctx, lse, tokens * 4, "lse"),
-                  _dense(ctx, grad_loss, tokens * 4, "grad_loss") if grad_loss is not None else None, tokens, rows, dimension,
-                  logit_scale, ws, nbytes, _dense(ctx, grad_hidden, tokens * dimension * 2, "grad_hidden"),
-                  _dense(ctx, grad_table, rows * dimension * 2, "grad_table"))
+        _checked(self._lib.va_softmax_xent_backward(
+            self.context.handle, _strided(dev, hidden, tokens, dimension, hs, 2, "hidden"), hs,
+            self._table(table, rows, dimension, ts), ts, _dense(dev, labels, tokens * 8, "labels"),
+            _dense(dev, lse, tokens * 4, "lse"), None if grad_loss is None else _dense(dev, grad_loss, tokens * 4, "grad_loss"),
+            tokens, rows, dimension, logit_scale, ws, nbytes, _dense(dev, grad_hidden, tokens * dimension * 2, "grad_hidden"),
+            _dense(dev, grad_table, rows * dimension * 2, "grad_table")), "va_softmax_xent_backward")
 
     def compute(self, hidden, table, labels, logit_scale: float = 1.0, grad_loss=None):
         """Host arrays (hidden and table are rounded to bf16) -> (loss [T], lse [T], grad_hidden [T, D],
