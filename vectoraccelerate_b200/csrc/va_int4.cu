@@ -145,88 +145,126 @@ struct QueryShared {
     float* weight;  // [group][NT * 4]: of a pair of columns (DIGITS_WIDE)
 };
 
-// One warp lays out group `grp` of query q (absent queries and elements are zeros). The 32-code block's word t has
-// the nibbles of elements 8t..8t + 7: the even ones are k = 4t.. of the mma, the odd ones k = 16 + 4t...
+// Eight elements of query q from column j on (zeros where there are none) as fp32. The vector form needs queries that start on 16 (int8: 8) bytes and whole vectors.
+__device__ __forceinline__ void load_query(const MatvecArgs& a, int q, int j, bool vector, float (&f)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = 0.f;
+    if (q >= a.nq || j >= a.dim) return;
+    const int64_t at = (int64_t)q * a.dim + j;
+    if (a.x_dtype == VA_DTYPE_F32) {
+        const float* x = static_cast<const float*>(a.x) + at;
+        if (vector) {
+            const float4 u = __ldg(reinterpret_cast<const float4*>(x)), v = __ldg(reinterpret_cast<const float4*>(x) + 1);
+            f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (j + k < a.dim) f[k] = __ldg(x + k);
+        }
+    } else if (a.x_dtype == VA_DTYPE_BF16) {
+        const uint16_t* x = static_cast<const uint16_t*>(a.x) + at;
+        if (vector) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(k & 1 ? w[k >> 1] & 0xFFFF0000u : w[k >> 1] << 16);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (j + k < a.dim) f[k] = va::bf2f(__ldg(x + k));
+        }
+    } else {
+        const int8_t* x = static_cast<const int8_t*>(a.x) + at;
+        if (vector) {
+            const int2 u = __ldg(reinterpret_cast<const int2*>(x));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = (float)(int8_t)((k < 4 ? u.x : u.y) >> (8 * (k & 3)));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (j + k < a.dim) f[k] = (float)__ldg(x + k);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t high_halves(float lo, float hi) {
+    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+}
+
+// One warp lays out chunk c of query q: lane 4b + t has the 8 elements of word t of 32-code block b.
 template <int NT, int GROUP, int MODE>
-__device__ __forceinline__ void lay_out(const MatvecArgs& a, const QueryShared& sh, int q, int grp, int lane) {
-    constexpr int E = GROUP / 32;
+__device__ __forceinline__ void lay_out(const MatvecArgs& a, const QueryShared& sh, int q, int c, bool vector, int lane) {
+    float f[8];
+    load_query(a, q, c * CHUNK + lane * 8, vector, f);
+    const int blk = c * 8 + (lane >> 2), t = lane & 3;
     if constexpr (is_bf16(MODE)) {
         // k16 step h of a block pairs the nibbles (2h, 2h + 4) and (2h + 1, 2h + 5) of each word.
         constexpr int P = pieces_of(MODE);
+        bool finite[8];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int blk = grp * E + e, j = blk * 32 + lane, r = lane & 7;
-            const int64_t at = (int64_t)q * a.dim + j;
-            const bool there = q < a.nq && j < a.dim;
-            uint16_t* to = reinterpret_cast<uint16_t*>(
-                               sh.frag + (((size_t)blk * 2 + ((r >> 1) & 1)) * NT + (q >> 3)) * P * 32 + (q & 7) * 4 + (lane >> 3)) +
-                           (r & 1) * 2 + (r >> 2);
-            if constexpr (P == 1) {
-                *to = there ? static_cast<const uint16_t*>(a.x)[at] : (uint16_t)0;
-            } else {
-                float v = there ? static_cast<const float*>(a.x)[at] : 0.f;
-                const bool finite = fabsf(v) < INFINITY;
+        for (int k = 0; k < 8; ++k) finite[k] = fabsf(f[k]) < INFINITY;
 #pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    // an infinity or a NaN stays in the first piece
-                    const uint32_t u = v != v ? 0x7FC00000u : __float_as_uint(v) & 0xFFFF0000u;
-                    to[(size_t)p * 32 * 4] = (uint16_t)(u >> 16);
-                    v = finite ? v - __uint_as_float(u) : 0.f;
-                }
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                sh.frag[((((size_t)blk * 2 + h) * NT + (q >> 3)) * P + p) * 32 + (q & 7) * 4 + t] =
+                    make_uint2(high_halves(f[2 * h], f[2 * h + 4]), high_halves(f[2 * h + 1], f[2 * h + 5]));
+            if constexpr (P > 1) {
+                // what truncation left for the next piece; an infinity or a NaN stays in the first
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    f[k] = finite[k] ? f[k] - __uint_as_float(__float_as_uint(f[k]) & 0xFFFF0000u) : 0.f;
             }
         }
-        return;
-    }
-    constexpr bool wide = MODE == DIGITS_WIDE;
-    int v[E];
-    float w = 0.f;
-    if constexpr (!wide) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int j = grp * GROUP + e * 32 + lane;
-            v[e] = q < a.nq && j < a.dim ? static_cast<const int8_t*>(a.x)[(int64_t)q * a.dim + j] : 0;
-        }
     } else {
-        float f[E], top = 0.f;
-        bool finite = true;
+        constexpr int LANES = GROUP / 8;  // of a group
+        constexpr bool wide = MODE == DIGITS_WIDE;
+        constexpr int planes = wide ? 4 : 1;
+        const int grp = (c * CHUNK + lane * 8) / GROUP;
+        int v[8];
+        if constexpr (wide) {
+            float top = 0.f;
+            int finite = 1;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int j = grp * GROUP + e * 32 + lane;
-            const int64_t at = (int64_t)q * a.dim + j;
-            f[e] = q >= a.nq || j >= a.dim ? 0.f
-                   : a.x_dtype == VA_DTYPE_F32 ? static_cast<const float*>(a.x)[at]
-                                               : va::bf2f(static_cast<const uint16_t*>(a.x)[at]);
-            finite = finite && fabsf(f[e]) < INFINITY;
-            top = fmaxf(top, fabsf(f[e]));
+            for (int k = 0; k < 8; ++k) {
+                finite &= fabsf(f[k]) < INFINITY;
+                top = fmaxf(top, fabsf(f[k]));
+            }
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) {
+                finite &= __shfl_xor_sync(0xFFFFFFFFu, finite, o);
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            }
+            // 2^e > top; the fixed point's unit is 2^(e - 30), not below the smallest fp32. (The factor may
+            // exceed fp32: two steps.)
+            const int e = max((int)(__float_as_uint(top) >> 23) - 126, -119);
+            const float up = ldexpf(1.f, (30 - e) / 2), up2 = ldexpf(1.f, 30 - e - (30 - e) / 2);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = finite ? __float2int_rn(f[k] * up * up2) : 0;
+            if (lane % LANES == 0) {
+                const float w = finite ? ldexpf(1.f, e - 30) : __int_as_float(0x7FC00000);
+                *reinterpret_cast<float2*>(sh.weight + (size_t)grp * NT * 4 + q * 2) = make_float2(w * 65536.f, w);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = (int)f[k];
         }
-        finite = __all_sync(0xFFFFFFFFu, finite);
-        top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));
-        // 2^e > top; the fixed point's unit is 2^(e - 30), not below the smallest fp32.
-        const int e = max((int)(__float_as_uint(top) >> 23) - 126, -119);
-        w = finite ? ldexpf(1.f, e - 30) : __int_as_float(0x7FC00000);
-        // (two steps: the factor alone may exceed fp32)
-        const float up = ldexpf(1.f, (30 - e) / 2), up2 = ldexpf(1.f, 30 - e - (30 - e) / 2);
 #pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = finite ? __float2int_rn(f[i] * up * up2) : 0;
-    }
-    constexpr int planes = wide ? 4 : 1;
+        for (int p = planes - 1; p >= 0; --p) {  // digits from the lowest; column p = 0 has the highest
+            const int col = q * planes + p;
+            uint32_t d[2];  // even and odd elements
 #pragma unroll
-    for (int p = planes - 1; p >= 0; --p) {  // digits from the lowest; column p = 0 has the highest
-        const int col = q * planes + p;
-        int sum = 0;
+            for (int o = 0; o < 2; ++o)
+                d[o] = __byte_perm(__byte_perm(v[o], v[2 + o], 0x0040), __byte_perm(v[4 + o], v[6 + o], 0x0040), 0x5410);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int d = (int)(int8_t)v[e];
-            v[e] = (v[e] - d) >> 8;
-            sum += d;
-            const int blk = grp * E + e;
-            int8_t* to = reinterpret_cast<int8_t*>(sh.frag + ((size_t)blk * NT + (col >> 3)) * 32 + (col & 7) * 4 + (lane >> 3));
-            to[(lane & 1) * 4 + ((lane & 7) >> 1)] = (int8_t)d;
+            for (int k = 0; k < 8; ++k) v[k] = (v[k] - (int)(int8_t)v[k]) >> 8;
+            sh.frag[((size_t)blk * NT + (col >> 3)) * 32 + (col & 7) * 4 + t] = make_uint2(d[0], d[1]);
+            int sum = __dp4a((int)d[0], 0x01010101, __dp4a((int)d[1], 0x01010101, 0));
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            if (lane % LANES == 0) sh.start[(size_t)grp * NT * 8 + col] = (int)(MAGIC - 8u * (uint32_t)sum);
         }
-        sum = __reduce_add_sync(0xFFFFFFFFu, sum);
-        if (lane == 0) sh.start[(size_t)grp * NT * 8 + col] = (int)(MAGIC - 8u * (uint32_t)sum);
     }
-    if (wide && lane < 2) sh.weight[(size_t)grp * NT * 4 + q * 2 + lane] = lane == 0 ? w * 65536.f : w;
 }
 
 // NT column tiles of 8; S = scale type (uint16_t: bf16); GROUP = 32, 64, 128.
@@ -285,7 +323,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     next.load(a, base, part, t);
 
     constexpr int QUERIES = WIDE ? NT * 2 : NT * 8;
-    for (int i = warp; i < groups_pad * QUERIES; i += WARPS) lay_out<NT, GROUP, MODE>(a, sh, i % QUERIES, i / QUERIES, lane);
+    const int item = a.x_dtype == VA_DTYPE_F32 ? 4 : a.x_dtype == VA_DTYPE_BF16 ? 2 : 1;
+    const bool vector = a.dim % 8 == 0 && ((uintptr_t)a.x & (item == 1 ? 7 : 15)) == 0;
+    for (int i = warp; i < a.chunks * QUERIES; i += WARPS) lay_out<NT, GROUP, MODE>(a, sh, i % QUERIES, i / QUERIES, vector, lane);
     __syncthreads();
 
     // (the 16-byte unit b of row r lies at unit b ^ (r & 7) of its 128 bytes)
