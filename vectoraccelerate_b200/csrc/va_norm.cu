@@ -7,13 +7,13 @@
 //   code_j = rint(127 z_j / a)
 //   scale  = a / (127 sqrt(mean(h^2) + eps)),   so that code_j * scale ~ z_j / rms(h)
 // The rms cancels from the codes, which are therefore exact: the fp32 quotient decides a code
-// except within 2^-12 of a border between two codes (one element in 2,000), where the exact
+// except within 2^-14 of a border between two codes (one element in 8,000), where the exact
 // remainder does. The sum of squares and the scales are fp32. A row (or group) with
 // a < 2^-80 has codes 0 and scale 0. A row whose sum of squares is not finite, and a group whose a is
 // not finite, has codes 0 and scale NaN.
 //
 // The work is one read of x and residual, one write of residual_out and the codes: HBM-bound, with
-// ~20 instructions per element to hide. A thread holds 8 neighbouring elements of a row in registers between
+// ~20 instructions per element to hide. A thread holds one or two vectors of 8 elements of a row in registers between
 // the statistics and the codes, so nothing is read twice. Blocks are persistent: each thread's vectors of
 // the next rows come through cp.async into shared memory of its own (no barrier), the weights stay in
 // registers, and a row costs one block barrier.
@@ -98,10 +98,59 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return d;
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
+// max(a, |b|), a NaN wins
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
     float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;\n\t}" : "=f"(d) : "f"(a), "f"(b));
     return d;
+}
+
+// Packed bf16 through the mixed-precision fma: a + b as fp32, and a b + c exactly as fp32 fma of the two values.
+// (As fast as an fp32 fma, where unpacking by shift or mask runs at half that rate.)
+template <int HALF>
+__device__ __forceinline__ float fma_half(uint32_t a, uint32_t b, float c) {
+    float d;
+    if constexpr (HALF == 0)
+        asm("{\n\t.reg .b16 al, ah, bl, bh;\n\tmov.b32 {al, ah}, %1;\n\tmov.b32 {bl, bh}, %2;\n\tfma.rn.f32.bf16 %0, al, bl, %3;\n\t}"
+            : "=f"(d)
+            : "r"(a), "r"(b), "f"(c));
+    else
+        asm("{\n\t.reg .b16 al, ah, bl, bh;\n\tmov.b32 {al, ah}, %1;\n\tmov.b32 {bl, bh}, %2;\n\tfma.rn.f32.bf16 %0, ah, bh, %3;\n\t}"
+            : "=f"(d)
+            : "r"(a), "r"(b), "f"(c));
+    return d;
+}
+
+// x + r, rounded to the type.
+template <typename T>
+__device__ __forceinline__ Vec<T> add8(const Vec<T>& x, const Vec<T>& r) {
+    Vec<T> h;
+    if constexpr (sizeof(T) == 2) {
+        constexpr uint32_t ONE = 0x3F803F80u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            h.w[k] = pack_bf16(fma_half<0>(x.w[k], ONE, fma_half<0>(r.w[k], ONE, 0.f)),
+                               fma_half<1>(x.w[k], ONE, fma_half<1>(r.w[k], ONE, 0.f)));
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h.w[k] = __float_as_uint(x[k] + r[k]);
+    }
+    return h;
+}
+
+// z = h w (exact for bf16) and the sum of squares of h.
+template <typename T>
+__device__ __forceinline__ void products(const Vec<T>& h, const Vec<T>& w, float (&z)[8], float& sum) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if constexpr (sizeof(T) == 2) {
+            z[k] = k & 1 ? fma_half<1>(h.w[k >> 1], w.w[k >> 1], 0.f) : fma_half<0>(h.w[k >> 1], w.w[k >> 1], 0.f);
+            sum = k & 1 ? fma_half<1>(h.w[k >> 1], h.w[k >> 1], sum) : fma_half<0>(h.w[k >> 1], h.w[k >> 1], sum);
+        } else {
+            z[k] = h[k] * w[k];
+            sum = fmaf(h[k], h[k], sum);
+        }
+    }
 }
 
 // The largest |z| so far, exactly: z = hi + lo with hi = fl(z). Rounding is monotonic, so hi decides
@@ -112,29 +161,36 @@ struct Top {
     float hi = 0.f, lo = 0.f;
     __device__ __forceinline__ void take(float h, float l) {
         if constexpr (sizeof(T) == 2) {
-            hi = max_nan(hi, h);
+            hi = max_abs_nan(hi, h);
         } else {
             const bool more = !(h <= hi) || (h == hi && l > lo);
             lo = more ? l : lo;
             hi = more ? h : hi;
         }
     }
-    __device__ __forceinline__ void element(float h, float w) {
-        const float z = h * w;
-        if constexpr (sizeof(T) == 2) {
-            take(fabsf(z), 0.f);
-        } else {
-            const float e = fmaf(h, w, -z);
-            take(fabsf(z), z < 0.f ? -e : e);
+    // Of a thread's eight elements: the largest hi first, then lo among the (nearly always one) that have it.
+    __device__ __forceinline__ void of(const Vec<T>& h, const Vec<T>& w, const float (&z)[8]) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) hi = max_abs_nan(hi, z[k]);
+        if constexpr (sizeof(T) == 4) {
+            lo = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (fabsf(z[k]) == hi) lo = fmaxf(lo, copysignf(1.f, z[k]) * fmaf(h[k], w[k], -z[k]));
         }
     }
     template <int WIDTH>
     __device__ __forceinline__ void lanes() {
+        if constexpr (sizeof(T) == 2 && WIDTH == 32) {
+            // non-negative floats (and a NaN above them) order like their bits
+            hi = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(hi)));
+        } else {
 #pragma unroll
-        for (int o = 1; o < WIDTH; o <<= 1) {
-            const float h = __shfl_xor_sync(0xFFFFFFFFu, hi, o);
-            const float l = sizeof(T) == 2 ? 0.f : __shfl_xor_sync(0xFFFFFFFFu, lo, o);
-            take(h, l);
+            for (int o = 1; o < WIDTH; o <<= 1) {
+                const float h = __shfl_xor_sync(0xFFFFFFFFu, hi, o);
+                const float l = sizeof(T) == 2 ? 0.f : __shfl_xor_sync(0xFFFFFFFFu, lo, o);
+                take(h, l);
+            }
         }
     }
     __device__ __forceinline__ void lanes(int width) {
@@ -147,31 +203,32 @@ struct Top {
     }
 };
 
-// rint(127 z / a) of eight elements, packed. t = z (127 / a) in fp32 is within 127 * 4 * 2^-24 < 2^-15 of the
-// quotient; adding 1.5 * 2^23 rounds it (to even) into the low byte. Where some t is within 2^-12 of the border
+// rint(127 z / a) of eight elements, packed. t = z (127 / a) in fp32 is within 127 * 3 * 2^-24 < 2^-15 of the
+// quotient; adding 1.5 * 2^23 rounds it (to even) into the low byte. Where some t is within 2^-14 of the border
 // b between two codes, the sign of 127 z - b a decides: for bf16 both products are exact in fp32 (7 + 16 and 8 + 16
 // bits); for fp32 their rounding errors and the low parts are added (48 bits).
 template <typename T>
-__device__ __forceinline__ uint2 codes_of(const Vec<T>& h, const Vec<T>& w, const Top<T>& a) {
+__device__ __forceinline__ uint2 codes_of(const Vec<T>& h, const Vec<T>& w, const float (&z)[8], const Top<T>& a) {
     uint32_t m[8];
     constexpr float SHIFT = 12582912.f;
+    constexpr float NEAR = 0.5f - 0x1p-14f;
     const float inv = 127.f / a.hi;
     float off = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const float t = h[k] * w[k] * inv, r = t + SHIFT;
+        const float t = z[k] * inv, r = t + SHIFT;
         m[k] = __float_as_uint(r);
         off = fmaxf(off, fabsf(t - (r - SHIFT)));
     }
-    if (off > 0.5f - 0x1p-12f) {
+    if (off > NEAR) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float z = h[k] * w[k], t = z * inv, r = __uint_as_float(m[k]) - SHIFT, d = t - r;
-            if (fabsf(d) > 0.5f - 0x1p-12f) {
-                const float b = r + copysignf(0.5f, d), p = b * a.hi, q = 127.f * z;
+            const float t = z[k] * inv, r = __uint_as_float(m[k]) - SHIFT, d = t - r;
+            if (fabsf(d) > NEAR) {
+                const float b = r + copysignf(0.5f, d), p = b * a.hi, q = 127.f * z[k];
                 float diff = q - p;
                 if constexpr (sizeof(T) == 4)
-                    diff += (fmaf(127.f, z, -q) - fmaf(b, a.hi, -p)) + (127.f * fmaf(h[k], w[k], -z) - b * a.lo);
+                    diff += (fmaf(127.f, z[k], -q) - fmaf(b, a.hi, -p)) + (127.f * fmaf(h[k], w[k], -z[k]) - b * a.lo);
                 const float past = copysignf(diff, 1.f) == 0.f ? ((m[k] & 1u) ? 1.f : -1.f) : (d > 0.f ? diff : -diff);
                 if (past > 0.f) m[k] += d > 0.f ? 1u : 0xFFFFFFFFu;
             }
@@ -192,146 +249,184 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Rows on their way per thread (16-byte accesses only).
-template <typename T>
-constexpr int stages_of() { return sizeof(T) == 2 ? 3 : 2; }
+constexpr int STAGES = 3;  // rows per thread in work or on their way (16-byte accesses only)
 
-// TPR threads per row, 8 elements each; 8 * TPR >= dim. Narrow rows share a block of 128 threads.
+// Threads of a block for rows of TPR threads: narrow rows share a block of 128.
+constexpr int threads_of(int tpr) { return tpr < 128 ? 128 : tpr; }
+// Vectors of 8 elements per thread: two share the reductions' cost (bf16, 65536 x 4096: 316 us, with one 390 us);
+// two of fp32 overflow the registers (10007 x 1000: 31 us, with one 25 us).
+template <typename T>
+constexpr int vectors_of() { return sizeof(T) == 2 ? 2 : 1; }
+// Blocks per SM: 768 threads of up to 80 registers, or 1024 of 64.
+template <typename T>
+constexpr int blocks_of(int tpr) { return (vectors_of<T>() == 2 ? 768 : 1024) / threads_of(tpr); }
+
+// TPR threads per row; vector i of thread t is at (i * TPR + t) * 8.
 template <typename T, int W, int TPR>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR < 512 ? 1024 / (TPR < 128 ? 128 : TPR) : 2)
-    k_rms_norm_int8(NormArgs a) {
-    constexpr int THREADS = TPR < 128 ? 128 : TPR, ROWS = THREADS / TPR, WARPS = TPR / 32, STAGES = stages_of<T>();
+__global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm_int8(NormArgs a) {
+    constexpr int THREADS = threads_of(TPR), ROWS = THREADS / TPR, WARPS = TPR / 32, NV = vectors_of<T>();
     constexpr int HALVES = sizeof(T) / 2;  // 16-byte pieces of a vector
-    extern __shared__ uint4 s_in[];        // [stage][x, residual][piece][thread]
-    __shared__ float s_sum[2][ROWS][WARPS], s_hi[2][ROWS][WARPS], s_lo[2][ROWS][WARPS];
-    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR, j = t * 8;
-    const Vec<T> w = load8<T, W>(static_cast<const T*>(a.weight) + j, a.dim - j);
+    extern __shared__ uint4 s_in[];        // [stage][x, residual][vector][piece][thread]
+    __shared__ float4 s_part[2][ROWS][WARPS];  // (sum, hi, lo, -) of each warp
+    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR, j0 = t * 8;
+    Vec<T> w[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = load8<T, W>(static_cast<const T*>(a.weight) + j0 + i * TPR * 8, a.dim - j0 - i * TPR * 8);
     const int64_t step = (int64_t)gridDim.x * ROWS;
-    // Every thread of a block makes the same number of turns (barriers); rows past the end repeat the last one.
-    const int64_t row0 = (int64_t)blockIdx.x * ROWS;
-    const auto mine = [&](int64_t r) { return min(r + slot, a.rows - 1); };
-    const auto fetch = [&](int64_t r, int stage) {
+    // Every thread of a block makes the same number of turns (barriers); a slot without a row works on zeros.
+    int64_t row = (int64_t)blockIdx.x * ROWS + slot, ahead = row;
+    int64_t turns = row - slot < a.rows ? (a.rows - (row - slot) + step - 1) / step : 0;
+    const T* px = static_cast<const T*>(a.x) + row * a.x_stride + j0;
+    const T* pr = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride + j0 : nullptr;
+    // Row `ahead` into a stage; px and pr point at it and move on.
+    const auto fetch = [&](int stage) {
         if constexpr (W == 16) {
-            if (r < a.rows && j < a.dim) {
-                const T* px = static_cast<const T*>(a.x) + mine(r) * a.x_stride + j;
-                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(s_in + (size_t)stage * 2 * HALVES * THREADS + threadIdx.x);
+            if (ahead < a.rows) {
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(s_in + stage * 2 * NV * HALVES * THREADS + threadIdx.x);
 #pragma unroll
-                for (int i = 0; i < HALVES; ++i) cp_async16(dst + i * THREADS * 16, reinterpret_cast<const uint4*>(px) + i);
-                if (a.residual) {
-                    const T* pr = static_cast<const T*>(a.residual) + mine(r) * a.residual_stride + j;
+                for (int i = 0; i < NV; ++i) {
+                    if (j0 + i * TPR * 8 >= a.dim) continue;
 #pragma unroll
-                    for (int i = 0; i < HALVES; ++i)
-                        cp_async16(dst + (HALVES + i) * THREADS * 16, reinterpret_cast<const uint4*>(pr) + i);
+                    for (int p = 0; p < HALVES; ++p)
+                        cp_async16(dst + (i * HALVES + p) * THREADS * 16, reinterpret_cast<const uint4*>(px + i * TPR * 8) + p);
+                    if (pr) {
+#pragma unroll
+                        for (int p = 0; p < HALVES; ++p)
+                            cp_async16(dst + ((NV + i) * HALVES + p) * THREADS * 16,
+                                       reinterpret_cast<const uint4*>(pr + i * TPR * 8) + p);
+                    }
                 }
             }
             cp_async_commit();
+            ahead += step;
+            px += step * a.x_stride;
+            if (pr) pr += step * a.residual_stride;
         }
     };
-    const auto take = [&](int64_t r, int stage, bool residual) {
+    // A vector of the current row: from its stage, or from memory where rows have no 16-byte alignment.
+    const auto take = [&](int stage, int which, int i) {
         if constexpr (W == 16) {
             Vec<T> v;
-            const uint4* from = s_in + ((size_t)stage * 2 + (residual ? 1 : 0)) * HALVES * THREADS + threadIdx.x;
+            const uint4* from = s_in + ((stage * 2 + which) * NV + i) * HALVES * THREADS + threadIdx.x;
 #pragma unroll
-            for (int i = 0; i < HALVES; ++i) {
-                const uint4 u = j < a.dim ? from[i * THREADS] : make_uint4(0u, 0u, 0u, 0u);
-                v.w[4 * i] = u.x, v.w[4 * i + 1] = u.y, v.w[4 * i + 2] = u.z, v.w[4 * i + 3] = u.w;
+            for (int p = 0; p < HALVES; ++p) {
+                const uint4 u = from[p * THREADS];
+                v.w[4 * p] = u.x, v.w[4 * p + 1] = u.y, v.w[4 * p + 2] = u.z, v.w[4 * p + 3] = u.w;
             }
             return v;
         } else {
-            const T* p = residual ? static_cast<const T*>(a.residual) + mine(r) * a.residual_stride
-                                  : static_cast<const T*>(a.x) + mine(r) * a.x_stride;
-            return load8<T, W>(p + j, a.dim - j);
+            return load8<T, W>((which ? pr : px) + i * TPR * 8, a.dim - j0 - i * TPR * 8);
         }
     };
-    for (int s = 0; s < STAGES - 1; ++s) fetch(row0 + s * step, s);
+    for (int s = 0; s < STAGES - 1; ++s) fetch(s);
     int stage = 0, turn = 0;
-    for (int64_t r = row0; r < a.rows; r += step, turn ^= 1) {
+    const float mean = 1.f / (float)a.dim;
+    for (; turns > 0; --turns, turn ^= 1) {
         // (residual_out may be x's or residual's own rows: a row is stored only after its loads.)
-        fetch(r + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
-        cp_async_wait<STAGES - 1>();
-        const int64_t row = mine(r);
-        const bool live = r + slot < a.rows;
-        Vec<T> h = take(r, stage, false);
-        if (a.residual) {
-            const Vec<T> v = take(r, stage, true);
-            if constexpr (sizeof(T) == 2) {
+        fetch(stage == 0 ? STAGES - 1 : stage - 1);
+        if constexpr (W == 16) cp_async_wait<STAGES - 1>();
+        const bool live = row < a.rows;
+        Vec<T> h[NV] = {};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) h.w[k] = pack_bf16(h[2 * k] + v[2 * k], h[2 * k + 1] + v[2 * k + 1]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) h.w[k] = __float_as_uint(h[k] + v[k]);
+        for (int i = 0; i < NV; ++i)
+            if (live && j0 + i * TPR * 8 < a.dim) {
+                h[i] = take(stage, 0, i);
+                if (a.residual) h[i] = add8<T>(h[i], take(stage, 1, i));
             }
-            if (a.residual_out && live && j < a.dim)
-                store8<T, W>(static_cast<T*>(a.residual_out) + row * a.dim + j, a.dim - j, h);
+        if (a.residual_out && live) {
+            T* out = static_cast<T*>(a.residual_out) + row * a.dim + j0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (j0 + i * TPR * 8 < a.dim) store8<T, W>(out + i * TPR * 8, a.dim - j0 - i * TPR * 8, h[i]);
+        }
+        if constexpr (W != 16) {
+            px += step * a.x_stride;
+            if (pr) pr += step * a.residual_stride;
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
-        float sum = 0.f;
-        Top<T> top;
+        float sum = 0.f, z[NV][8];
+        Top<T> top[NV];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            sum = fmaf(h[k], h[k], sum);
-            top.element(h[k], w[k]);
+        for (int i = 0; i < NV; ++i) {
+            products<T>(h[i], w[i], z[i], sum);
+            top[i].of(h[i], w[i], z[i]);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        if (a.group)
-            top.lanes(a.group / 8);
-        else
-            top.template lanes<32>();
-        if constexpr (WARPS > 1) {
-            // Two sets of slots in turn: one barrier per row.
-            if ((t & 31) == 0) {
-                s_sum[turn][slot][t >> 5] = sum;
-                s_hi[turn][slot][t >> 5] = top.hi;
-                s_lo[turn][slot][t >> 5] = top.lo;
-            }
-            __syncthreads();
-            sum = 0.f;
+        if (a.group) {
 #pragma unroll
-            for (int k = 0; k < WARPS; ++k) sum += s_sum[turn][slot][k];
-            if (!a.group) {
-#pragma unroll
-                for (int k = 0; k < WARPS; ++k) top.take(s_hi[turn][slot][k], s_lo[turn][slot][k]);
-            }
-        }
-        if (!live || j >= a.dim) continue;
-        const bool ok = sum < INFINITY && top.hi < INFINITY;  // false for NaN too
-        if (a.group ? j % a.group == 0 : j == 0) {
-            const float per = rsqrtf(sum / (float)a.dim + a.eps) / 127.f;
-            a.scales[row * a.groups + (a.group ? j / a.group : 0)] =
-                !ok ? __int_as_float(0x7FC00000) : top.hi >= SMALLEST ? top.hi * per : 0.f;
-        }
-        uint2 packed = make_uint2(0u, 0u);
-        if (ok && top.hi >= SMALLEST) packed = codes_of<T>(h, w, top);
-        int8_t* codes = a.codes + row * a.dim + j;
-        if constexpr (W == 16) {
-            *reinterpret_cast<uint2*>(codes) = packed;
+            for (int i = 0; i < NV; ++i) top[i].lanes(a.group / 8);
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (j + k < a.dim) codes[k] = (int8_t)((k < 4 ? packed.x : packed.y) >> (8 * (k & 3)));
+            for (int i = 1; i < NV; ++i) top[0].take(top[i].hi, top[i].lo);
+            top[0].template lanes<32>();
         }
+        if constexpr (WARPS > 1) {
+            // Two sets of slots in turn: one barrier per row. Lane i takes warp i's part, then the lanes add up.
+            if ((t & 31) == 0) s_part[turn][slot][t >> 5] = make_float4(sum, top[0].hi, top[0].lo, 0.f);
+            __syncthreads();
+            const float4 p = s_part[turn][slot][t & (WARPS - 1)];
+            sum = p.x;
+#pragma unroll
+            for (int o = 1; o < WARPS; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            if (!a.group) {
+                top[0].hi = p.y;
+                top[0].lo = p.z;
+                top[0].template lanes<WARPS>();
+            }
+        }
+        if (!a.group) {
+#pragma unroll
+            for (int i = 1; i < NV; ++i) top[i] = top[0];
+        }
+        if (live) {
+            int8_t* codes = a.codes + row * a.dim + j0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int j = j0 + i * TPR * 8;
+                if (j >= a.dim) continue;
+                const bool ok = sum < INFINITY && top[i].hi < INFINITY;  // false for NaN too
+                if (a.group ? (j & (a.group - 1)) == 0 : j == 0) {
+                    const float per = rsqrtf(sum * mean + a.eps) * (1.f / 127.f);
+                    a.scales[row * a.groups + (a.group ? j / a.group : 0)] =
+                        !ok ? __int_as_float(0x7FC00000) : top[i].hi >= SMALLEST ? top[i].hi * per : 0.f;
+                }
+                uint2 packed = make_uint2(0u, 0u);
+                if (ok && top[i].hi >= SMALLEST) packed = codes_of<T>(h[i], w[i], z[i], top[i]);
+                int8_t* to = codes + i * TPR * 8;
+                if constexpr (W == 16) {
+                    *reinterpret_cast<uint2*>(to) = packed;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (j + k < a.dim) to[k] = (int8_t)((k < 4 ? packed.x : packed.y) >> (8 * (k & 3)));
+                }
+            }
+        }
+        row += step;
     }
 }
 
 template <typename T, int W, int TPR>
 int launch_rows(va_context* ctx, const NormArgs& a) {
-    constexpr int THREADS = TPR < 128 ? 128 : TPR, ROWS = THREADS / TPR, BLOCKS = TPR < 512 ? 1024 / THREADS : 2;
-    constexpr size_t SMEM = W == 16 ? (size_t)stages_of<T>() * 2 * (sizeof(T) / 2) * THREADS * 16 : 0;
+    constexpr int THREADS = threads_of(TPR), ROWS = THREADS / TPR;
+    constexpr size_t SMEM = W == 16 ? (size_t)STAGES * 2 * vectors_of<T>() * (sizeof(T) / 2) * THREADS * 16 : 0;
     if (SMEM > 47 * 1024)  // (with the static part over the 48 KB that need no asking)
         VA_CUDA_TRY(cudaFuncSetAttribute(k_rms_norm_int8<T, W, TPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
-    const int64_t grid = std::min<int64_t>((a.rows + ROWS - 1) / ROWS, (int64_t)ctx->sm_count * BLOCKS);
+    const int64_t grid = std::min<int64_t>((a.rows + ROWS - 1) / ROWS, (int64_t)ctx->sm_count * blocks_of<T>(TPR));
     k_rms_norm_int8<T, W, TPR><<<(unsigned)grid, THREADS, SMEM, ctx->stream>>>(a);
     return va_check_launch("k_rms_norm_int8");
 }
 
 template <typename T, int W>
 int launch_norm(va_context* ctx, const NormArgs& a) {
-    if (a.dim <= 256) return launch_rows<T, W, 32>(ctx, a);
-    if (a.dim <= 512) return launch_rows<T, W, 64>(ctx, a);
-    if (a.dim <= 1024) return launch_rows<T, W, 128>(ctx, a);
-    if (a.dim <= 2048) return launch_rows<T, W, 256>(ctx, a);
-    return launch_rows<T, W, 512>(ctx, a);
+    constexpr int PER = 8 * vectors_of<T>();  // elements of a thread
+    if (a.dim <= 32 * PER) return launch_rows<T, W, 32>(ctx, a);
+    if (a.dim <= 64 * PER) return launch_rows<T, W, 64>(ctx, a);
+    if (a.dim <= 128 * PER) return launch_rows<T, W, 128>(ctx, a);
+    if (a.dim <= 256 * PER) return launch_rows<T, W, 256>(ctx, a);
+    if constexpr (PER == 8) return launch_rows<T, W, 512>(ctx, a);
+    return VA_ERR_UNSUPPORTED;  // (not reached: 256 * 16 is the largest dimension)
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
