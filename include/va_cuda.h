@@ -493,8 +493,9 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
                             float logit_scale, void* workspace, size_t workspace_bytes, float* loss, float* lse);
 /* Gradients of sum_t grad_loss[t] * loss[t] (grad_loss NULL: 1) with respect to hidden and table, bf16,
  * contiguous [tokens x dim] and [rows x dim], both written whole; lse is the forward pass's. The logits are
- * recomputed in chunks of table rows; their gradient is rounded to bf16 before it is multiplied
- * with table and hidden. */
+ * recomputed in chunks of table rows. Roundings to bf16 before the products, which are summed in fp32: softmax
+ * minus one-hot; and, for grad_table, hidden rows weighted by their grad_loss relative to the first token's (exact
+ * where these are equal). */
 int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hidden_stride, const uint16_t* table,
                              int64_t table_stride, const int64_t* labels, const float* lse, const float* grad_loss,
                              int64_t tokens, int64_t rows, int dim, float logit_scale, void* workspace,

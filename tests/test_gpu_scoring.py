@@ -271,6 +271,28 @@ def test_matvec_large_table_of_many_tiles(tctx):
     assert ((out.double() - want).abs() <= matvec_tolerance(512, 64) * size).all()
 
 
+def test_matvec_and_norm_past_32_bit_offsets(tctx):
+    n, dim = 1100000, 4090  # 2.25e9 bytes of codes
+    g = gen(9)
+    codes = torch.randint(0, 256, (n, va.scoring.int4_row_bytes(dim)), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.rand(n, 32, generator=g, device="cuda")
+    x = randn(g, 2, dim)
+    out = run_matvec(tctx, x, None, codes, scales, None, dim, 128)
+    for rows in (slice(0, 500), slice(n - 500, n)):
+        want, size = matvec_reference(x, None, codes[rows], scales[rows], None, dim, 128)
+        assert ((out[:, rows].double() - want).abs() <= matvec_tolerance(dim, 128) * size).all()
+    del codes
+    rows = 530000  # 2.17e9 elements
+    x = torch.empty(rows, 4096, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    w = torch.ones(4096, dtype=torch.bfloat16, device="cuda")
+    codes, scales, _ = run_norm(tctx, x, w, None, "bf16", 128)
+    for part in (slice(0, 200), slice(rows - 200, rows)):
+        want, ws = norm_reference(x[part], w, 1e-6, 128)
+        assert torch.equal(codes[part].double(), want) and ((scales[part].double() - ws).abs() <= SCALE_TOL * ws).all()
+    del x, codes
+    torch.cuda.empty_cache()
+
+
 def test_matvec_strided_output_and_extreme_queries(tctx):
     g = gen(6)
     codes, scales, _ = make_table(g, 70, 96, 32, "f32", False)
@@ -341,11 +363,12 @@ def loss_reference(h, w, labels, c, grad):
     dz = (18 * dim / 16 + 24) * U32 * size
     dl = dz + (rows / 256 + 64) * U32 + 8 * U32 * lse.abs()
     dp = torch.expm1(dz + dl) + 2.0 ** -20
-    # G is rounded once to bf16, its products are summed in fp32 (the same count of roundings), the result rounded.
+    # p - [label] is rounded once to bf16, the products are summed in fp32 (the same count of roundings), the result
+    # rounded; for dw the weighted rows of h are rounded to bf16 too: (1 + U16)^2 - 1 <= 2 U16 + U16^2 of each product.
     dg = gz.abs() * U16 + (p.abs() + 2.0 ** -126) * dp[:, None] * (1 + U16) + 1e-40
     tokens = h.shape[0]
     bh = dg @ w.abs() + (18 * rows / 16 + 64) * U32 * (gz.abs() @ w.abs())
-    bw = dg.t() @ hm.abs() + (18 * tokens / 16 + 64) * U32 * (gz.abs().t() @ hm.abs())
+    bw = dg.t() @ hm.abs() * (1 + U16) + ((18 * tokens / 16 + 64) * U32 + U16) * (gz.abs().t() @ hm.abs())
     return loss, lse, dh, dw, dl, bh * (1 + U16) + dh.abs() * U16 + 1e-38, bw * (1 + U16) + dw.abs() * U16 + 1e-38
 
 
@@ -384,6 +407,61 @@ def check_loss(got, want):
 def test_loss_matches_64_bits(tctx, t, v, d):
     h, w, labels, grad = make_loss(t * 7 + v + d, t, v, d)
     check_loss(run_loss(tctx, h, w, labels, 1.0, grad), loss_reference(h, w, labels, 1.0, grad))
+
+
+@pytest.mark.parametrize("t, v, d", [(257, 38000, 72), (1300, 15001, 200), (513, 30000, 768), (2047, 9999, 1000)])
+def test_loss_of_many_tiles(tctx, t, v, d):
+    # enough tiles for pairs of CTAs, with ragged last tiles
+    h, w, labels, grad = make_loss(t + v + d, t, v, d)
+    got = run_loss(tctx, h, w, labels, 1.0, grad)
+    check_loss(got, loss_reference(h, w, labels, 1.0, grad))
+    assert all(torch.equal(a, b) for a, b in zip(got, run_loss(tctx, h, w, labels, 1.0, grad)))
+
+
+def test_loss_weights_of_every_size(tctx):
+    h, w, labels, grad = make_loss(17, 300, 900, 64)
+    for g in (grad * 1e-30, torch.where(torch.arange(300, device="cuda") % 7 == 0, grad * 1e20, grad), torch.full_like(grad, 0.1),
+              torch.cat([torch.zeros(299, device="cuda"), torch.ones(1, device="cuda")]), -grad.abs() - 0.1):
+        check_loss(run_loss(tctx, h, w, labels, 1.0, g), loss_reference(h, w, labels, 1.0, g))
+
+
+def test_loss_leaves_its_neighbours_alone(tctx):
+    for t, v, d in ((70, 300, 72), (400, 20000, 136)):
+        h, w, labels, grad = make_loss(18, t, v, d)
+        k = va.SoftmaxCrossEntropyKernel(tctx)
+        bufs = [torch.full((n,), 7.0, device="cuda", dtype=dt) for n, dt in ((t + 999, torch.float32), (t + 999, torch.float32),
+                                                                           (t * d + 9999, torch.bfloat16), (v * d + 9999, torch.bfloat16))]
+        need = max(k.workspace_bytes(t, v, d, b) for b in (False, True))
+        space = torch.full((need + 4096,), 0x55, dtype=torch.uint8, device="cuda")
+        ws = space.data_ptr()
+        k.encode_forward(h, w, labels, t, v, d, bufs[0], bufs[1], workspace=ws)
+        k.encode_backward(h, w, labels, bufs[1], grad, t, v, d, bufs[2], bufs[3], workspace=ws)
+        tctx.synchronize()
+        for b, n in zip(bufs, (t, t, t * d, v * d)):
+            assert (b[n:] == 7.0).all()
+        assert (space[need:] == 0x55).all()
+
+
+def test_loss_past_32_bit_offsets(tctx):
+    # a table of 2.2e9 elements: the last rows against the first
+    t, v, d = 130, 1500000, 1472
+    g = gen(19)
+    w = torch.empty(v, d, dtype=torch.bfloat16, device="cuda").normal_(0, 0.02, generator=g)
+    h = randn(g, t, d).bfloat16()
+    labels = torch.randint(v - 1000, v, (t,), generator=g, device="cuda")
+    loss, lse, dh, dw = run_loss(tctx, h, w, labels, 1.0, None)
+    z = torch.cat([h.double() @ w[i:i + 100000].double().t() for i in range(0, v, 100000)], 1)
+    want = torch.logsumexp(z, 1)
+    assert ((lse.double() - want).abs() <= 1e-5 * want.abs()).all()
+    p = torch.softmax(z, 1)
+    p[torch.arange(t, device="cuda"), labels] -= 1
+    for rows in (slice(0, 300), slice(v - 1000, v)):
+        ref = p[:, rows].t() @ h.double()
+        # two roundings before the product, one after, and the logits' errors (2^-14 of p)
+        bound = (3 * U16 + 2.0 ** -12) * (p[:, rows].abs().t() @ h.double().abs()) + 1e-38
+        assert ((dw[rows].double() - ref).abs() <= bound).all()
+    del p, z, w, dw
+    torch.cuda.empty_cache()
 
 
 def test_loss_in_several_chunks(tctx):
