@@ -246,6 +246,11 @@ __device__ __forceinline__ void tear_down(const Roles<PAIR>& r) {
     }
 }
 
+// Programmatic launches: the next kernel of the stream may start its set-up while this one runs; before it touches
+// global memory it waits for this one to be complete.
+__device__ __forceinline__ void pdl_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // A ring position shared by the producer and the MMA issuer.
 template <bool PAIR>
 struct Ring {
@@ -357,7 +362,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     k_xent_scores(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
                   const __grid_constant__ CUtensorMap map_g, ScoreWork w, int* err, uint64_t limit_ns) {
     extern __shared__ uint8_t smem_raw[];
+    pdl_start();
     const Roles<PAIR> r = set_up<PAIR>(smem_raw);
+    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n_items = w.token_tiles * w.splits;
     constexpr int TM = Tile<PAIR>::M;
@@ -547,7 +554,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                  const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_dh,
                  const __grid_constant__ CUtensorMap map_dw, GradWork w, int* err, uint64_t limit_ns) {
     extern __shared__ uint8_t smem_raw[];
+    pdl_start();
     const Roles<PAIR> r = set_up<PAIR>(smem_raw);
+    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int TM = Tile<PAIR>::M;
     const int boxes = w.n / 64 / Tile<PAIR>::CTAS;  // of B that this CTA loads
@@ -700,6 +709,8 @@ __global__ void __launch_bounds__(128)
     k_xent_join(const float2* __restrict__ part, int splits, int64_t pitch, const uint16_t* __restrict__ h,
                 int64_t h_stride, const uint16_t* __restrict__ table, int64_t w_stride, const int64_t* __restrict__ labels,
                 int64_t tokens, int64_t rows, int dim, float scale, float* __restrict__ loss, float* __restrict__ lse) {
+    pdl_start();
+    pdl_wait();
     const int lane = threadIdx.x & 31;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (t >= tokens) return;
@@ -749,6 +760,8 @@ __global__ void __launch_bounds__(128)
     k_xent_tokens(const uint16_t* __restrict__ h, int64_t h_stride, const int64_t* __restrict__ labels,
                   const float* __restrict__ lse, const float* __restrict__ grad, int64_t tokens, int64_t rows, int dim,
                   float scale, TokenGrad* __restrict__ tok, float* __restrict__ rho_out, uint16_t* __restrict__ weighted) {
+    pdl_start();
+    pdl_wait();
     const int lane = threadIdx.x & 31;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (t >= tokens) return;
@@ -787,6 +800,8 @@ __global__ void __launch_bounds__(128)
 // Sums the K splits of dh in order, applies the token's c g and rounds.
 __global__ void __launch_bounds__(256) k_xent_finish(const float4* __restrict__ part, int splits, int64_t pitch, int64_t n,
                                                      int per_token, const TokenGrad* __restrict__ tok, uint2* __restrict__ out) {
+    pdl_start();
+    pdl_wait();
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         float4 v = part[i];
         for (int s = 1; s < splits; ++s) {
@@ -923,23 +938,33 @@ int workspace_of(va_context* ctx, void* workspace, size_t have, size_t need, voi
     return va_workspace(ctx, need, out);
 }
 
+// Every kernel here is launched programmatically (see pdl_wait): the small ones of a short call would otherwise
+// spend as long on being launched one after another as on their work.
+template <typename... Args>
+int launch(va_context* ctx, unsigned grid, unsigned block, size_t smem, bool pair, const char* name, void (*kern)(Args...), Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pair ? 2 : 1;
+    VA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+    return va_check_launch(name);
+}
+
 // `items` workers of one or two CTAs, at most one CTA per SM.
 template <typename... Args>
 int launch_tiles(va_context* ctx, bool pair, int items, const char* name, void (*kern)(Args...), Args... args) {
     VA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(pair ? 2 * std::min(ctx->sm_count / 2, items) : std::min(ctx->sm_count, items)));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = SMEM;
-    cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pair ? 1 : 0;
-    VA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
-    return va_check_launch(name);
+    const int grid = pair ? 2 * std::min(ctx->sm_count / 2, items) : std::min(ctx->sm_count, items);
+    return launch(ctx, (unsigned)grid, THREADS, SMEM, pair, name, kern, args...);
 }
 
 template <int MODE>
@@ -988,10 +1013,9 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
     w.scale2 = logit_scale * LOG2E;
     w.part = static_cast<float2*>(ws);
     VA_TRY(launch_scores<FORWARD>(ctx, p.pair, mh, mw, mh, w));
-    k_xent_join<<<(unsigned)((tokens + 3) / 4), 128, 0, ctx->stream>>>(w.part, p.splits, (int64_t)p.token_tiles * (p.pair ? 2 * BM : BM), hidden,
-                                                                     hidden_stride, table, table_stride, labels, tokens, rows,
-                                                                     dim, logit_scale, loss, lse);
-    return va_check_launch("k_xent_join");
+    return launch(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_join", k_xent_join, (const float2*)w.part, p.splits,
+                  (int64_t)p.token_tiles * (p.pair ? 2 * BM : BM), hidden, hidden_stride, table, table_stride, labels, tokens, rows,
+                  dim, logit_scale, loss, lse);
 }
 
 int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hidden_stride, const uint16_t* table,
@@ -1017,9 +1041,8 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
     uint16_t* weighted = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_h);
     float* dh = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_dh);
     uint16_t* g = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_g);
-    k_xent_tokens<<<(unsigned)((tokens + 3) / 4), 128, 0, ctx->stream>>>(hidden, hidden_stride, labels, lse, grad_loss, tokens,
-                                                                       rows, dim, logit_scale, tok, rho, weighted);
-    VA_TRY(va_check_launch("k_xent_tokens"));
+    VA_TRY(launch(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_tokens", k_xent_tokens, hidden, hidden_stride, labels, lse,
+                  grad_loss, tokens, rows, dim, logit_scale, tok, rho, weighted));
 
     const int tm = p.pair ? 2 * BM : BM;
     const int64_t tokens_pad = (int64_t)p.token_tiles * tm;
@@ -1069,9 +1092,9 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
                             mh64, mdh, mdw, w, ctx->d_error, wait_limit_ns(ctx->timeout_ms)));
     }
     const int64_t n4 = tokens * dim / 4;
-    k_xent_finish<<<(unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)ctx->sm_count * 8), 256, 0, ctx->stream>>>(
-        reinterpret_cast<const float4*>(dh), p.splits, tokens_pad * dim / 4, n4, dim / 4, tok, reinterpret_cast<uint2*>(grad_hidden));
-    return va_check_launch("k_xent_finish");
+    return launch(ctx, (unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)ctx->sm_count * 8), 256, 0, false, "k_xent_finish",
+                  k_xent_finish, (const float4*)dh, p.splits, tokens_pad * dim / 4, n4, dim / 4, (const TokenGrad*)tok,
+                  (uint2*)grad_hidden);
 }
 
 }  // extern "C"
