@@ -43,9 +43,10 @@ constexpr int BOX = 64 * 128;             // bytes of a 64-row box of 128-byte r
 constexpr int A_BYTES = 2 * BOX;
 constexpr int RING_BYTES = 4 * 6 * BOX;   // 4 stages of 6 boxes, or 6 stages of 4 (pairs)
 constexpr int EPI_BYTES = 32 * 128;       // one staged 32-row x 128-byte piece of an epilogue warp
-constexpr int THREADS = 192;              // TMA warp, MMA warp, four epilogue warps
+constexpr int EPI_WARPS = 8;              // two per quarter of the TMEM lanes: each takes half of a tile's columns
+constexpr int THREADS = 64 + 32 * EPI_WARPS;  // TMA warp, MMA warp, epilogue warps
 constexpr int TMEM_COLS = 512;
-constexpr size_t SMEM = 1024 + RING_BYTES + 4 * 2 * EPI_BYTES + (2 * 6 + 5) * 8 + 16;
+constexpr size_t SMEM = 1024 + RING_BYTES + EPI_WARPS * EPI_BYTES + (2 * 6 + 5) * 8 + 16;
 constexpr int64_t G_ENTRIES = 1 << 27;    // gradient entries of a chunk (256 MB of bf16)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
@@ -187,7 +188,7 @@ __device__ __forceinline__ Roles<PAIR> set_up(uint8_t* smem_raw) {
     r.sA = smem;
     r.sB = smem + (size_t)STAGES * A_BYTES;
     r.sE = smem + RING_BYTES;
-    r.full = (uint64_t*)(r.sE + 4 * 2 * EPI_BYTES);
+    r.full = (uint64_t*)(r.sE + EPI_WARPS * EPI_BYTES);
     r.empty = r.full + STAGES;
     r.tfull = r.empty + STAGES;
     r.tempty = r.tfull + 2;
@@ -204,7 +205,7 @@ __device__ __forceinline__ Roles<PAIR> set_up(uint8_t* smem_raw) {
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&r.tfull[b], 1);
-            mbar_init(&r.tempty[b], 4 * Tile<PAIR>::CTAS);
+            mbar_init(&r.tempty[b], EPI_WARPS * Tile<PAIR>::CTAS);
         }
         mbar_init(r.dbar, 1);
         *r.abort_flag = 0;
@@ -294,7 +295,7 @@ struct ScoreWork {
     int token_tiles, row_tiles, splits, k_blocks;
     int n;                 // table rows of a tile: 256, or 128 (single CTAs)
     float scale2;          // c * log2(e)
-    float2* part;          // forward: (maximum, sum) per [split][token_tiles * tile rows]
+    float2* part;          // forward: (maximum, sum) per [split][column half][token_tiles * tile rows]
     const TokenGrad* tok;  // gradient
 };
 
@@ -417,8 +418,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             r.settle_mmas();
         }
     } else {
-        const int quarter = warp & 3;
-        uint8_t* piece = r.sE + (size_t)quarter * 2 * EPI_BYTES;
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        uint8_t* piece = r.sE + (size_t)(warp - 2) * EPI_BYTES;
         uint32_t tile = 0;
         for (int item = r.worker; item < n_items; item += r.workers) {
             score_item(w, item, tt, split, r0, r1);
@@ -430,9 +431,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             for (int t = r0; t < r1; ++t, ++tile) {
                 if (!wait_accumulator(r, tile, lane, err, limit_ns)) goto epilogue_done;
-                const uint32_t at = r.tmem + ((uint32_t)(quarter * 32) << 16) + (tile & 1u) * BN;
-                const int64_t col0 = (int64_t)t * w.n;
-                const int valid = (int)min((int64_t)w.n, w.rows - col0);
+                const int first = half * (w.n / 2);  // this warp's columns of the tile
+                const uint32_t at = r.tmem + ((uint32_t)(quarter * 32) << 16) + (tile & 1u) * BN + first;
+                const int64_t col0 = (int64_t)t * w.n + first;
+                const int valid = (int)max(min((int64_t)w.n / 2, w.rows - col0), (int64_t)0);
                 int64_t label = -1;
                 if constexpr (MODE == GRADIENT) label = (int64_t)tg.label - w.row0 - col0;
                 // 64 columns at a time, the next ones on their way from TMEM meanwhile.
@@ -440,40 +442,35 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if constexpr (MODE == FORWARD) {
                         lse_chunk(v, w.scale2, valid - 64 * c, top, nb, sum);
                     } else {
-                        uint8_t* p = piece + (c & 1) * EPI_BYTES;
-                        // the store that last used this piece has read it
-                        if (lane == 0) bulk_wait_read<1>();
+                        // the store that last used the piece has read it
+                        if (lane == 0) bulk_wait_read<0>();
                         __syncwarp();
-                        grad_chunk(v, w.scale2, tg, (int)max(min(label, (int64_t)BN) - 64 * c, (int64_t)-1), p, lane);
+                        grad_chunk(v, w.scale2, tg, (int)max(min(label, (int64_t)BN) - 64 * c, (int64_t)-1), piece, lane);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) {
-                            if (token0 < w.tokens && 64 * c < valid) tma_store_2d(&map_g, p, (int)(col0 + 64 * c), (int)token0);
+                            if (token0 < w.tokens && 64 * c < valid) tma_store_2d(&map_g, piece, (int)(col0 + 64 * c), (int)token0);
                             bulk_commit();
                         }
                     }
                 };
-                uint32_t ra[64], rb[64];
+                uint32_t ra[64];
                 tmem_ld64(at, ra);
                 tmem_wait64(ra);
-                tmem_ld64(at + 64, rb);
-                use(0, ra);
-                tmem_wait64(rb);
                 if (w.n > 128) {
-                    tmem_ld64(at + 128, ra);
-                    use(1, rb);
-                    tmem_wait64(ra);
-                    tmem_ld64(at + 192, rb);
-                    use(2, ra);
+                    uint32_t rb[64];
+                    tmem_ld64(at + 64, rb);
+                    use(0, ra);
                     tmem_wait64(rb);
                     release_accumulator(r, tile, lane);
-                    use(3, rb);
+                    use(1, rb);
                 } else {
                     release_accumulator(r, tile, lane);
-                    use(1, rb);
+                    use(0, ra);
                 }
             }
-            if constexpr (MODE == FORWARD) w.part[(int64_t)split * w.token_tiles * TM + token] = make_float2(-nb, sum);
+            if constexpr (MODE == FORWARD)
+                w.part[((int64_t)split * 2 + half) * w.token_tiles * TM + token] = make_float2(-nb, sum);
         }
     epilogue_done:
         if (MODE == GRADIENT && lane == 0) bulk_wait_all();
@@ -617,68 +614,61 @@ __global__ void __launch_bounds__(THREADS, 1)
             r.settle_mmas();
         }
     } else {
-        const int quarter = warp & 3;
-        uint8_t* piece = r.sE + (size_t)quarter * 2 * EPI_BYTES;
-        uint32_t tile = 0, pieces = 0;
-        bool both = false;  // the last store group read both pieces
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        uint8_t* piece = r.sE + (size_t)(warp - 2) * EPI_BYTES;
+        uint32_t tile = 0;
         const float rho = *w.rho;
+        // This warp's columns of a tile, in steps of 64.
+        const int c0 = half * ((w.n / 64 + 1) / 2), c1 = half ? w.n / 64 : (w.n / 64 + 1) / 2;
         for (int k = 0, item; (item = grad_item(w, r.worker, r.workers, k, is_h)) >= 0; ++k) {
             const GradTile t = grad_tile(w, item, is_h);
             if (t.kb0 >= t.kb1) continue;
             if (!wait_accumulator(r, tile, lane, err, limit_ns)) break;
             const uint32_t at = r.tmem + ((uint32_t)(quarter * 32) << 16) + (tile & 1u) * BN;
-            const int row = t.m * TM + (int)r.rank * BM + quarter * 32, pieces_n = w.n / 64;
-            for (int c = 0; c < pieces_n; ++c) {
+            const int row = t.m * TM + (int)r.rank * BM + quarter * 32;
+            if (c0 == c1) release_accumulator(r, tile, lane);
+            for (int c = c0; c < c1; ++c) {
                 uint32_t v[64];
                 tmem_ld64(at + 64 * c, v);
                 tmem_wait64(v);
-                if (c == pieces_n - 1) release_accumulator(r, tile, lane);
+                if (c == c1 - 1) release_accumulator(r, tile, lane);
                 const int col = t.d * w.n + 64 * c;
-                if (is_h) {
-                    // Both pieces: 32 fp32 columns each.
+                // fp32: 32 columns a piece; bf16: 64.
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (!is_h && i == 1) break;
                     if (lane == 0) bulk_wait_read<0>();
                     __syncwarp();
-                    both = true;
+                    if (is_h) {
 #pragma unroll
-                    for (int u = 0; u < 16; ++u)
-                        stage_unit(piece + (u >> 3) * EPI_BYTES, lane, u & 7, make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]));
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) {
-                        const int at_row = (int)(t.split * w.tokens_pad + row);
-                        for (int i = 0; i < 2; ++i) {
-                            if (col + 32 * i >= w.dim) break;
-                            if (w.first)
-                                tma_store_2d(&map_dh, piece + i * EPI_BYTES, col + 32 * i, at_row);
-                            else
-                                tma_add_2d(&map_dh, piece + i * EPI_BYTES, col + 32 * i, at_row);
+                        for (int u = 0; u < 8; ++u)
+                            stage_unit(piece, lane, u, make_uint4(v[32 * i + 4 * u], v[32 * i + 4 * u + 1], v[32 * i + 4 * u + 2], v[32 * i + 4 * u + 3]));
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            uint32_t b[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                asm("cvt.rn.bf16x2.f32 %0, %1, %2;"
+                                    : "=r"(b[e])
+                                    : "f"(__uint_as_float(v[u * 8 + 2 * e + 1]) * rho), "f"(__uint_as_float(v[u * 8 + 2 * e]) * rho));
+                            stage_unit(piece, lane, u, make_uint4(b[0], b[1], b[2], b[3]));
                         }
-                        bulk_commit();
-                    }
-                } else {
-                    uint8_t* p = piece + (pieces++ & 1u) * EPI_BYTES;
-                    if (lane == 0) {
-                        if (both)
-                            bulk_wait_read<0>();
-                        else
-                            bulk_wait_read<1>();
-                    }
-                    both = false;
-                    __syncwarp();
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        uint32_t b[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;"
-                                : "=r"(b[e])
-                                : "f"(__uint_as_float(v[u * 8 + 2 * e + 1]) * rho), "f"(__uint_as_float(v[u * 8 + 2 * e]) * rho));
-                        stage_unit(p, lane, u, make_uint4(b[0], b[1], b[2], b[3]));
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) {
-                        if (col < w.dim && w.row0 + row < w.rows) tma_store_2d(&map_dw, p, col, (int)(w.row0 + row));
+                        if (is_h) {
+                            const int at_row = (int)(t.split * w.tokens_pad + row);
+                            if (col + 32 * i < w.dim) {
+                                if (w.first)
+                                    tma_store_2d(&map_dh, piece, col + 32 * i, at_row);
+                                else
+                                    tma_add_2d(&map_dh, piece, col + 32 * i, at_row);
+                            }
+                        } else if (col < w.dim && w.row0 + row < w.rows) {
+                            tma_store_2d(&map_dw, piece, col, (int)(w.row0 + row));
+                        }
                         bulk_commit();
                     }
                 }
@@ -704,7 +694,7 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b) {
     return s;
 }
 
-// One warp per token: joins the splits' (maximum, sum) pairs and forms the label's logit.
+// One warp per token: joins the (maximum, sum) pairs of the splits' halves and forms the label's logit.
 __global__ void __launch_bounds__(128)
     k_xent_join(const float2* __restrict__ part, int splits, int64_t pitch, const uint16_t* __restrict__ h,
                 int64_t h_stride, const uint16_t* __restrict__ table, int64_t w_stride, const int64_t* __restrict__ labels,
@@ -858,12 +848,12 @@ ForwardPlan plan_forward(int sms, int64_t tokens, int64_t rows) {
     p.splits = 1;
     for (int sp = 1; sp <= std::min(workers, p.row_tiles); ++sp) {
         const double cost = (double)(((int64_t)p.token_tiles * sp + workers - 1) / workers) * ((p.row_tiles + sp - 1) / sp + 0.5);
-        if (sp == 1 || cost < best) {
+        if (sp == 1 || cost <= best) {  // (of equals, the one that uses more workers)
             best = cost;
             p.splits = sp;
         }
     }
-    p.bytes = (size_t)p.splits * p.token_tiles * tm * sizeof(float2);
+    p.bytes = (size_t)p.splits * 2 * p.token_tiles * tm * sizeof(float2);
     return p;
 }
 
@@ -1013,7 +1003,7 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
     w.scale2 = logit_scale * LOG2E;
     w.part = static_cast<float2*>(ws);
     VA_TRY(launch_scores<FORWARD>(ctx, p.pair, mh, mw, mh, w));
-    return launch(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_join", k_xent_join, (const float2*)w.part, p.splits,
+    return launch(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_join", k_xent_join, (const float2*)w.part, 2 * p.splits,
                   (int64_t)p.token_tiles * (p.pair ? 2 * BM : BM), hidden, hidden_stride, table, table_stride, labels, tokens, rows,
                   dim, logit_scale, loss, lse);
 }
