@@ -540,8 +540,8 @@ struct Launch {
 
 template <int MODE, int NT, typename S, bool ZERO, int GROUP>
 int launch_matvec(va_context* ctx, const Launch& l) {
-    auto kern = k_int4_matvec<MODE, NT, warps_of(NT), S, ZERO, GROUP>;
-    VA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)l.smem));
+    constexpr auto kern = k_int4_matvec<MODE, NT, warps_of(NT), S, ZERO, GROUP>;
+    VA_TRY(va_kernel_once<kern>(ctx->device, kMaxBlockSmem));
     kern<<<l.grid, warps_of(NT) * 32, l.smem, ctx->stream>>>(l.codes, l.a, ctx->d_error, wait_limit_ns(ctx->timeout_ms));
     return va_check_launch("k_int4_matvec");
 }

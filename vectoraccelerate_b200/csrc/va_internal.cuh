@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -66,6 +67,20 @@ struct VaDeviceGuard {
     bool moved = false;
     cudaError_t err = cudaSuccess;
 };
+
+// Once per kernel and device: lets the kernel take up to `smem` bytes of dynamic shared memory (0: leaves that) and asks
+// for the large shared-memory partition, so that kernels of one call do not repartition an SM between them.
+template <auto KERN>
+inline int va_kernel_once(int device, size_t smem) {
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+    if (done.load(std::memory_order_acquire) & bit) return VA_OK;
+    if (smem) VA_CUDA_TRY(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    VA_CUDA_TRY(cudaFuncSetAttribute(KERN, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    done.fetch_or(bit, std::memory_order_release);
+    return VA_OK;
+}
+constexpr size_t kMaxBlockSmem = 227 * 1024;
 
 // Device-side error codes written to the context's error word.
 #define VA_DEVERR_WAIT_TIMEOUT 1

@@ -411,10 +411,10 @@ template <typename T, int W, int TPR>
 int launch_rows(va_context* ctx, const NormArgs& a) {
     constexpr int THREADS = threads_of(TPR), ROWS = THREADS / TPR;
     constexpr size_t SMEM = W == 16 ? (size_t)STAGES * 2 * vectors_of<T>() * (sizeof(T) / 2) * THREADS * 16 : 0;
-    if (SMEM > 47 * 1024)  // (with the static part over the 48 KB that need no asking)
-        VA_CUDA_TRY(cudaFuncSetAttribute(k_rms_norm_int8<T, W, TPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+    constexpr auto kern = k_rms_norm_int8<T, W, TPR>;
+    VA_TRY(va_kernel_once<kern>(ctx->device, SMEM));
     const int64_t grid = std::min<int64_t>((a.rows + ROWS - 1) / ROWS, (int64_t)ctx->sm_count * blocks_of<T>(TPR));
-    k_rms_norm_int8<T, W, TPR><<<(unsigned)grid, THREADS, SMEM, ctx->stream>>>(a);
+    kern<<<(unsigned)grid, THREADS, SMEM, ctx->stream>>>(a);
     return va_check_launch("k_rms_norm_int8");
 }
 

@@ -247,8 +247,9 @@ __device__ __forceinline__ void tear_down(const Roles<PAIR>& r) {
     }
 }
 
-// Programmatic launches: the next kernel of the stream may start its set-up while this one runs; before it touches
-// global memory it waits for this one to be complete.
+// Programmatic launches: the next tile kernel of the stream may start its set-up while this kernel runs; before it
+// touches global memory it waits for this one to be complete. (So nothing here is read through the read-only path, which
+// assumes data that no kernel in flight writes.)
 __device__ __forceinline__ void pdl_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -696,21 +697,25 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b) {
 
 // One warp per token: joins the (maximum, sum) pairs of the splits' halves and forms the label's logit.
 __global__ void __launch_bounds__(128)
-    k_xent_join(const float2* __restrict__ part, int splits, int64_t pitch, const uint16_t* __restrict__ h,
-                int64_t h_stride, const uint16_t* __restrict__ table, int64_t w_stride, const int64_t* __restrict__ labels,
-                int64_t tokens, int64_t rows, int dim, float scale, float* __restrict__ loss, float* __restrict__ lse) {
+    k_xent_join(const float2* part, int splits, int64_t pitch, const uint16_t* h, int64_t h_stride, const uint16_t* table,
+                int64_t w_stride, const int64_t* labels, int64_t tokens, int64_t rows, int dim, float scale, float* loss, float* lse) {
     pdl_start();
-    pdl_wait();
     const int lane = threadIdx.x & 31;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (t >= tokens) return;
     float top = -INFINITY, sum = 0.f;
-    for (int i = lane; i < splits; i += 32) {
-        const float2 p = part[i * pitch + t];
-        if (p.y == 0.f) continue;  // no finite logit there
-        const float m = fmaxf(top, p.x);
-        sum = (sum != 0.f ? sum * ex2(top - m) : 0.f) + p.y * ex2(p.x - m);
-        top = m;
+    // Eight pairs in flight per lane. (Loads of what the kernel before wrote go to L2.)
+    for (int i0 = lane; i0 < splits; i0 += 256) {
+        float2 p[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[k] = i0 + 32 * k < splits ? __ldcg(part + (i0 + 32 * k) * pitch + t) : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (p[k].y == 0.f) continue;  // no finite logit there
+            const float m = fmaxf(top, p[k].x);
+            sum = (sum != 0.f ? sum * ex2(top - m) : 0.f) + p[k].y * ex2(p[k].x - m);
+            top = m;
+        }
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -747,11 +752,9 @@ __device__ __forceinline__ float token_scale(const int64_t* labels, const float*
 // first of the leading 256 tokens that has a loss, if it lies within 2^-60..2^60 (the quotients then stay in range),
 // else 1.
 __global__ void __launch_bounds__(128)
-    k_xent_tokens(const uint16_t* __restrict__ h, int64_t h_stride, const int64_t* __restrict__ labels,
-                  const float* __restrict__ lse, const float* __restrict__ grad, int64_t tokens, int64_t rows, int dim,
-                  float scale, TokenGrad* __restrict__ tok, float* __restrict__ rho_out, uint16_t* __restrict__ weighted) {
+    k_xent_tokens(const uint16_t* h, int64_t h_stride, const int64_t* labels, const float* lse, const float* grad, int64_t tokens,
+                  int64_t rows, int dim, float scale, TokenGrad* tok, float* rho_out, uint16_t* weighted) {
     pdl_start();
-    pdl_wait();
     const int lane = threadIdx.x & 31;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (t >= tokens) return;
@@ -788,10 +791,9 @@ __global__ void __launch_bounds__(128)
 }
 
 // Sums the K splits of dh in order, applies the token's c g and rounds.
-__global__ void __launch_bounds__(256) k_xent_finish(const float4* __restrict__ part, int splits, int64_t pitch, int64_t n,
-                                                     int per_token, const TokenGrad* __restrict__ tok, uint2* __restrict__ out) {
+__global__ void __launch_bounds__(256) k_xent_finish(const float4* part, int splits, int64_t pitch, int64_t n, int per_token,
+                                                     const TokenGrad* tok, uint2* out) {
     pdl_start();
-    pdl_wait();
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         float4 v = part[i];
         for (int s = 1; s < splits; ++s) {
@@ -928,10 +930,12 @@ int workspace_of(va_context* ctx, void* workspace, size_t have, size_t need, voi
     return va_workspace(ctx, need, out);
 }
 
-// Every kernel here is launched programmatically (see pdl_wait): the small ones of a short call would otherwise
-// spend as long on being launched one after another as on their work.
-template <typename... Args>
-int launch(va_context* ctx, unsigned grid, unsigned block, size_t smem, bool pair, const char* name, void (*kern)(Args...), Args... args) {
+// The tile kernels are launched programmatically (see pdl_wait): in a short call their set-up takes as long as their
+// work. The small kernels are not: their blocks would wait on the SMs where the tiles are still being worked on, and
+// slow them down (64 x 100000 x 768: 48 us instead of 36).
+template <auto KERN, typename... Args>
+int launch(va_context* ctx, unsigned grid, unsigned block, size_t smem, bool pair, const char* name, Args... args) {
+    VA_TRY(va_kernel_once<KERN>(ctx->device, smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
@@ -939,30 +943,30 @@ int launch(va_context* ctx, unsigned grid, unsigned block, size_t smem, bool pai
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].val.programmaticStreamSerializationAllowed = smem ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = 2;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pair ? 2 : 1;
-    VA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+    VA_CUDA_TRY(cudaLaunchKernelEx(&cfg, KERN, args...));
     return va_check_launch(name);
 }
 
 // `items` workers of one or two CTAs, at most one CTA per SM.
-template <typename... Args>
-int launch_tiles(va_context* ctx, bool pair, int items, const char* name, void (*kern)(Args...), Args... args) {
-    VA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+template <auto KERN, typename... Args>
+int launch_tiles(va_context* ctx, bool pair, int items, const char* name, Args... args) {
     const int grid = pair ? 2 * std::min(ctx->sm_count / 2, items) : std::min(ctx->sm_count, items);
-    return launch(ctx, (unsigned)grid, THREADS, SMEM, pair, name, kern, args...);
+    return launch<KERN>(ctx, (unsigned)grid, THREADS, SMEM, pair, name, args...);
 }
 
 template <int MODE>
 int launch_scores(va_context* ctx, bool pair, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& g,
                   const ScoreWork& work) {
-    return launch_tiles(ctx, pair, work.token_tiles * work.splits, "k_xent_scores",
-                        pair ? k_xent_scores<MODE, true> : k_xent_scores<MODE, false>, h, w, g, work, ctx->d_error,
-                        wait_limit_ns(ctx->timeout_ms));
+    const int items = work.token_tiles * work.splits;
+    const uint64_t limit = wait_limit_ns(ctx->timeout_ms);
+    return pair ? launch_tiles<k_xent_scores<MODE, true>>(ctx, true, items, "k_xent_scores", h, w, g, work, ctx->d_error, limit)
+                : launch_tiles<k_xent_scores<MODE, false>>(ctx, false, items, "k_xent_scores", h, w, g, work, ctx->d_error, limit);
 }
 
 }  // namespace
@@ -1003,7 +1007,7 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
     w.scale2 = logit_scale * LOG2E;
     w.part = static_cast<float2*>(ws);
     VA_TRY(launch_scores<FORWARD>(ctx, p.pair, mh, mw, mh, w));
-    return launch(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_join", k_xent_join, (const float2*)w.part, 2 * p.splits,
+    return launch<k_xent_join>(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_join", (const float2*)w.part, 2 * p.splits,
                   (int64_t)p.token_tiles * (p.pair ? 2 * BM : BM), hidden, hidden_stride, table, table_stride, labels, tokens, rows,
                   dim, logit_scale, loss, lse);
 }
@@ -1031,7 +1035,7 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
     uint16_t* weighted = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_h);
     float* dh = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_dh);
     uint16_t* g = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_g);
-    VA_TRY(launch(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_tokens", k_xent_tokens, hidden, hidden_stride, labels, lse,
+    VA_TRY(launch<k_xent_tokens>(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_tokens", hidden, hidden_stride, labels, lse,
                   grad_loss, tokens, rows, dim, logit_scale, tok, rho, weighted));
 
     const int tm = p.pair ? 2 * BM : BM;
@@ -1078,12 +1082,17 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
         const double cost_h = (double)w.kb_rows / p.splits, cost_w = w.kb_tokens;
         w.long_h = cost_h >= cost_w;
         w.extra = (int)std::lround(std::max(cost_h, cost_w) / std::max(1.0, std::min(cost_h, cost_w)));
-        VA_TRY(launch_tiles(ctx, p.pair, items_h + items_w, "k_xent_grads", p.pair ? k_xent_grads<true> : k_xent_grads<false>, mg, mw64,
-                            mh64, mdh, mdw, w, ctx->d_error, wait_limit_ns(ctx->timeout_ms)));
+        const uint64_t limit = wait_limit_ns(ctx->timeout_ms);
+        if (p.pair)
+            VA_TRY(launch_tiles<k_xent_grads<true>>(ctx, true, items_h + items_w, "k_xent_grads", mg, mw64, mh64, mdh, mdw, w,
+                                                    ctx->d_error, limit));
+        else
+            VA_TRY(launch_tiles<k_xent_grads<false>>(ctx, false, items_h + items_w, "k_xent_grads", mg, mw64, mh64, mdh, mdw, w,
+                                                     ctx->d_error, limit));
     }
     const int64_t n4 = tokens * dim / 4;
-    return launch(ctx, (unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)ctx->sm_count * 8), 256, 0, false, "k_xent_finish",
-                  k_xent_finish, (const float4*)dh, p.splits, tokens_pad * dim / 4, n4, dim / 4, (const TokenGrad*)tok,
+    return launch<k_xent_finish>(ctx, (unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)ctx->sm_count * 8), 256, 0, false,
+                                 "k_xent_finish", (const float4*)dh, p.splits, tokens_pad * dim / 4, n4, dim / 4, (const TokenGrad*)tok,
                   (uint2*)grad_hidden);
 }
 
