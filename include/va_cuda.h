@@ -492,7 +492,7 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
                             int64_t table_stride, const int64_t* labels, int64_t tokens, int64_t rows, int dim,
                             float logit_scale, void* workspace, size_t workspace_bytes, float* loss, float* lse);
 /* Gradients of sum_t grad_loss[t] * loss[t] (grad_loss NULL: 1) with respect to hidden and table, bf16,
- * contiguous [tokens x dim] and [rows x dim], both written whole; lse is the forward pass's. The logits are
+ * contiguous [tokens x dim] and [rows x dim], both written whole (neither may be hidden or table); lse is the forward pass's. The logits are
  * recomputed in chunks of table rows. Roundings to bf16 before the products, which are summed in fp32: softmax
  * minus one-hot; and, for grad_table, hidden rows weighted by their grad_loss relative to the first token's (exact
  * where these are equal). */

@@ -4,6 +4,10 @@ products with queries, softmax cross entropy with its gradients, and a run of th
 Tolerances count roundings: fp32 2^-24 and bf16 2^-8 of the value each (half a unit in the last place).
 """
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -308,6 +312,56 @@ def test_matvec_strided_output_and_extreme_queries(tctx):
     x[0, 50] = float("inf")
     out = run_matvec(tctx, x, None, codes, scales, None, 96, 32)
     assert torch.isnan(out[2]).all() and not torch.isfinite(out[0]).any() and torch.isfinite(out[1]).all()
+
+
+@pytest.mark.parametrize("nq", [1, 3])
+def test_matvec_query_with_outliers(tctx, nq):
+    # a few elements far above the rest: one or two queries are fixed-point numbers below their group's largest
+    g = gen(10)
+    codes, scales, zp = make_table(g, 400, 512, 64, "f32", True)
+    x = randn(g, nq, 512)
+    x[:, ::100] *= 3e4
+    out = run_matvec(tctx, x, None, codes, scales, zp, 512, 64)
+    want, size = matvec_reference(x, None, codes, scales, zp, 512, 64)
+    at = torch.arange(512, device="cuda") // 64
+    top = x.abs().double().view(nq, 8, 64).amax(2)[:, at]
+    w = ((unpack(codes, 512) - zp.to(torch.int32)[:, at]).double() * scales.double()[:, at]).abs()
+    assert ((out.double() - want).abs() <= matvec_tolerance(512, 64) * size + 2.0 ** -30 * (top @ w.t())).all()
+
+
+def test_first_call_inside_a_capture():
+    """In a process of its own: nothing has been loaded or set up before the capture."""
+    code = """
+import torch, vectoraccelerate_b200 as va
+s = torch.cuda.Stream()
+c = va.GPUContext(va.Metal4Configuration(device=0, stream=s.cuda_stream))
+t, v, d = 40, 500, 64
+h, w = torch.randn(t, d, device="cuda").bfloat16(), torch.randn(v, d, device="cuda").bfloat16()
+y, one = torch.zeros(t, dtype=torch.int64, device="cuda"), torch.ones(d, dtype=torch.bfloat16, device="cuda")
+q, qs, out = torch.empty(t, d, dtype=torch.int8, device="cuda"), torch.empty(t, 1, device="cuda"), torch.empty(t, v, device="cuda")
+codes, sc = torch.zeros(v, 32, dtype=torch.uint8, device="cuda") + 0x11, torch.ones(v, 1, dtype=torch.bfloat16, device="cuda")
+loss, lse, dh, dw = torch.empty(t, device="cuda"), torch.empty(t, device="cuda"), torch.empty_like(h), torch.empty_like(w)
+k = va.SoftmaxCrossEntropyKernel(c)
+ws = torch.empty(max(k.workspace_bytes(t, v, d, b) for b in (False, True)), dtype=torch.uint8, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    va.RMSNormInt8Kernel(c).encode(h, one, t, d, q, qs)
+    va.Int4MatVecKernel(c).encode(q, t, codes, sc, v, d, 64, out, query_dtype=va.DTYPE_INT8, query_scales=qs)
+    k.encode_forward(h, w, y, t, v, d, loss, lse, workspace=ws)
+    k.encode_backward(h, w, y, lse, None, t, v, d, dh, dw, workspace=ws)
+g.replay()
+torch.cuda.synchronize()
+assert torch.allclose(out, (q.float().sum(1, keepdim=True) * qs).expand(t, v), rtol=1e-5, atol=1e-5)
+assert torch.allclose(lse, torch.logsumexp(h.float() @ w.float().t(), 1), rtol=1e-4)
+assert torch.isfinite(dh.float()).all() and torch.isfinite(dw.float()).all()
+del g
+c.synchronize()
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert "captured" in r.stdout, r.stdout + r.stderr
 
 
 def test_matvec_nothing_to_do(tctx):

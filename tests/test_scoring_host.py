@@ -81,10 +81,10 @@ def test_loss_forward_refusals(change, word):
     refused("va_softmax_xent_forward", forward_args(**change), word)
 
 
-@pytest.mark.parametrize("change, word", LOSS + [(dict(gh=P + 2), "16 bytes"), (dict(gw=None), "NULL"), (dict(lse=None), "NULL")])
+@pytest.mark.parametrize("change, word", LOSS + [(dict(gw=P), "must not be"), (dict(gh=P), "must not be"), (dict(gh=P + 2), "16 bytes"), (dict(gw=None), "NULL"), (dict(lse=None), "NULL")])
 def test_loss_backward_refusals(change, word):
-    a = dict(ctx=CTX, h=P, hs=64, w=P, ws=64, labels=P, lse=P, g=None, tokens=5, rows=100, dim=64, scale=1.0, space=None, size=0, gh=P,
-             gw=P)
+    a = dict(ctx=CTX, h=P, hs=64, w=P, ws=64, labels=P, lse=P, g=None, tokens=5, rows=100, dim=64, scale=1.0, space=None, size=0, gh=2 * P,
+             gw=3 * P)
     a.update(change)
     refused("va_softmax_xent_backward", list(a.values()), word)
 

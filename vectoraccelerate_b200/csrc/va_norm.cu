@@ -16,7 +16,9 @@
 // ~20 instructions per element to hide. A thread holds one or two vectors of 8 elements of a row in registers between
 // the statistics and the codes, so nothing is read twice. Blocks are persistent: each thread's vectors of
 // the next rows come through cp.async into shared memory of its own (no barrier), the weights stay in
-// registers, and a row costs one block barrier.
+// registers, and a row costs one block barrier. Measured: 65536 x 4096 bf16 with residual 310 us, 6.0 TB/s; without a
+// residual (3 bytes an element) the instructions show: 16384 x 4096 70 us, 2.9 TB/s. Rows without 16-byte alignment are
+// read and written element by element, at a quarter to a half of that rate.
 #include <algorithm>
 
 #include "va_internal.cuh"
