@@ -519,7 +519,7 @@ def test_loss_past_32_bit_offsets(tctx):
 
 
 def test_loss_in_several_chunks(tctx):
-    # more than 2^27 gradient entries: several pieces of the table, dh added up over them
+    # more than 2^28 gradient entries: several pieces of the table, dh added up over them
     h, w, labels, grad = make_loss(11, 4099, 70001, 64)
     check_loss(run_loss(tctx, h, w, labels, 1.0, grad), loss_reference(h, w, labels, 1.0, grad))
 

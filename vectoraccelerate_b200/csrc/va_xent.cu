@@ -10,7 +10,8 @@
 // tcgen05.mma, two TMEM accumulators) and its epilogue keeps each token's running maximum and sum of
 // exponentials (in powers of two) in registers; the partial pairs of the row splits are joined by k_xent_join, which
 // also forms the label's logit.
-// Backward, 6TVD: the table is taken in chunks of rows so that G of a chunk (bf16) is at most 256 MB.
+// Backward, 6TVD: the table is taken in chunks of rows so that G of a chunk (bf16) is at most 512 MB (with 256 MB
+// the last, partly filled round of tiles weighs more: 2% slower at 8192 x 131072 x 1536).
 // k_xent_scores<GRADIENT> recomputes the chunk's logits and stores G; k_xent_grads multiplies it both
 // ways, with operands that are contiguous along the wrong axis read as MN-major tiles instead of being
 // transposed in memory: dw tiles (M = rows, K = tokens) are finished in one go; dh tiles (M = tokens, K = the
@@ -24,8 +25,8 @@
 // 128-row tiles twice over keep single CTAs, which spread wider; and where even those leave SMs idle, the logits' tiles
 // are 128 wide (333 x 5003 x 512: 7.8 us instead of 12.4).
 //
-// Measured (B200): forward 1380 TFLOP/s at 8192 x 131072 x 1536 (cuBLAS's own rate under the power cap); forward and
-// backward 10.2 ms there, 8TVD at 1290 TFLOP/s; 15 us of it the three small kernels.
+// Measured (B200, 8192 x 131072 x 1536): forward 2.4 ms, 1380 TFLOP/s; forward and backward 10.6 ms under the power cap,
+// 8TVD at 1240 TFLOP/s, where cuBLAS runs the same three products at 1330; 45 us of it are the three small kernels.
 //
 // Roundings: G is kept as P - [label] in bf16, without c g_t: a label's entry is then -1 to within its p, where
 // c g_t itself would round alike for every token of a mean and bias the gradients by up to 2^-8 (measured: 0.33%
@@ -52,7 +53,7 @@ constexpr int EPI_WARPS = 8;              // two per quarter of the TMEM lanes: 
 constexpr int THREADS = 64 + 32 * EPI_WARPS;  // TMA warp, MMA warp, epilogue warps
 constexpr int TMEM_COLS = 512;
 constexpr size_t SMEM = 1024 + RING_BYTES + EPI_WARPS * EPI_BYTES + (2 * 6 + 5) * 8 + 16;
-constexpr int64_t G_ENTRIES = 1 << 27;    // gradient entries of a chunk (256 MB of bf16)
+constexpr int64_t G_ENTRIES = 1 << 28;    // gradient entries of a chunk (512 MB of bf16)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
