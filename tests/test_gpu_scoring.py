@@ -457,7 +457,7 @@ def check_loss(got, want):
 
 @pytest.mark.parametrize("t, v, d", [(1, 1, 8), (1, 300, 64), (2, 257, 72), (127, 255, 64), (129, 256, 128), (130, 1000, 200),
                                      (64, 5003, 512), (333, 5003, 320), (1000, 777, 768), (257, 12345, 136), (2000, 130, 1024), (5, 40000, 1536),
-                                     (3, 515, 4096), (700, 600, 4088)])
+                                     (8192, 1000, 64), (4000, 300, 200), (20001, 700, 72), (3, 515, 4096), (700, 600, 4088)])
 def test_loss_matches_64_bits(tctx, t, v, d):
     h, w, labels, grad = make_loss(t * 7 + v + d, t, v, d)
     check_loss(run_loss(tctx, h, w, labels, 1.0, grad), loss_reference(h, w, labels, 1.0, grad))

@@ -15,7 +15,8 @@
 // k_xent_scores<GRADIENT> recomputes the chunk's logits and stores G; k_xent_grads multiplies it both
 // ways, with operands that are contiguous along the wrong axis read as MN-major tiles instead of being
 // transposed in memory: dw tiles (M = rows, K = tokens) are finished in one go; dh tiles (M = tokens, K = the
-// chunk's rows) add into an fp32 buffer per K split, which k_xent_finish sums and rounds.
+// chunk's rows) add into an fp32 buffer per K split, which k_xent_finish sums and rounds. Where few rows meet many
+// tokens dw is split the same way (8192 x 1000 x 64: backward 60 us in one go, 30 split).
 // Both directions are compute-bound once T and V pass a few hundred: the tensor pipe and its operand feed are the
 // limit, and the exponentials (16 per clock and SM) hide behind it above D = 256.
 //
@@ -489,13 +490,15 @@ __global__ void __launch_bounds__(THREADS, 1)
 // The two products of a chunk's G
 // ------------------------------------------------------------------------------------------------
 // Items: n_h = token_tiles * d_tiles * splits of dh (K = a split of the chunk's rows) and n_w = row_tiles *
-// d_tiles of dw (K = the tokens). A worker is a CTA or a pair.
+// d_tiles * splits_w of dw (K = the tokens, or a split of them). A worker is a CTA or a pair.
 struct GradWork {
     int64_t row0;           // first table row of the chunk
     int64_t rows;           // rows of the whole table
     int dim;
     int64_t tokens_pad;     // token_tiles * tile rows: of one split's dh buffer
+    int64_t rows_pad;       // row_tiles * tile rows: of one split's dw buffer
     int token_tiles, row_tiles, d_tiles, splits;
+    int splits_w;           // K splits of dw; 1: dw is finished at once
     const float* rho;       // what dw is multiplied by
     int n;                  // columns of a tile: 64, 128, 192 or 256 (pairs: 128 or 256)
     int kb_rows, kb_tokens; // K blocks of 64: chunk rows, tokens
@@ -507,7 +510,7 @@ struct GradWork {
 // The k-th item of worker b, or -1. The longer items go round the workers first; then `extra` shorter
 // ones to each worker left with one longer item less (as many as make up for it), then the rest to all.
 __device__ __forceinline__ int grad_item(const GradWork& w, int b, int grid, int k, bool& is_h) {
-    const int n_h = w.token_tiles * w.d_tiles * w.splits, n_w = w.row_tiles * w.d_tiles;
+    const int n_h = w.token_tiles * w.d_tiles * w.splits, n_w = w.row_tiles * w.d_tiles * w.splits_w;
     const int n_long = w.long_h ? n_h : n_w, n_short = w.long_h ? n_w : n_h;
     const int over = n_long % grid;
     const int longs = n_long / grid + (b < over ? 1 : 0);
@@ -544,10 +547,10 @@ __device__ __forceinline__ GradTile grad_tile(const GradWork& w, int item, bool 
         t.kb0 = (int)((int64_t)w.kb_rows * t.split / w.splits);
         t.kb1 = (int)((int64_t)w.kb_rows * (t.split + 1) / w.splits);
     } else {
-        t.m = rest;
-        t.split = 0;
-        t.kb0 = 0;
-        t.kb1 = w.kb_tokens;
+        t.m = rest % w.row_tiles;
+        t.split = rest / w.row_tiles;
+        t.kb0 = (int)((int64_t)w.kb_tokens * t.split / w.splits_w);
+        t.kb1 = (int)((int64_t)w.kb_tokens * (t.split + 1) / w.splits_w);
     }
     return t;
 }
@@ -556,7 +559,8 @@ template <bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
     k_xent_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_w,
                  const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_dh,
-                 const __grid_constant__ CUtensorMap map_dw, GradWork w, int* err, uint64_t limit_ns) {
+                 const __grid_constant__ CUtensorMap map_dw, const __grid_constant__ CUtensorMap map_dwp, GradWork w, int* err,
+                 uint64_t limit_ns) {
     extern __shared__ uint8_t smem_raw[];
     pdl_start();
     const Roles<PAIR> r = set_up<PAIR>(smem_raw);
@@ -641,12 +645,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (c == c1 - 1) release_accumulator(r, tile, lane);
                 const int col = t.d * w.n + 64 * c;
                 // fp32: 32 columns a piece; bf16: 64.
+                const bool f32 = is_h || w.splits_w > 1;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (!is_h && i == 1) break;
+                    if (!f32 && i == 1) break;
                     if (lane == 0) bulk_wait_read<0>();
                     __syncwarp();
-                    if (is_h) {
+                    if (f32) {
 #pragma unroll
                         for (int u = 0; u < 8; ++u)
                             stage_unit(piece, lane, u, make_uint4(v[32 * i + 4 * u], v[32 * i + 4 * u + 1], v[32 * i + 4 * u + 2], v[32 * i + 4 * u + 3]));
@@ -665,10 +670,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) {
-                        if (is_h) {
-                            const int at_row = (int)(t.split * w.tokens_pad + row);
+                        if (f32) {
+                            const int at_row = (int)(t.split * (is_h ? w.tokens_pad : w.rows_pad) + row);
                             if (col + 32 * i < w.dim) {
-                                if (w.first)
+                                if (!is_h)
+                                    tma_store_2d(&map_dwp, piece, col + 32 * i, at_row);
+                                else if (w.first)
                                     tma_store_2d(&map_dh, piece, col + 32 * i, at_row);
                                 else
                                     tma_add_2d(&map_dh, piece, col + 32 * i, at_row);
@@ -796,9 +803,9 @@ __global__ void __launch_bounds__(128)
     }
 }
 
-// Sums the K splits of dh in order, applies the token's c g and rounds.
-__global__ void __launch_bounds__(256) k_xent_finish(const float4* part, int splits, int64_t pitch, int64_t n, int per_token,
-                                                     const TokenGrad* tok, uint2* out) {
+// Sums K splits in order, applies the token's c g (dh) or rho (dw, tok NULL) and rounds.
+__global__ void __launch_bounds__(256) k_xent_finish(const float4* part, int splits, int64_t pitch, int64_t n, int per_row,
+                                                     const TokenGrad* tok, const float* rho, uint2* out) {
     pdl_start();
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         float4 v = part[i];
@@ -806,9 +813,9 @@ __global__ void __launch_bounds__(256) k_xent_finish(const float4* part, int spl
             const float4 u = part[i + s * pitch];
             v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
         }
-        const float g = tok[i / per_token].scale;
+        const float g = tok ? tok[i / per_row].scale : *rho;
         // (a token without loss has no gradient, whatever the table holds)
-        if (g == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (tok && g == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
         out[i] = make_uint2(va::f2bf_rn(v.x * g) | ((uint32_t)va::f2bf_rn(v.y * g) << 16),
                             va::f2bf_rn(v.z * g) | ((uint32_t)va::f2bf_rn(v.w * g) << 16));
     }
@@ -869,8 +876,9 @@ struct BackwardPlan {
     bool pair;
     int64_t chunk;  // table rows per chunk (a multiple of 256)
     int n_scores;   // tile width of the logits
-    int token_tiles, d_tiles, n, splits;
-    size_t off_rho, off_h, off_dh, off_g, bytes;
+    int token_tiles, d_tiles, n, splits, splits_w;
+    int64_t rows_pad;
+    size_t off_rho, off_h, off_dh, off_dw, off_g, bytes;
 };
 
 BackwardPlan plan_backward(int sms, int64_t tokens, int64_t rows, int dim) {
@@ -891,10 +899,15 @@ BackwardPlan plan_backward(int sms, int64_t tokens, int64_t rows, int dim) {
     const int64_t item = std::max<int64_t>(8, work / (2 * workers));
     const int64_t room = std::max<int64_t>(1, ((int64_t)64 << 20) / (p.token_tiles * tm * (int64_t)dim * 4));
     p.splits = (int)std::min(std::min((kb_rows + item - 1) / item, room), kb_rows);
+    // The same for dw, where the table is one chunk.
+    p.rows_pad = (chunk_rows + tm - 1) / tm * tm;
+    const int64_t room_w = std::max<int64_t>(1, ((int64_t)64 << 20) / (p.rows_pad * dim * 4));
+    p.splits_w = chunks > 1 ? 1 : (int)std::min(std::min((kb_tokens + item - 1) / item, room_w), kb_tokens);
     p.off_rho = (size_t)tokens * sizeof(TokenGrad);
     p.off_h = (size_t)up((int64_t)p.off_rho + 4, 1024);
     p.off_dh = p.off_h + (size_t)up(tokens * dim * 2, 1024);
-    p.off_g = p.off_dh + (size_t)up((int64_t)p.splits * p.token_tiles * tm * dim * 4, 1024);
+    p.off_dw = p.off_dh + (size_t)up((int64_t)p.splits * p.token_tiles * tm * dim * 4, 1024);
+    p.off_g = p.off_dw + (p.splits_w > 1 ? (size_t)up(p.splits_w * p.rows_pad * dim * 4, 1024) : 0);
     p.bytes = p.off_g + (size_t)(tokens * p.chunk * 2);
     return p;
 }
@@ -1042,19 +1055,22 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
     float* rho = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_rho);
     uint16_t* weighted = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_h);
     float* dh = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_dh);
+    float* dw = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_dw);
     uint16_t* g = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_g);
     VA_TRY(launch<k_xent_tokens>(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_tokens", hidden, hidden_stride, labels, lse,
                   grad_loss, tokens, rows, dim, logit_scale, tok, rho, weighted));
 
     const int tm = p.pair ? 2 * BM : BM;
     const int64_t tokens_pad = (int64_t)p.token_tiles * tm;
-    CUtensorMap mh, mw, mw64, mh64, mdh, mdw;
+    CUtensorMap mh, mw, mw64, mh64, mdh, mdw, mdwp;
     VA_TRY(make_map(&mh, hidden, false, dim, tokens, hidden_stride, BK, BM));
     VA_TRY(make_map(&mw, table, false, dim, rows, table_stride, BK, p.pair ? BN / 2 : p.n_scores));
     VA_TRY(make_map(&mh64, weighted, false, dim, tokens, dim, 64, 64));
     VA_TRY(make_map(&mw64, table, false, dim, rows, table_stride, 64, 64));
     VA_TRY(make_map(&mdh, dh, true, dim, p.splits * tokens_pad, dim, 32, 32));
     VA_TRY(make_map(&mdw, grad_table, false, dim, rows, dim, 64, 32));
+    mdwp = mdw;
+    if (p.splits_w > 1) VA_TRY(make_map(&mdwp, dw, true, dim, p.splits_w * p.rows_pad, dim, 32, 32));
     for (int64_t row0 = 0; row0 < rows; row0 += p.chunk) {
         const int64_t count = std::min(p.chunk, rows - row0);
         CUtensorMap mg_out, mg;
@@ -1081,27 +1097,33 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
         w.row_tiles = (int)((count + tm - 1) / tm);
         w.d_tiles = p.d_tiles;
         w.splits = p.splits;
+        w.splits_w = p.splits_w;
+        w.rows_pad = p.rows_pad;
         w.rho = rho;
         w.n = p.n;
         w.kb_rows = (int)((count + BK - 1) / BK);
         w.kb_tokens = (int)((tokens + BK - 1) / BK);
         w.first = row0 == 0;
-        const int items_h = p.token_tiles * p.d_tiles * p.splits, items_w = w.row_tiles * p.d_tiles;
-        const double cost_h = (double)w.kb_rows / p.splits, cost_w = w.kb_tokens;
+        const int items_h = p.token_tiles * p.d_tiles * p.splits, items_w = w.row_tiles * p.d_tiles * p.splits_w;
+        const double cost_h = (double)w.kb_rows / p.splits, cost_w = (double)w.kb_tokens / p.splits_w;
         w.long_h = cost_h >= cost_w;
         w.extra = (int)std::lround(std::max(cost_h, cost_w) / std::max(1.0, std::min(cost_h, cost_w)));
         const uint64_t limit = wait_limit_ns(ctx->timeout_ms);
         if (p.pair)
-            VA_TRY(launch_tiles<k_xent_grads<true>>(ctx, true, items_h + items_w, "k_xent_grads", mg, mw64, mh64, mdh, mdw, w,
+            VA_TRY(launch_tiles<k_xent_grads<true>>(ctx, true, items_h + items_w, "k_xent_grads", mg, mw64, mh64, mdh, mdw, mdwp, w,
                                                     ctx->d_error, limit));
         else
-            VA_TRY(launch_tiles<k_xent_grads<false>>(ctx, false, items_h + items_w, "k_xent_grads", mg, mw64, mh64, mdh, mdw, w,
+            VA_TRY(launch_tiles<k_xent_grads<false>>(ctx, false, items_h + items_w, "k_xent_grads", mg, mw64, mh64, mdh, mdw, mdwp, w,
                                                      ctx->d_error, limit));
     }
-    const int64_t n4 = tokens * dim / 4;
-    return launch<k_xent_finish>(ctx, (unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)ctx->sm_count * 8), 256, 0, false,
-                                 "k_xent_finish", (const float4*)dh, p.splits, tokens_pad * dim / 4, n4, dim / 4, (const TokenGrad*)tok,
-                  (uint2*)grad_hidden);
+    const auto finish = [&](const float* part, int splits, int64_t pad, int64_t n_rows, const TokenGrad* of, uint16_t* out) {
+        const int64_t n4 = n_rows * dim / 4;
+        return launch<k_xent_finish>(ctx, (unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)ctx->sm_count * 8), 256, 0, false,
+                                     "k_xent_finish", (const float4*)part, splits, pad * dim / 4, n4, dim / 4, of,
+                                     (const float*)rho, (uint2*)out);
+    };
+    if (p.splits_w > 1) VA_TRY(finish(dw, p.splits_w, p.rows_pad, rows, nullptr, grad_table));
+    return finish(dh, p.splits, tokens_pad, tokens, tok, grad_hidden);
 }
 
 }  // extern "C"
