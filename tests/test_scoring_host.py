@@ -129,6 +129,30 @@ def test_tensor_arguments_are_checked():
         norm.encode(P, P, 4, 64, torch.zeros(4, 63, dtype=torch.int8), P)
 
 
+def test_tensors_of_another_type_are_refused():
+    torch = pytest.importorskip("torch")
+    norm, matvec, loss = (k(_Context()) for k in (va.RMSNormInt8Kernel, va.Int4MatVecKernel, va.SoftmaxCrossEntropyKernel))
+    half, table = torch.zeros(4, 64, dtype=torch.float16), torch.zeros(9, 64, dtype=torch.bfloat16)
+    with pytest.raises(va.InvalidInput, match="x is torch.float16"):
+        norm.encode(half, P, 4, 64, P, P)
+    with pytest.raises(va.InvalidInput, match="weight has elements of 4 bytes"):  # fp32 weights of bf16 rows
+        norm.encode(P, torch.zeros(64), 4, 64, P, P)
+    with pytest.raises(va.InvalidInput, match="scales has elements of 4 bytes"):
+        matvec.encode(P, 1, P, torch.zeros(4, 1), 4, 64, 64, P, scale_dtype=BF16)
+    with pytest.raises(va.InvalidInput, match="queries is torch.int32"):
+        matvec.encode(torch.zeros(1, 64, dtype=torch.int32), 1, P, P, 4, 64, 64, P, query_dtype=F32)
+    with pytest.raises(va.InvalidInput, match="hidden is torch.float16"):
+        loss.encode_forward(half, table, P, 4, 9, 64, P, P)
+    with pytest.raises(va.InvalidInput, match="labels has elements of 4 bytes"):
+        loss.encode_forward(P, P, torch.zeros(8, dtype=torch.int32), 4, 9, 64, P, P)
+    with pytest.raises(va.InvalidInput, match="grad_table has elements of 4 bytes"):
+        loss.encode_backward(P, P, P, P, None, 4, 9, 64, P, torch.zeros(9, 64))
+    with pytest.raises(va.InvalidInput, match="workspace"):
+        loss.encode_forward(P, P, P, 4, 9, 64, P, P, workspace=torch.zeros(64, dtype=torch.uint8))
+    with pytest.raises(va.InvalidInput, match="hidden is on cpu"):  # bf16 bit patterns are taken
+        loss.encode_forward(torch.zeros(4, 64, dtype=torch.int16), P, P, 4, 9, 64, P, P)
+
+
 def test_bf16_conversion_rounds_to_even():
     x = np.array([1.0, 1.00390625, 1.01171875, -2.5, 3.0e38, np.inf, -np.inf, 1e-40], np.float32)
     assert scoring._to_bf16(x).tolist() == [0x3F80, 0x3F80, 0x3F82, 0xC020, 0x7F62, 0x7F80, 0xFF80, 0x0001]

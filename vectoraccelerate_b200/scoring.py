@@ -42,41 +42,61 @@ def _checked(status: int, name: str) -> None:
         raise_for_status(status, f"{name}: {_ffi.last_error()}")
 
 
-def _dense(device: int, x, nbytes: int, name: str):
-    """Device address of a contiguous array of at least ``nbytes``; what knows its own size, device or layout is
-    checked."""
+# Element types that a tensor may have where elements of so many bytes are expected (bf16 also as bit patterns), by
+# name, and their type objects as they are met: looking an object up is what a call of a few microseconds affords.
+_TYPE_NAMES = {1: {"int8", "uint8"}, 2: {"bfloat16", "int16", "uint16"}, 4: {"float32"}, 8: {"int64"}}
+_TYPES = {item: set() for item in _TYPE_NAMES}
+
+
+def _dense(device: int, x, count: int, item: int, name: str):
+    """Device address of a contiguous array of at least ``count`` elements of ``item`` bytes; what knows its own
+    size, type, device or layout is checked."""
     if x.__class__ is int:
         return x
-    if hasattr(x, "data_ptr"):
-        if x.get_device() == device and x.is_contiguous() and x.nbytes >= nbytes:
+    if x.__class__ is DeviceBuffer:
+        return _buffer(device, x, count * item, name)
+    try:
+        if x.dtype in _TYPES[item] and x.get_device() == device and x.nbytes >= count * item and x.is_contiguous():
             return x.data_ptr()
+        _check_type(x, item, name)
         if not x.is_contiguous():
             raise InvalidInput(f"{name} must be contiguous")
-        if x.nbytes < nbytes:
-            raise InvalidInput(f"{name} holds {x.nbytes} bytes, {nbytes} are needed")
+        if x.nbytes < count * item:
+            raise InvalidInput(f"{name} holds {x.nbytes} bytes, {count * item} are needed")
         _device_of(device, x, name)
-    return _buffer(device, x, nbytes, name)
+        return x.data_ptr()
+    except AttributeError:
+        return _buffer(device, x, 0, name)
 
 
 def _strided(device: int, x, rows: int, dim: int, stride: int, item: int, name: str):
     """Device address of rows of ``dim`` elements that lie ``stride`` elements apart."""
     if x.__class__ is int:
         return x
-    if hasattr(x, "data_ptr"):
-        if (stride == dim and x.get_device() == device and x.is_contiguous() and x.itemsize == item
-                and x.nbytes >= rows * dim * item):
+    if x.__class__ is DeviceBuffer:
+        return _buffer(device, x, ((rows - 1) * stride + dim) * item if rows > 0 else 0, name)
+    try:
+        if (stride == dim and x.dtype in _TYPES[item] and x.get_device() == device and x.nbytes >= rows * dim * item
+                and x.is_contiguous()):
             return x.data_ptr()
-        if x.element_size() != item:
-            raise InvalidInput(f"{name} has elements of {x.element_size()} bytes, {item} expected")
-        if x.dim() != 2 or x.shape[0] < rows or x.shape[1] < dim or (dim > 1 and x.stride(1) != 1) or (
-                rows > 1 and x.stride(0) != stride):
-            if rows > 0 and not (stride == dim and x.is_contiguous() and x.numel() >= rows * dim):
-                raise InvalidInput(f"{name} of shape {tuple(x.shape)} and strides {x.stride()} does not hold {rows} rows of "
-                                   f"{dim} elements {stride} apart")
-        if x.get_device() != device:
-            _device_of(device, x, name)
+        _check_type(x, item, name)
+        if rows > 0 and not (stride == dim and x.is_contiguous() and x.nbytes >= rows * dim * item) and (
+                x.dim() != 2 or x.shape[0] < rows or x.shape[1] < dim or (dim > 1 and x.stride(1) != 1)
+                or (rows > 1 and x.stride(0) != stride)):
+            raise InvalidInput(f"{name} of shape {tuple(x.shape)} and strides {x.stride()} does not hold {rows} rows of "
+                               f"{dim} elements {stride} apart")
+        _device_of(device, x, name)
         return x.data_ptr()
-    return _buffer(device, x, ((rows - 1) * stride + dim) * item if rows > 0 else 0, name)
+    except AttributeError:
+        return _buffer(device, x, 0, name)
+
+
+def _check_type(x, item: int, name: str) -> None:
+    if x.itemsize != item:
+        raise InvalidInput(f"{name} has elements of {x.itemsize} bytes, {item} expected")
+    if str(x.dtype).rpartition(".")[2] not in _TYPE_NAMES[item]:
+        raise InvalidInput(f"{name} is {x.dtype}, expected {' or '.join(sorted(_TYPE_NAMES[item]))}")
+    _TYPES[item].add(x.dtype)
 
 
 def _device_of(device: int, x, name: str) -> None:
@@ -129,9 +149,9 @@ class RMSNormInt8Kernel(_ScoringKernel):
         _checked(self._lib.va_rms_norm_int8(
             self.context.handle, _strided(dev, x, rows, dimension, xs, item, "x"),
             None if residual is None else _strided(dev, residual, rows, dimension, rs, item, "residual"),
-            _dense(dev, weight, dimension * item, "weight"), rows, dimension, dtype, xs, rs, epsilon, group,
-            None if residual_out is None else _dense(dev, residual_out, n * item, "residual_out"),
-            _dense(dev, codes, n, "codes"), _dense(dev, scales, rows * groups * 4, "scales")), "va_rms_norm_int8")
+            _dense(dev, weight, dimension, item, "weight"), rows, dimension, dtype, xs, rs, epsilon, group,
+            None if residual_out is None else _dense(dev, residual_out, n, item, "residual_out"),
+            _dense(dev, codes, n, 1, "codes"), _dense(dev, scales, rows * groups, 4, "scales")), "va_rms_norm_int8")
 
     def compute(self, x, weight, residual=None, epsilon: float = 1e-6, group: int = 0):
         """fp32 host arrays -> (codes int8 [rows, dim], scales [rows, groups], h [rows, dim])."""
@@ -179,9 +199,9 @@ class Int4GroupQuantizationKernel(_ScoringKernel):
         groups = -(-dimension // group)
         _checked(self._lib.va_sq_quantize_int4_groups(
             self.context.handle, _strided(dev, x, rows, dimension, stride, _ITEM[dtype], "x"), dtype, rows, dimension, stride,
-            group, scale_dtype, _dense(dev, codes, rows * int4_row_bytes(dimension), "codes"),
-            _dense(dev, scales, rows * groups * _ITEM[scale_dtype], "scales"),
-            None if zero_points is None else _dense(dev, zero_points, rows * groups, "zero_points")),
+            group, scale_dtype, _dense(dev, codes, rows * int4_row_bytes(dimension), 1, "codes"),
+            _dense(dev, scales, rows * groups, _ITEM[scale_dtype], "scales"),
+            None if zero_points is None else _dense(dev, zero_points, rows * groups, 1, "zero_points")),
             "va_sq_quantize_int4_groups")
 
     def quantize(self, rows, group: int = 64, type: str = "symmetric",  # noqa: A002
@@ -236,11 +256,11 @@ class Int4MatVecKernel(_ScoringKernel):
         stride = rows if out_stride is None else out_stride
         groups = -(-dimension // group)
         _checked(self._lib.va_int4_matvec(
-            self.context.handle, _dense(dev, queries, num_queries * dimension * _ITEM[query_dtype], "queries"), query_dtype,
-            None if query_scales is None else _dense(dev, query_scales, num_queries * 4, "query_scales"), num_queries,
-            _dense(dev, codes, rows * int4_row_bytes(dimension), "codes"),
-            _dense(dev, scales, rows * groups * _ITEM[scale_dtype], "scales"),
-            None if zero_points is None else _dense(dev, zero_points, rows * groups, "zero_points"), rows, dimension, group,
+            self.context.handle, _dense(dev, queries, num_queries * dimension, _ITEM[query_dtype], "queries"), query_dtype,
+            None if query_scales is None else _dense(dev, query_scales, num_queries, 4, "query_scales"), num_queries,
+            _dense(dev, codes, rows * int4_row_bytes(dimension), 1, "codes"),
+            _dense(dev, scales, rows * groups, _ITEM[scale_dtype], "scales"),
+            None if zero_points is None else _dense(dev, zero_points, rows * groups, 1, "zero_points"), rows, dimension, group,
             scale_dtype, _strided(dev, out, num_queries, rows, stride, 4, "out"), stride), "va_int4_matvec")
 
     def compute(self, queries, table: Int4Rows) -> np.ndarray:
@@ -325,7 +345,12 @@ class SoftmaxCrossEntropyKernel(_ScoringKernel):
             return None, 0
         if isinstance(workspace, int):
             return workspace, self.workspace_bytes(tokens, rows, dimension, backward)
-        return _dense(self._device, workspace, 0, "workspace"), workspace.nbytes
+        if not hasattr(workspace, "data_ptr"):
+            return _buffer(self._device, workspace, 0, "workspace"), workspace.nbytes
+        _device_of(self._device, workspace, "workspace")
+        if not workspace.is_contiguous():
+            raise InvalidInput("workspace must be contiguous")
+        return workspace.data_ptr(), workspace.nbytes
 
     def encode_forward(self, hidden, table, labels, tokens: int, rows: int, dimension: int, loss, lse,
                        logit_scale: float = 1.0, hidden_stride: int | None = None, table_stride: int | None = None,
@@ -338,8 +363,8 @@ class SoftmaxCrossEntropyKernel(_ScoringKernel):
         ws, nbytes = self._workspace(workspace, tokens, rows, dimension, False)
         _checked(self._lib.va_softmax_xent_forward(
             self.context.handle, _strided(dev, hidden, tokens, dimension, hs, 2, "hidden"), hs,
-            self._table(table, rows, dimension, ts), ts, _dense(dev, labels, tokens * 8, "labels"), tokens, rows, dimension,
-            logit_scale, ws, nbytes, _dense(dev, loss, tokens * 4, "loss"), _dense(dev, lse, tokens * 4, "lse")),
+            self._table(table, rows, dimension, ts), ts, _dense(dev, labels, tokens, 8, "labels"), tokens, rows, dimension,
+            logit_scale, ws, nbytes, _dense(dev, loss, tokens, 4, "loss"), _dense(dev, lse, tokens, 4, "lse")),
             "va_softmax_xent_forward")
 
     def encode_backward(self, hidden, table, labels, lse, grad_loss, tokens: int, rows: int, dimension: int, grad_hidden,
@@ -352,10 +377,10 @@ class SoftmaxCrossEntropyKernel(_ScoringKernel):
         ws, nbytes = self._workspace(workspace, tokens, rows, dimension, True)
         _checked(self._lib.va_softmax_xent_backward(
             self.context.handle, _strided(dev, hidden, tokens, dimension, hs, 2, "hidden"), hs,
-            self._table(table, rows, dimension, ts), ts, _dense(dev, labels, tokens * 8, "labels"),
-            _dense(dev, lse, tokens * 4, "lse"), None if grad_loss is None else _dense(dev, grad_loss, tokens * 4, "grad_loss"),
-            tokens, rows, dimension, logit_scale, ws, nbytes, _dense(dev, grad_hidden, tokens * dimension * 2, "grad_hidden"),
-            _dense(dev, grad_table, rows * dimension * 2, "grad_table")), "va_softmax_xent_backward")
+            self._table(table, rows, dimension, ts), ts, _dense(dev, labels, tokens, 8, "labels"),
+            _dense(dev, lse, tokens, 4, "lse"), None if grad_loss is None else _dense(dev, grad_loss, tokens, 4, "grad_loss"),
+            tokens, rows, dimension, logit_scale, ws, nbytes, _dense(dev, grad_hidden, tokens * dimension, 2, "grad_hidden"),
+            _dense(dev, grad_table, rows * dimension, 2, "grad_table")), "va_softmax_xent_backward")
 
     def compute(self, hidden, table, labels, logit_scale: float = 1.0, grad_loss=None):
         """Host arrays (hidden and table are rounded to bf16) -> (loss [T], lse [T], grad_hidden [T, D],
