@@ -103,6 +103,50 @@ def test_norm_in_place_and_untouched_neighbours(tctx, dtype):
     assert torch.equal(codes.double(), norm_reference(h, w, 1e-6, 0)[0])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows, dim, pad, group, offsets, inplace", [
+    (1, 1, 0, 0, (1, 2, 3, 5), None), (40, 3, 0, 0, (3, 0, 1, 2), None), (20000, 9, 2, 0, (0, 1, 0, 7), None),
+    (9001, 17, 0, 32, (5, 5, 5, 5), "x"), (7000, 255, 0, 64, (7, 3, 2, 1), None), (6001, 256, 1, 0, (1, 0, 0, 3), None),
+    (5000, 257, 0, 128, (0, 0, 0, 0), "residual"), (4000, 511, 3, 0, (2, 4, 6, 4), None), (3001, 513, 0, 32, (0, 6, 0, 0), "x"),
+    (2000, 1023, 0, 0, (4, 4, 4, 0), "residual"), (1500, 1024, 0, 64, (1, 1, 1, 1), None), (1201, 2047, 0, 0, (6, 1, 7, 6), None),
+    (1000, 2050, 0, 128, (0, 0, 0, 0), "x"), (900, 4095, 0, 0, (0, 0, 0, 0), None), (901, 4089, 2, 32, (7, 2, 5, 3), None),
+    (700, 4096, 0, 0, (0, 1, 0, 1), None)])
+def test_norm_rows_at_any_address(tctx, dtype, rows, dim, pad, group, offsets, inplace):
+    # every array at its own offset from a 16-byte boundary, many rows per block, neighbours kept
+    g = gen(dim)
+
+    def at(offset, stride, t, fill):
+        flat = torch.full((offset + rows * stride + 64,), fill, dtype=t, device="cuda")
+        return flat, flat[offset:offset + rows * stride].view(rows, stride)[:, :dim]
+
+    xs, rs, outs = dim + (0 if inplace == "x" else pad), dim, dim
+    fx, x = at(offsets[0], xs, DT[dtype], float("nan"))
+    fr, r = at(offsets[1], rs, DT[dtype], float("nan"))
+    x.copy_((randn(g, rows, dim) * 2).to(DT[dtype]))
+    r.copy_((randn(g, rows, dim) * 3).to(DT[dtype]))
+    w = (1 + 0.3 * randn(g, dim + 1)).to(DT[dtype])[1:]
+    h = (x.float() + r.float()).to(DT[dtype])
+    flat, out = {"x": (fx, x), "residual": (fr, r), None: at(offsets[2], outs, DT[dtype], 55.0)}[inplace]
+    first = offsets[{"x": 0, "residual": 1, None: 2}[inplace]]
+    fc, codes = at(offsets[3], dim, torch.int8, 99)
+    scales = torch.full((rows, -(-dim // group) if group else 1), -1.0, device="cuda")
+    edges = [t.clone() for t in (flat[:first], flat[first + rows * dim:])]
+    va.RMSNormInt8Kernel(tctx).encode(x, w, rows, dim, codes, scales, r, out, VA[dtype], 1e-6, group, xs, rs)
+    tctx.synchronize()
+    want_codes, want_scales = norm_reference(h, w, 1e-6, group)
+    assert torch.equal(out, h)
+    assert torch.equal(codes.double(), want_codes)
+    assert ((scales.double() - want_scales).abs() <= SCALE_TOL * want_scales).all()
+    assert all(torch.equal(torch.nan_to_num(a, 77.0), torch.nan_to_num(b, 77.0))
+               for a, b in zip(edges, (flat[:first], flat[first + rows * dim:])))
+    assert (fc[:offsets[3]] == 99).all() and (fc[offsets[3] + rows * dim:] == 99).all()
+    if not inplace:
+        bare = torch.empty_like(codes)
+        va.RMSNormInt8Kernel(tctx).encode(h, w, rows, dim, bare, scales, dtype=VA[dtype], group=group)
+        tctx.synchronize()
+        assert torch.equal(bare, codes)
+
+
 def test_norm_zero_and_non_finite_rows(tctx):
     x = torch.ones(6, 256, device="cuda")
     x[1] = 0

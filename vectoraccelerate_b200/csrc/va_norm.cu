@@ -52,12 +52,11 @@ struct Vec {
     }
 };
 
-// Eight elements from p, `n` of them inside the row (the others read as 0). W is the widest access in bytes
-// that every row start allows: 16, or the element's size.
-template <typename T, int W>
+// Eight elements from p, `n` of them inside the row (the others read as 0).
+template <typename T, bool ALIGNED>
 __device__ __forceinline__ Vec<T> load8(const T* p, int n) {
     Vec<T> v;
-    if constexpr (W == 16) {
+    if constexpr (ALIGNED) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
             const uint4 u = n > 0 ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0u, 0u, 0u, 0u);
@@ -76,23 +75,49 @@ __device__ __forceinline__ Vec<T> load8(const T* p, int n) {
     return v;
 }
 
-template <typename T, int W>
-__device__ __forceinline__ void store8(T* p, int n, const Vec<T>& v) {
-    if constexpr (W == 16) {
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const Vec<T>& v) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-            reinterpret_cast<uint4*>(p)[i] = make_uint4(v.w[4 * i], v.w[4 * i + 1], v.w[4 * i + 2], v.w[4 * i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) {
-                if constexpr (sizeof(T) == 2)
-                    p[i] = (T)(i & 1 ? v.w[i >> 1] >> 16 : v.w[i >> 1]);
-                else
-                    p[i] = __uint_as_float(v.w[i]);
-            }
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(v.w[4 * i], v.w[4 * i + 1], v.w[4 * i + 2], v.w[4 * i + 3]);
 }
+
+// The eight elements that start `s` elements (less than 16 bytes) into the 16-byte pieces at p in shared memory.
+template <typename T>
+__device__ __forceinline__ Vec<T> window8(const uint4* p, int s) {
+    constexpr int N = sizeof(T) * 2, MORE = sizeof(T) == 2 ? 1 : 0;  // words; one more where halves are joined
+    uint32_t u[N + 4], v[N + MORE + 1];
+#pragma unroll
+    for (int i = 0; i < N / 4 + 1; ++i) {
+        const uint4 q = p[i];
+        u[4 * i] = q.x, u[4 * i + 1] = q.y, u[4 * i + 2] = q.z, u[4 * i + 3] = q.w;
+    }
+    const int words = MORE ? s >> 1 : s;
+#pragma unroll
+    for (int i = 0; i < N + MORE + 1; ++i) v[i] = words & 2 ? u[i + 2] : u[i];
+#pragma unroll
+    for (int i = 0; i < N + MORE; ++i) v[i] = words & 1 ? v[i + 1] : v[i];
+    Vec<T> out;
+    const uint32_t halves = s & 1 ? 0x5432u : 0x3210u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) out.w[i] = MORE ? __byte_perm(v[i], v[i + MORE], halves) : v[i];
+    return out;
+}
+
+// Rows in memory that start anywhere: `past` elements after an 8-element boundary of their own. Elements before `head`
+// and from `tail` on lie in boundaries shared with neighbouring rows and are stored one by one.
+struct Edges {
+    int head, tail;
+    __device__ __forceinline__ Edges(int past, int dim) {
+        head = past ? min(8 - past, dim) : 0;
+        tail = head + ((dim - head) & ~7);
+    }
+    // Which element thread t of the row's first 16 stores, or -1.
+    __device__ __forceinline__ int of(int t, int dim) const {
+        if (t < 8) return t < head ? t : -1;
+        return t < 16 && tail + t - 8 < dim ? tail + t - 8 : -1;
+    }
+};
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t d;
@@ -251,7 +276,14 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-constexpr int STAGES = 3;  // rows per thread in work or on their way (16-byte accesses only)
+// As cp_async16, of the first `bytes`; the rest becomes zero.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// Rows in work or on their way: three, or two where shared memory also holds the results of fp32 rows.
+template <typename T, bool ALIGNED>
+constexpr int stages_of() { return ALIGNED || sizeof(T) == 2 ? 3 : 2; }
 
 // Threads of a block for rows of TPR threads: narrow rows share a block of 128.
 constexpr int threads_of(int tpr) { return tpr < 128 ? 128 : tpr; }
@@ -263,27 +295,72 @@ constexpr int vectors_of() { return sizeof(T) == 2 ? 2 : 1; }
 template <typename T>
 constexpr int blocks_of(int tpr) { return (vectors_of<T>() == 2 ? 768 : 1024) / threads_of(tpr); }
 
+// Shared memory of a block. ALIGNED: [stage][x, residual][vector][piece][thread] of 16 bytes. Else rows as they lie in
+// memory, [stage][x, residual][row][piece], then [2][row][piece] of residual_out and [2][row][vector] of codes (8 bytes).
+template <typename T, bool ALIGNED, int TPR>
+struct Shared {
+    static constexpr int THREADS = threads_of(TPR), ROWS = THREADS / TPR, NV = vectors_of<T>(), HALVES = sizeof(T) / 2;
+    static constexpr int STAGES = stages_of<T, ALIGNED>();
+    static constexpr int PIECES = TPR * NV * HALVES + 1;  // of a row that starts inside its first
+    static constexpr int CODES = TPR * NV + 1;
+    static constexpr int OUT = STAGES * 2 * ROWS * PIECES;
+    static constexpr size_t BYTES = ALIGNED ? (size_t)STAGES * 2 * NV * HALVES * THREADS * 16
+                                            : (size_t)(OUT + 2 * ROWS * PIECES) * 16 + 2 * ROWS * CODES * 8;
+};
+
 // TPR threads per row; vector i of thread t is at (i * TPR + t) * 8.
-template <typename T, int W, int TPR>
+template <typename T, bool ALIGNED, int TPR>
 __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm_int8(NormArgs a) {
-    constexpr int THREADS = threads_of(TPR), ROWS = THREADS / TPR, WARPS = TPR / 32, NV = vectors_of<T>();
-    constexpr int HALVES = sizeof(T) / 2;  // 16-byte pieces of a vector
-    extern __shared__ uint4 s_in[];        // [stage][x, residual][vector][piece][thread]
+    using S = Shared<T, ALIGNED, TPR>;
+    constexpr int THREADS = S::THREADS, ROWS = S::ROWS, WARPS = TPR / 32, NV = S::NV, STAGES = S::STAGES;
+    constexpr int HALVES = S::HALVES;                   // 16-byte pieces of a vector
+    constexpr int A = 16 / sizeof(T), ES = sizeof(T);   // elements of a piece
+    extern __shared__ uint4 s_in[];
     __shared__ float4 s_part[2][ROWS][WARPS];  // (sum, hi, lo, -) of each warp
     const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR, j0 = t * 8;
     Vec<T> w[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) w[i] = load8<T, W>(static_cast<const T*>(a.weight) + j0 + i * TPR * 8, a.dim - j0 - i * TPR * 8);
+    for (int i = 0; i < NV; ++i)
+        w[i] = load8<T, ALIGNED>(static_cast<const T*>(a.weight) + j0 + i * TPR * 8, a.dim - j0 - i * TPR * 8);
     const int64_t step = (int64_t)gridDim.x * ROWS;
     // Every thread of a block makes the same number of turns (barriers); a slot without a row works on zeros.
     int64_t row = (int64_t)blockIdx.x * ROWS + slot, ahead = row;
     int64_t turns = row - slot < a.rows ? (a.rows - (row - slot) + step - 1) / step : 0;
-    const T* px = static_cast<const T*>(a.x) + row * a.x_stride + j0;
-    const T* pr = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride + j0 : nullptr;
+    const int lead = ALIGNED ? j0 : 0;
+    const T* px = static_cast<const T*>(a.x) + row * a.x_stride + lead;
+    const T* pr = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride + lead : nullptr;
+    const auto in_row = [&](int stage, int which) { return s_in + ((stage * 2 + which) * ROWS + slot) * S::PIECES; };
+    const auto out_row = [&](int turn) { return s_in + S::OUT + (turn * ROWS + slot) * S::PIECES; };
+    const auto code_row = [&](int turn) {
+        return reinterpret_cast<uint2*>(s_in + S::OUT + 2 * ROWS * S::PIECES) + (turn * ROWS + slot) * S::CODES;
+    };
+    const auto barrier = [&] {
+        if constexpr (WARPS > 1)
+            __syncthreads();
+        else
+            __syncwarp();
+    };
+    // Elements between a 16-byte boundary and the start of a row.
+    const auto past = [](const void* p, int64_t row, int64_t stride) {
+        return (int)(((uint32_t)((uintptr_t)p / ES) + (uint32_t)row * (uint32_t)stride) & (A - 1));
+    };
+    // The pieces of a row, from the boundary before it (which its allocation holds) to its last element.
+    const auto fetch_pieces = [&](uint4* to, const T* from) {
+        const int before = (int)((uintptr_t)from / ES) & (A - 1), end = (a.dim + before) * ES;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(from - before);
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+#pragma unroll
+        for (int i = 0; i < NV * HALVES; ++i) {
+            const int at = (t + i * TPR) * 16;
+            if (at < end) cp_async16(dst + at, src + at, min(16, end - at));
+        }
+        constexpr int LAST = TPR * NV * HALVES * 16;
+        if (t == 0 && LAST < end) cp_async16(dst + LAST, src + LAST, end - LAST);
+    };
     // Row `ahead` into a stage; px and pr point at it and move on.
     const auto fetch = [&](int stage) {
-        if constexpr (W == 16) {
-            if (ahead < a.rows) {
+        if (ahead < a.rows) {
+            if constexpr (ALIGNED) {
                 const uint32_t dst = (uint32_t)__cvta_generic_to_shared(s_in + stage * 2 * NV * HALVES * THREADS + threadIdx.x);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
@@ -298,52 +375,102 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
                                        reinterpret_cast<const uint4*>(pr + i * TPR * 8) + p);
                     }
                 }
+            } else {
+                fetch_pieces(in_row(stage, 0), px);
+                if (pr) fetch_pieces(in_row(stage, 1), pr);
             }
-            cp_async_commit();
-            ahead += step;
-            px += step * a.x_stride;
-            if (pr) pr += step * a.residual_stride;
         }
+        cp_async_commit();
+        ahead += step;
+        px += step * a.x_stride;
+        if (pr) pr += step * a.residual_stride;
     };
-    // A vector of the current row: from its stage, or from memory where rows have no 16-byte alignment.
-    const auto take = [&](int stage, int which, int i) {
-        if constexpr (W == 16) {
-            Vec<T> v;
+    // A vector of the current row from its stage.
+    const auto take = [&](int stage, int which, int i, int before) {
+        Vec<T> v;
+        if constexpr (ALIGNED) {
             const uint4* from = s_in + ((stage * 2 + which) * NV + i) * HALVES * THREADS + threadIdx.x;
 #pragma unroll
             for (int p = 0; p < HALVES; ++p) {
                 const uint4 u = from[p * THREADS];
                 v.w[4 * p] = u.x, v.w[4 * p + 1] = u.y, v.w[4 * p + 2] = u.z, v.w[4 * p + 3] = u.w;
             }
-            return v;
         } else {
-            return load8<T, W>((which ? pr : px) + i * TPR * 8, a.dim - j0 - i * TPR * 8);
+            v = window8<T>(in_row(stage, which) + (t + i * TPR) * HALVES, before);
+            const int n = a.dim - j0 - i * TPR * 8;
+            if (n < 8) {
+#pragma unroll
+                for (int k = 0; k < (int)sizeof(T) * 2; ++k) {
+                    if constexpr (ES == 2)
+                        v.w[k] = 2 * k + 1 < n ? v.w[k] : 2 * k < n ? v.w[k] & 0xFFFFu : 0u;
+                    else
+                        v.w[k] = k < n ? v.w[k] : 0u;
+                }
+            }
         }
+        return v;
+    };
+    // A row's residual_out and codes from shared memory to any address: whole 16 (codes: 8) bytes and edges.
+    const auto put_out = [&](int turn) {
+        T* out = static_cast<T*>(a.residual_out) + row * a.dim;
+        const int m = past(a.residual_out, row, a.dim);
+        const Edges edge(m, a.dim);
+        const uint4* from = out_row(turn);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int v = t + i * TPR, at = v * 8 - m;
+            if (at >= edge.head && at < edge.tail) store8<T>(out + at, window8<T>(from + v * HALVES - (m ? 1 : 0), (A - m) & (A - 1)));
+        }
+        const int e = edge.of(t, a.dim);
+        if (e >= 0) out[e] = reinterpret_cast<const T*>(from)[e];
+    };
+    const auto put_codes = [&](int turn, int64_t of) {
+        int8_t* out = a.codes + of * a.dim;
+        const int m = (int)((uintptr_t)out & 7), s = (8 - m) & 7;
+        const Edges edge(m, a.dim);
+        const uint2* from = code_row(turn);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int v = t + i * TPR, at = v * 8 - m;
+            if (at >= edge.head && at < edge.tail) {
+                const uint2 p = from[v - (m ? 1 : 0)], q = from[v - (m ? 1 : 0) + 1];
+                const uint32_t u0 = s & 4 ? p.y : p.x, u1 = s & 4 ? q.x : p.y, u2 = s & 4 ? q.y : q.x;
+                *reinterpret_cast<uint2*>(out + at) =
+                    make_uint2(__funnelshift_r(u0, u1, 8 * (s & 3)), __funnelshift_r(u1, u2, 8 * (s & 3)));
+            }
+        }
+        const int e = edge.of(t, a.dim);
+        if (e >= 0) out[e] = reinterpret_cast<const int8_t*>(from)[e];
     };
     for (int s = 0; s < STAGES - 1; ++s) fetch(s);
+    if constexpr (!ALIGNED) {
+        cp_async_wait<STAGES - 2>();
+        barrier();
+    }
     int stage = 0, turn = 0;
     const float mean = 1.f / (float)a.dim;
     for (; turns > 0; --turns, turn ^= 1) {
         // (residual_out may be x's or residual's own rows: a row is stored only after its loads.)
         fetch(stage == 0 ? STAGES - 1 : stage - 1);
-        if constexpr (W == 16) cp_async_wait<STAGES - 1>();
+        if constexpr (ALIGNED) cp_async_wait<STAGES - 1>();
         const bool live = row < a.rows;
+        const int before_x = past(a.x, row, a.x_stride), before_r = past(a.residual, row, a.residual_stride);
         Vec<T> h[NV] = {};
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (live && j0 + i * TPR * 8 < a.dim) {
-                h[i] = take(stage, 0, i);
-                if (a.residual) h[i] = add8<T>(h[i], take(stage, 1, i));
+                h[i] = take(stage, 0, i, before_x);
+                if (a.residual) h[i] = add8<T>(h[i], take(stage, 1, i, before_r));
             }
         if (a.residual_out && live) {
-            T* out = static_cast<T*>(a.residual_out) + row * a.dim + j0;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (j0 + i * TPR * 8 < a.dim) store8<T, W>(out + i * TPR * 8, a.dim - j0 - i * TPR * 8, h[i]);
-        }
-        if constexpr (W != 16) {
-            px += step * a.x_stride;
-            if (pr) pr += step * a.residual_stride;
+                if (j0 + i * TPR * 8 < a.dim) {
+                    if constexpr (ALIGNED)
+                        store8<T>(static_cast<T*>(a.residual_out) + row * a.dim + j0 + i * TPR * 8, h[i]);
+                    else
+                        store8<T>(reinterpret_cast<T*>(out_row(turn)) + j0 + i * TPR * 8, h[i]);
+                }
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         float sum = 0.f, z[NV][8];
@@ -363,10 +490,12 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
             for (int i = 1; i < NV; ++i) top[0].take(top[i].hi, top[i].lo);
             top[0].template lanes<32>();
         }
+        // (Two sets of everything that threads exchange, in turn: one barrier per row.)
+        if constexpr (!ALIGNED) cp_async_wait<STAGES - 2>();  // the next row is there behind the barrier
         if constexpr (WARPS > 1) {
-            // Two sets of slots in turn: one barrier per row. Lane i takes warp i's part, then the lanes add up.
+            // Lane i takes warp i's part, then the lanes add up.
             if ((t & 31) == 0) s_part[turn][slot][t >> 5] = make_float4(sum, top[0].hi, top[0].lo, 0.f);
-            __syncthreads();
+            barrier();
             const float4 p = s_part[turn][slot][t & (WARPS - 1)];
             sum = p.x;
 #pragma unroll
@@ -376,13 +505,18 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
                 top[0].lo = p.z;
                 top[0].template lanes<WARPS>();
             }
+        } else if constexpr (!ALIGNED) {
+            barrier();
+        }
+        if constexpr (!ALIGNED) {
+            if (a.residual_out && live) put_out(turn);
+            if (row >= step) put_codes(turn ^ 1, row - step);  // the row before's (this block's first row is below step)
         }
         if (!a.group) {
 #pragma unroll
             for (int i = 1; i < NV; ++i) top[i] = top[0];
         }
         if (live) {
-            int8_t* codes = a.codes + row * a.dim + j0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int j = j0 + i * TPR * 8;
@@ -395,39 +529,38 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
                 }
                 uint2 packed = make_uint2(0u, 0u);
                 if (ok && top[i].hi >= SMALLEST) packed = codes_of<T>(h[i], w[i], z[i], top[i]);
-                int8_t* to = codes + i * TPR * 8;
-                if constexpr (W == 16) {
-                    *reinterpret_cast<uint2*>(to) = packed;
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (j + k < a.dim) to[k] = (int8_t)((k < 4 ? packed.x : packed.y) >> (8 * (k & 3)));
-                }
+                if constexpr (ALIGNED)
+                    *reinterpret_cast<uint2*>(a.codes + row * a.dim + j) = packed;
+                else
+                    code_row(turn)[t + i * TPR] = packed;
             }
         }
         row += step;
     }
+    if constexpr (!ALIGNED) {
+        barrier();
+        if (row >= step && row - step < a.rows) put_codes(turn ^ 1, row - step);
+    }
 }
 
-template <typename T, int W, int TPR>
+template <typename T, bool ALIGNED, int TPR>
 int launch_rows(va_context* ctx, const NormArgs& a) {
-    constexpr int THREADS = threads_of(TPR), ROWS = THREADS / TPR;
-    constexpr size_t SMEM = W == 16 ? (size_t)STAGES * 2 * vectors_of<T>() * (sizeof(T) / 2) * THREADS * 16 : 0;
-    constexpr auto kern = k_rms_norm_int8<T, W, TPR>;
-    VA_TRY(va_kernel_once<kern>(ctx->device, SMEM));
-    const int64_t grid = std::min<int64_t>((a.rows + ROWS - 1) / ROWS, (int64_t)ctx->sm_count * blocks_of<T>(TPR));
-    kern<<<(unsigned)grid, THREADS, SMEM, ctx->stream>>>(a);
+    using S = Shared<T, ALIGNED, TPR>;
+    constexpr auto kern = k_rms_norm_int8<T, ALIGNED, TPR>;
+    VA_TRY(va_kernel_once<kern>(ctx->device, S::BYTES));
+    const int64_t grid = std::min<int64_t>((a.rows + S::ROWS - 1) / S::ROWS, (int64_t)ctx->sm_count * blocks_of<T>(TPR));
+    kern<<<(unsigned)grid, S::THREADS, S::BYTES, ctx->stream>>>(a);
     return va_check_launch("k_rms_norm_int8");
 }
 
-template <typename T, int W>
+template <typename T, bool ALIGNED>
 int launch_norm(va_context* ctx, const NormArgs& a) {
     constexpr int PER = 8 * vectors_of<T>();  // elements of a thread
-    if (a.dim <= 32 * PER) return launch_rows<T, W, 32>(ctx, a);
-    if (a.dim <= 64 * PER) return launch_rows<T, W, 64>(ctx, a);
-    if (a.dim <= 128 * PER) return launch_rows<T, W, 128>(ctx, a);
-    if (a.dim <= 256 * PER) return launch_rows<T, W, 256>(ctx, a);
-    if constexpr (PER == 8) return launch_rows<T, W, 512>(ctx, a);
+    if (a.dim <= 32 * PER) return launch_rows<T, ALIGNED, 32>(ctx, a);
+    if (a.dim <= 64 * PER) return launch_rows<T, ALIGNED, 64>(ctx, a);
+    if (a.dim <= 128 * PER) return launch_rows<T, ALIGNED, 128>(ctx, a);
+    if (a.dim <= 256 * PER) return launch_rows<T, ALIGNED, 256>(ctx, a);
+    if constexpr (PER == 8) return launch_rows<T, ALIGNED, 512>(ctx, a);
     return VA_ERR_UNSUPPORTED;  // (not reached: 256 * 16 is the largest dimension)
 }
 
@@ -469,8 +602,8 @@ int va_rms_norm_int8(va_context* ctx, const void* x, const void* residual, const
                       (!residual || (aligned16(residual) && residual_stride * es % 16 == 0)) &&
                       (!residual_out || aligned16(residual_out)) && ((uintptr_t)codes & 7) == 0;
     if (dtype == VA_DTYPE_BF16)
-        return wide ? launch_norm<uint16_t, 16>(ctx, a) : launch_norm<uint16_t, 2>(ctx, a);
-    return wide ? launch_norm<float, 16>(ctx, a) : launch_norm<float, 4>(ctx, a);
+        return wide ? launch_norm<uint16_t, true>(ctx, a) : launch_norm<uint16_t, false>(ctx, a);
+    return wide ? launch_norm<float, true>(ctx, a) : launch_norm<float, false>(ctx, a);
 }
 
 }  // extern "C"
