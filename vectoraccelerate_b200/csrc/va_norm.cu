@@ -208,9 +208,15 @@ struct Top {
     }
     template <int WIDTH>
     __device__ __forceinline__ void lanes() {
-        if constexpr (sizeof(T) == 2 && WIDTH == 32) {
-            // non-negative floats (and a NaN above them) order like their bits
-            hi = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(hi)));
+        if constexpr (WIDTH == 32) {
+            // non-negative floats (and a NaN above them) order like their bits, negative ones against them
+            const uint32_t own = __float_as_uint(hi), top = __reduce_max_sync(0xFFFFFFFFu, own);
+            if constexpr (sizeof(T) == 4) {
+                const auto ordered = [](int b) { return b ^ ((b >> 31) & 0x7FFFFFFF); };
+                const int low = __reduce_max_sync(0xFFFFFFFFu, own == top ? ordered(__float_as_int(lo)) : (int)0x80000000);
+                lo = __int_as_float(ordered(low));
+            }
+            hi = __uint_as_float(top);
         } else {
 #pragma unroll
             for (int o = 1; o < WIDTH; o <<= 1) {
@@ -293,7 +299,7 @@ template <typename T>
 constexpr int vectors_of() { return sizeof(T) == 2 ? 2 : 1; }
 // Blocks per SM: 768 threads of up to 80 registers, or 1024 of 64.
 template <typename T>
-constexpr int blocks_of(int tpr) { return (vectors_of<T>() == 2 ? 768 : 1024) / threads_of(tpr); }
+constexpr int blocks_of(int tpr) { return (tpr < 512 ? 768 : 1024) / threads_of(tpr); }
 
 // Shared memory of a block. ALIGNED: [stage][x, residual][vector][piece][thread] of 16 bytes. Else rows as they lie in
 // memory, [stage][x, residual][row][piece], then [2][row][piece] of residual_out and [2][row][vector] of codes (8 bytes).
@@ -307,6 +313,40 @@ struct Shared {
     static constexpr size_t BYTES = ALIGNED ? (size_t)STAGES * 2 * NV * HALVES * THREADS * 16
                                             : (size_t)(OUT + 2 * ROWS * PIECES) * 16 + 2 * ROWS * CODES * 8;
 };
+
+// A row's residual_out and codes from shared memory to any address: whole 16 (codes: 8) bytes and edges. A thread's
+// vectors are t, t + TPR, ...
+template <typename T, int NV, int TPR>
+__device__ __forceinline__ void put_row(T* out, int dim, const uint4* from, int t) {
+    constexpr int A = 16 / sizeof(T), HALVES = sizeof(T) / 2;
+    const int m = (int)((uintptr_t)out / sizeof(T)) & (A - 1);
+    const Edges edge(m, dim);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = t + i * TPR, at = v * 8 - m;
+        if (at >= edge.head && at < edge.tail)
+            store8<T>(out + at, window8<T>(from + v * HALVES - (m ? 1 : 0), (A - m) & (A - 1)));
+    }
+    const int e = edge.of(t, dim);
+    if (e >= 0) out[e] = reinterpret_cast<const T*>(from)[e];
+}
+
+template <int NV, int TPR>
+__device__ __forceinline__ void put_codes(int8_t* out, int dim, const uint2* from, int t) {
+    const int m = (int)((uintptr_t)out & 7), s = (8 - m) & 7;
+    const Edges edge(m, dim);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = t + i * TPR, at = v * 8 - m;
+        if (at >= edge.head && at < edge.tail) {
+            const uint2 p = from[v - (m ? 1 : 0)], q = from[v - (m ? 1 : 0) + 1];
+            const uint32_t u0 = s & 4 ? p.y : p.x, u1 = s & 4 ? q.x : p.y, u2 = s & 4 ? q.y : q.x;
+            *reinterpret_cast<uint2*>(out + at) = make_uint2(__funnelshift_r(u0, u1, 8 * (s & 3)), __funnelshift_r(u1, u2, 8 * (s & 3)));
+        }
+    }
+    const int e = edge.of(t, dim);
+    if (e >= 0) out[e] = reinterpret_cast<const int8_t*>(from)[e];
+}
 
 // TPR threads per row; vector i of thread t is at (i * TPR + t) * 8.
 template <typename T, bool ALIGNED, int TPR>
@@ -410,38 +450,6 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
         }
         return v;
     };
-    // A row's residual_out and codes from shared memory to any address: whole 16 (codes: 8) bytes and edges.
-    const auto put_out = [&](int turn) {
-        T* out = static_cast<T*>(a.residual_out) + row * a.dim;
-        const int m = past(a.residual_out, row, a.dim);
-        const Edges edge(m, a.dim);
-        const uint4* from = out_row(turn);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int v = t + i * TPR, at = v * 8 - m;
-            if (at >= edge.head && at < edge.tail) store8<T>(out + at, window8<T>(from + v * HALVES - (m ? 1 : 0), (A - m) & (A - 1)));
-        }
-        const int e = edge.of(t, a.dim);
-        if (e >= 0) out[e] = reinterpret_cast<const T*>(from)[e];
-    };
-    const auto put_codes = [&](int turn, int64_t of) {
-        int8_t* out = a.codes + of * a.dim;
-        const int m = (int)((uintptr_t)out & 7), s = (8 - m) & 7;
-        const Edges edge(m, a.dim);
-        const uint2* from = code_row(turn);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int v = t + i * TPR, at = v * 8 - m;
-            if (at >= edge.head && at < edge.tail) {
-                const uint2 p = from[v - (m ? 1 : 0)], q = from[v - (m ? 1 : 0) + 1];
-                const uint32_t u0 = s & 4 ? p.y : p.x, u1 = s & 4 ? q.x : p.y, u2 = s & 4 ? q.y : q.x;
-                *reinterpret_cast<uint2*>(out + at) =
-                    make_uint2(__funnelshift_r(u0, u1, 8 * (s & 3)), __funnelshift_r(u1, u2, 8 * (s & 3)));
-            }
-        }
-        const int e = edge.of(t, a.dim);
-        if (e >= 0) out[e] = reinterpret_cast<const int8_t*>(from)[e];
-    };
     for (int s = 0; s < STAGES - 1; ++s) fetch(s);
     if constexpr (!ALIGNED) {
         cp_async_wait<STAGES - 2>();
@@ -463,14 +471,10 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
                 if (a.residual) h[i] = add8<T>(h[i], take(stage, 1, i, before_r));
             }
         if (a.residual_out && live) {
+            T* out = (ALIGNED ? static_cast<T*>(a.residual_out) + row * a.dim : reinterpret_cast<T*>(out_row(turn))) + j0;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (j0 + i * TPR * 8 < a.dim) {
-                    if constexpr (ALIGNED)
-                        store8<T>(static_cast<T*>(a.residual_out) + row * a.dim + j0 + i * TPR * 8, h[i]);
-                    else
-                        store8<T>(reinterpret_cast<T*>(out_row(turn)) + j0 + i * TPR * 8, h[i]);
-                }
+                if (j0 + i * TPR * 8 < a.dim) store8<T>(out + i * TPR * 8, h[i]);
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         float sum = 0.f, z[NV][8];
@@ -503,20 +507,22 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
             if (!a.group) {
                 top[0].hi = p.y;
                 top[0].lo = p.z;
-                top[0].template lanes<WARPS>();
+                top[0].template lanes<32>();  // (each warp's part is there 32 / WARPS times)
             }
         } else if constexpr (!ALIGNED) {
             barrier();
         }
         if constexpr (!ALIGNED) {
-            if (a.residual_out && live) put_out(turn);
-            if (row >= step) put_codes(turn ^ 1, row - step);  // the row before's (this block's first row is below step)
+            if (a.residual_out && live) put_row<T, NV, TPR>(static_cast<T*>(a.residual_out) + row * a.dim, a.dim, out_row(turn), t);
+            // the row before's (this block's first row is below step)
+            if (row >= step) put_codes<NV, TPR>(a.codes + (row - step) * a.dim, a.dim, code_row(turn ^ 1), t);
         }
         if (!a.group) {
 #pragma unroll
             for (int i = 1; i < NV; ++i) top[i] = top[0];
         }
         if (live) {
+            uint2* codes = ALIGNED ? reinterpret_cast<uint2*>(a.codes + row * a.dim + j0) : code_row(turn) + t;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int j = j0 + i * TPR * 8;
@@ -529,17 +535,14 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
                 }
                 uint2 packed = make_uint2(0u, 0u);
                 if (ok && top[i].hi >= SMALLEST) packed = codes_of<T>(h[i], w[i], z[i], top[i]);
-                if constexpr (ALIGNED)
-                    *reinterpret_cast<uint2*>(a.codes + row * a.dim + j) = packed;
-                else
-                    code_row(turn)[t + i * TPR] = packed;
+                codes[i * TPR] = packed;
             }
         }
         row += step;
     }
     if constexpr (!ALIGNED) {
         barrier();
-        if (row >= step && row - step < a.rows) put_codes(turn ^ 1, row - step);
+        if (row >= step && row - step < a.rows) put_codes<NV, TPR>(a.codes + (row - step) * a.dim, a.dim, code_row(turn ^ 1), t);
     }
 }
 
