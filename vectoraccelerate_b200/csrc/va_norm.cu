@@ -287,31 +287,26 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// Rows in work or on their way: three, or two where shared memory also holds the results of fp32 rows.
-template <typename T, bool ALIGNED>
-constexpr int stages_of() { return ALIGNED || sizeof(T) == 2 ? 3 : 2; }
-
-// Threads of a block for rows of TPR threads: narrow rows share a block of 128.
-constexpr int threads_of(int tpr) { return tpr < 128 ? 128 : tpr; }
-// Vectors of 8 elements per thread: two share the reductions' cost (bf16, 65536 x 4096: 316 us, with one 390 us);
-// two of fp32 overflow the registers (10007 x 1000: 31 us, with one 25 us).
-template <typename T>
-constexpr int vectors_of() { return sizeof(T) == 2 ? 2 : 1; }
-// Blocks per SM: 768 threads of up to 80 registers, or 1024 of 64.
-template <typename T>
-constexpr int blocks_of(int tpr) { return (tpr < 512 ? 768 : 1024) / threads_of(tpr); }
-
-// Shared memory of a block. ALIGNED: [stage][x, residual][vector][piece][thread] of 16 bytes. Else rows as they lie in
-// memory, [stage][x, residual][row][piece], then [2][row][piece] of residual_out and [2][row][vector] of codes (8 bytes).
-template <typename T, bool ALIGNED, int TPR>
-struct Shared {
-    static constexpr int THREADS = threads_of(TPR), ROWS = THREADS / TPR, NV = vectors_of<T>(), HALVES = sizeof(T) / 2;
-    static constexpr int STAGES = stages_of<T, ALIGNED>();
+// A block works on one row at a time with TPR threads of NV vectors (8 elements) each. (Narrow rows do not share a
+// block: with rows, addresses and barriers of a warp's own, 200000 x 128 bf16 took 72 us instead of 68.) Two vectors
+// share the reductions' cost (bf16, 65536 x 4096: 316 us, with one 390 us); two of fp32 overflow the registers
+// (10007 x 1000: 31 us, with one 25 us).
+template <typename T, bool ALIGNED, int TPR, int NV>
+struct Plan {
+    static constexpr int HALVES = sizeof(T) / 2;  // 16-byte pieces of a vector
+    // Rows in work or on their way. (Three: 65536 x 4096 bf16 with residual 338 us instead of 293.)
+    static constexpr int STAGES = 2;
+    // Shared memory. ALIGNED: [stage][x, residual][vector][piece][thread] of 16 bytes. Else rows as they lie in
+    // memory, [stage][x, residual][piece], then [2][piece] of residual_out and [2][vector] of codes (8 bytes).
     static constexpr int PIECES = TPR * NV * HALVES + 1;  // of a row that starts inside its first
     static constexpr int CODES = TPR * NV + 1;
-    static constexpr int OUT = STAGES * 2 * ROWS * PIECES;
-    static constexpr size_t BYTES = ALIGNED ? (size_t)STAGES * 2 * NV * HALVES * THREADS * 16
-                                            : (size_t)(OUT + 2 * ROWS * PIECES) * 16 + 2 * ROWS * CODES * 8;
+    static constexpr int OUT = STAGES * 2 * PIECES;
+    static constexpr int BYTES = ALIGNED ? STAGES * 2 * NV * HALVES * TPR * 16 : (OUT + 2 * PIECES) * 16 + 2 * CODES * 8;
+    // Blocks per SM: 768 threads of up to 80 registers, or 512 of 128 where two fp32 vectors take them, if their
+    // shared memory (with 1 KB of the system's and the static part) fits the SM's 228 KB: all blocks have to run at once.
+    static constexpr int WANTED = (sizeof(T) * NV == 8 ? 512 : 768) / TPR;
+    static constexpr int FIT = 228 * 1024 / (BYTES + 1024 + TPR / 32 * 32);
+    static constexpr int BLOCKS = WANTED < FIT ? WANTED : FIT;
 };
 
 // A row's residual_out and codes from shared memory to any address: whole 16 (codes: 8) bytes and edges. A thread's
@@ -348,32 +343,27 @@ __device__ __forceinline__ void put_codes(int8_t* out, int dim, const uint2* fro
     if (e >= 0) out[e] = reinterpret_cast<const int8_t*>(from)[e];
 }
 
-// TPR threads per row; vector i of thread t is at (i * TPR + t) * 8.
-template <typename T, bool ALIGNED, int TPR>
-__global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm_int8(NormArgs a) {
-    using S = Shared<T, ALIGNED, TPR>;
-    constexpr int THREADS = S::THREADS, ROWS = S::ROWS, WARPS = TPR / 32, NV = S::NV, STAGES = S::STAGES;
-    constexpr int HALVES = S::HALVES;                   // 16-byte pieces of a vector
-    constexpr int A = 16 / sizeof(T), ES = sizeof(T);   // elements of a piece
+// Vector i of thread t is at (i * TPR + t) * 8.
+template <typename T, bool ALIGNED, int TPR, int NV>
+__global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_norm_int8(NormArgs a) {
+    using P = Plan<T, ALIGNED, TPR, NV>;
+    constexpr int WARPS = TPR / 32, STAGES = P::STAGES, HALVES = P::HALVES;
+    constexpr int A = 16 / sizeof(T), ES = sizeof(T);  // elements of a piece
     extern __shared__ uint4 s_in[];
-    __shared__ float4 s_part[2][ROWS][WARPS];  // (sum, hi, lo, -) of each warp
-    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR, j0 = t * 8;
+    __shared__ float4 s_part[2][WARPS];  // (sum, hi, lo, -) of each warp
+    const int t = threadIdx.x, j0 = t * 8;
     Vec<T> w[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         w[i] = load8<T, ALIGNED>(static_cast<const T*>(a.weight) + j0 + i * TPR * 8, a.dim - j0 - i * TPR * 8);
-    const int64_t step = (int64_t)gridDim.x * ROWS;
-    // Every thread of a block makes the same number of turns (barriers); a slot without a row works on zeros.
-    int64_t row = (int64_t)blockIdx.x * ROWS + slot, ahead = row;
-    int64_t turns = row - slot < a.rows ? (a.rows - (row - slot) + step - 1) / step : 0;
+    const int64_t step = gridDim.x;
+    int64_t row = blockIdx.x, ahead = row;
     const int lead = ALIGNED ? j0 : 0;
     const T* px = static_cast<const T*>(a.x) + row * a.x_stride + lead;
     const T* pr = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride + lead : nullptr;
-    const auto in_row = [&](int stage, int which) { return s_in + ((stage * 2 + which) * ROWS + slot) * S::PIECES; };
-    const auto out_row = [&](int turn) { return s_in + S::OUT + (turn * ROWS + slot) * S::PIECES; };
-    const auto code_row = [&](int turn) {
-        return reinterpret_cast<uint2*>(s_in + S::OUT + 2 * ROWS * S::PIECES) + (turn * ROWS + slot) * S::CODES;
-    };
+    const auto in_row = [&](int stage, int which) { return s_in + (stage * 2 + which) * P::PIECES; };
+    const auto out_row = [&](int turn) { return s_in + P::OUT + turn * P::PIECES; };
+    const auto code_row = [&](int turn) { return reinterpret_cast<uint2*>(s_in + P::OUT + 2 * P::PIECES) + turn * P::CODES; };
     const auto barrier = [&] {
         if constexpr (WARPS > 1)
             __syncthreads();
@@ -401,17 +391,17 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
     const auto fetch = [&](int stage) {
         if (ahead < a.rows) {
             if constexpr (ALIGNED) {
-                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(s_in + stage * 2 * NV * HALVES * THREADS + threadIdx.x);
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(s_in + stage * 2 * NV * HALVES * TPR + t);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     if (j0 + i * TPR * 8 >= a.dim) continue;
 #pragma unroll
                     for (int p = 0; p < HALVES; ++p)
-                        cp_async16(dst + (i * HALVES + p) * THREADS * 16, reinterpret_cast<const uint4*>(px + i * TPR * 8) + p);
+                        cp_async16(dst + (i * HALVES + p) * TPR * 16, reinterpret_cast<const uint4*>(px + i * TPR * 8) + p);
                     if (pr) {
 #pragma unroll
                         for (int p = 0; p < HALVES; ++p)
-                            cp_async16(dst + ((NV + i) * HALVES + p) * THREADS * 16,
+                            cp_async16(dst + ((NV + i) * HALVES + p) * TPR * 16,
                                        reinterpret_cast<const uint4*>(pr + i * TPR * 8) + p);
                     }
                 }
@@ -429,10 +419,10 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
     const auto take = [&](int stage, int which, int i, int before) {
         Vec<T> v;
         if constexpr (ALIGNED) {
-            const uint4* from = s_in + ((stage * 2 + which) * NV + i) * HALVES * THREADS + threadIdx.x;
+            const uint4* from = s_in + ((stage * 2 + which) * NV + i) * HALVES * TPR + t;
 #pragma unroll
             for (int p = 0; p < HALVES; ++p) {
-                const uint4 u = from[p * THREADS];
+                const uint4 u = from[p * TPR];
                 v.w[4 * p] = u.x, v.w[4 * p + 1] = u.y, v.w[4 * p + 2] = u.z, v.w[4 * p + 3] = u.w;
             }
         } else {
@@ -457,20 +447,19 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
     }
     int stage = 0, turn = 0;
     const float mean = 1.f / (float)a.dim;
-    for (; turns > 0; --turns, turn ^= 1) {
+    for (; row < a.rows; row += step, turn ^= 1) {
         // (residual_out may be x's or residual's own rows: a row is stored only after its loads.)
         fetch(stage == 0 ? STAGES - 1 : stage - 1);
         if constexpr (ALIGNED) cp_async_wait<STAGES - 1>();
-        const bool live = row < a.rows;
         const int before_x = past(a.x, row, a.x_stride), before_r = past(a.residual, row, a.residual_stride);
         Vec<T> h[NV] = {};
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (live && j0 + i * TPR * 8 < a.dim) {
+            if (j0 + i * TPR * 8 < a.dim) {
                 h[i] = take(stage, 0, i, before_x);
                 if (a.residual) h[i] = add8<T>(h[i], take(stage, 1, i, before_r));
             }
-        if (a.residual_out && live) {
+        if (a.residual_out) {
             T* out = (ALIGNED ? static_cast<T*>(a.residual_out) + row * a.dim : reinterpret_cast<T*>(out_row(turn))) + j0;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
@@ -498,9 +487,9 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
         if constexpr (!ALIGNED) cp_async_wait<STAGES - 2>();  // the next row is there behind the barrier
         if constexpr (WARPS > 1) {
             // Lane i takes warp i's part, then the lanes add up.
-            if ((t & 31) == 0) s_part[turn][slot][t >> 5] = make_float4(sum, top[0].hi, top[0].lo, 0.f);
+            if ((t & 31) == 0) s_part[turn][t >> 5] = make_float4(sum, top[0].hi, top[0].lo, 0.f);
             barrier();
-            const float4 p = s_part[turn][slot][t & (WARPS - 1)];
+            const float4 p = s_part[turn][t & (WARPS - 1)];
             sum = p.x;
 #pragma unroll
             for (int o = 1; o < WARPS; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
@@ -513,58 +502,53 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of<T>(TPR)) k_rms_norm
             barrier();
         }
         if constexpr (!ALIGNED) {
-            if (a.residual_out && live) put_row<T, NV, TPR>(static_cast<T*>(a.residual_out) + row * a.dim, a.dim, out_row(turn), t);
-            // the row before's (this block's first row is below step)
+            if (a.residual_out) put_row<T, NV, TPR>(static_cast<T*>(a.residual_out) + row * a.dim, a.dim, out_row(turn), t);
+            // the row before's (a block's first row is below step)
             if (row >= step) put_codes<NV, TPR>(a.codes + (row - step) * a.dim, a.dim, code_row(turn ^ 1), t);
         }
         if (!a.group) {
 #pragma unroll
             for (int i = 1; i < NV; ++i) top[i] = top[0];
         }
-        if (live) {
-            uint2* codes = ALIGNED ? reinterpret_cast<uint2*>(a.codes + row * a.dim + j0) : code_row(turn) + t;
+        uint2* codes = ALIGNED ? reinterpret_cast<uint2*>(a.codes + row * a.dim + j0) : code_row(turn) + t;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int j = j0 + i * TPR * 8;
-                if (j >= a.dim) continue;
-                const bool ok = sum < INFINITY && top[i].hi < INFINITY;  // false for NaN too
-                if (a.group ? (j & (a.group - 1)) == 0 : j == 0) {
-                    const float per = rsqrtf(sum * mean + a.eps) * (1.f / 127.f);
-                    a.scales[row * a.groups + (a.group ? j / a.group : 0)] =
-                        !ok ? __int_as_float(0x7FC00000) : top[i].hi >= SMALLEST ? top[i].hi * per : 0.f;
-                }
-                uint2 packed = make_uint2(0u, 0u);
-                if (ok && top[i].hi >= SMALLEST) packed = codes_of<T>(h[i], w[i], z[i], top[i]);
-                codes[i * TPR] = packed;
+        for (int i = 0; i < NV; ++i) {
+            const int j = j0 + i * TPR * 8;
+            if (j >= a.dim) continue;
+            const bool ok = sum < INFINITY && top[i].hi < INFINITY;  // false for NaN too
+            if (a.group ? (j & (a.group - 1)) == 0 : j == 0) {
+                const float per = rsqrtf(sum * mean + a.eps) * (1.f / 127.f);
+                a.scales[row * a.groups + (a.group ? j / a.group : 0)] =
+                    !ok ? __int_as_float(0x7FC00000) : top[i].hi >= SMALLEST ? top[i].hi * per : 0.f;
             }
+            uint2 packed = make_uint2(0u, 0u);
+            if (ok && top[i].hi >= SMALLEST) packed = codes_of<T>(h[i], w[i], z[i], top[i]);
+            codes[i * TPR] = packed;
         }
-        row += step;
     }
     if constexpr (!ALIGNED) {
         barrier();
-        if (row >= step && row - step < a.rows) put_codes<NV, TPR>(a.codes + (row - step) * a.dim, a.dim, code_row(turn ^ 1), t);
+        put_codes<NV, TPR>(a.codes + (row - step) * a.dim, a.dim, code_row(turn ^ 1), t);
     }
 }
 
-template <typename T, bool ALIGNED, int TPR>
+template <typename T, bool ALIGNED, int TPR, int NV>
 int launch_rows(va_context* ctx, const NormArgs& a) {
-    using S = Shared<T, ALIGNED, TPR>;
-    constexpr auto kern = k_rms_norm_int8<T, ALIGNED, TPR>;
-    VA_TRY(va_kernel_once<kern>(ctx->device, S::BYTES));
-    const int64_t grid = std::min<int64_t>((a.rows + S::ROWS - 1) / S::ROWS, (int64_t)ctx->sm_count * blocks_of<T>(TPR));
-    kern<<<(unsigned)grid, S::THREADS, S::BYTES, ctx->stream>>>(a);
+    using P = Plan<T, ALIGNED, TPR, NV>;
+    constexpr auto kern = k_rms_norm_int8<T, ALIGNED, TPR, NV>;
+    VA_TRY(va_kernel_once<kern>(ctx->device, P::BYTES));
+    const int64_t grid = std::min<int64_t>(a.rows, (int64_t)ctx->sm_count * P::BLOCKS);
+    kern<<<(unsigned)grid, TPR, P::BYTES, ctx->stream>>>(a);
     return va_check_launch("k_rms_norm_int8");
 }
 
 template <typename T, bool ALIGNED>
 int launch_norm(va_context* ctx, const NormArgs& a) {
-    constexpr int PER = 8 * vectors_of<T>();  // elements of a thread
-    if (a.dim <= 32 * PER) return launch_rows<T, ALIGNED, 32>(ctx, a);
-    if (a.dim <= 64 * PER) return launch_rows<T, ALIGNED, 64>(ctx, a);
-    if (a.dim <= 128 * PER) return launch_rows<T, ALIGNED, 128>(ctx, a);
-    if (a.dim <= 256 * PER) return launch_rows<T, ALIGNED, 256>(ctx, a);
-    if constexpr (PER == 8) return launch_rows<T, ALIGNED, 512>(ctx, a);
-    return VA_ERR_UNSUPPORTED;  // (not reached: 256 * 16 is the largest dimension)
+    if (a.dim <= 256) return launch_rows<T, ALIGNED, 32, 1>(ctx, a);
+    if (a.dim <= 512) return launch_rows<T, ALIGNED, 32, 2>(ctx, a);
+    if (a.dim <= 1024) return launch_rows<T, ALIGNED, 64, 2>(ctx, a);
+    if (a.dim <= 2048) return launch_rows<T, ALIGNED, 128, 2>(ctx, a);
+    return launch_rows<T, ALIGNED, 256, 2>(ctx, a);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
