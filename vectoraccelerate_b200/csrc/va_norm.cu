@@ -14,11 +14,13 @@
 //
 // The work is one read of x and residual, one write of residual_out and the codes: HBM-bound, with
 // ~20 instructions per element to hide. A thread holds one or two vectors of 8 elements of a row in registers between
-// the statistics and the codes, so nothing is read twice. Blocks are persistent: each thread's vectors of
-// the next rows come through cp.async into shared memory of its own (no barrier), the weights stay in
-// registers, and a row costs one block barrier. Measured: 65536 x 4096 bf16 with residual 310 us, 6.0 TB/s; without a
-// residual (3 bytes an element) the instructions show: 16384 x 4096 70 us, 2.9 TB/s. Rows without 16-byte alignment are
-// read and written element by element, at a quarter to a half of that rate.
+// the statistics and the codes, so nothing is read twice. Blocks are persistent: while a row is worked on the next one
+// comes through cp.async into shared memory, the weights stay in registers, and a row costs one block barrier.
+// Measured: 65536 x 4096 bf16 with residual 291 us, 6.5 TB/s; 32768 x 4096 fp32 394 us, 4.4 TB/s; without a residual
+// (3 bytes an element) the instructions show: 65536 x 4096 bf16 244 us, 3.3 TB/s.
+// Rows that do not start on 16-byte boundaries are copied as the 16-byte pieces that hold them and cut out by shifts;
+// results go through shared memory to whole 16-byte (codes: 8-byte) stores, one row later for the codes: 32768 x 4091 fp32
+// within 2% of the aligned time, 16384 x 4095 bf16 with residual 140 us (element by element 281, aligned 78).
 #include <algorithm>
 
 #include "va_internal.cuh"
@@ -356,11 +358,11 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         w[i] = load8<T, ALIGNED>(static_cast<const T*>(a.weight) + j0 + i * TPR * 8, a.dim - j0 - i * TPR * 8);
-    const int64_t step = gridDim.x;
-    int64_t row = blockIdx.x, ahead = row;
+    const uint32_t step = gridDim.x, rows = (uint32_t)a.rows;  // (below 2^31: a row index plus step fits)
+    uint32_t row = blockIdx.x, ahead = row;
     const int lead = ALIGNED ? j0 : 0;
-    const T* px = static_cast<const T*>(a.x) + row * a.x_stride + lead;
-    const T* pr = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride + lead : nullptr;
+    const T* px = static_cast<const T*>(a.x) + (int64_t)row * a.x_stride + lead;
+    const T* pr = a.residual ? static_cast<const T*>(a.residual) + (int64_t)row * a.residual_stride + lead : nullptr;
     const auto in_row = [&](int stage, int which) { return s_in + (stage * 2 + which) * P::PIECES; };
     const auto out_row = [&](int turn) { return s_in + P::OUT + turn * P::PIECES; };
     const auto code_row = [&](int turn) { return reinterpret_cast<uint2*>(s_in + P::OUT + 2 * P::PIECES) + turn * P::CODES; };
@@ -371,8 +373,8 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
             __syncwarp();
     };
     // Elements between a 16-byte boundary and the start of a row.
-    const auto past = [](const void* p, int64_t row, int64_t stride) {
-        return (int)(((uint32_t)((uintptr_t)p / ES) + (uint32_t)row * (uint32_t)stride) & (A - 1));
+    const auto past = [](const void* p, uint32_t row, int64_t stride) {
+        return (int)(((uint32_t)((uintptr_t)p / ES) + row * (uint32_t)stride) & (A - 1));
     };
     // The pieces of a row, from the boundary before it (which its allocation holds) to its last element.
     const auto fetch_pieces = [&](uint4* to, const T* from) {
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
     };
     // Row `ahead` into a stage; px and pr point at it and move on.
     const auto fetch = [&](int stage) {
-        if (ahead < a.rows) {
+        if (ahead < rows) {
             if constexpr (ALIGNED) {
                 const uint32_t dst = (uint32_t)__cvta_generic_to_shared(s_in + stage * 2 * NV * HALVES * TPR + t);
 #pragma unroll
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
         } else {
             v = window8<T>(in_row(stage, which) + (t + i * TPR) * HALVES, before);
             const int n = a.dim - j0 - i * TPR * 8;
-            if (n < 8) {
+            if (n < 8) {  // (what lies behind the row is not its)
 #pragma unroll
                 for (int k = 0; k < (int)sizeof(T) * 2; ++k) {
                     if constexpr (ES == 2)
@@ -446,8 +448,13 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
         barrier();
     }
     int stage = 0, turn = 0;
+    // The current row's residual_out and codes.
+    T* out = static_cast<T*>(a.residual_out) + (int64_t)row * a.dim + lead;
+    int8_t* codes = a.codes + (int64_t)row * a.dim + lead;
+    float* scales = a.scales + (int64_t)row * a.groups;
+    const int64_t out_step = (int64_t)step * a.dim, scale_step = (int64_t)step * a.groups;
     const float mean = 1.f / (float)a.dim;
-    for (; row < a.rows; row += step, turn ^= 1) {
+    for (; row < rows; row += step, turn ^= 1) {
         // (residual_out may be x's or residual's own rows: a row is stored only after its loads.)
         fetch(stage == 0 ? STAGES - 1 : stage - 1);
         if constexpr (ALIGNED) cp_async_wait<STAGES - 1>();
@@ -460,10 +467,10 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
                 if (a.residual) h[i] = add8<T>(h[i], take(stage, 1, i, before_r));
             }
         if (a.residual_out) {
-            T* out = (ALIGNED ? static_cast<T*>(a.residual_out) + row * a.dim : reinterpret_cast<T*>(out_row(turn))) + j0;
+            T* to = ALIGNED ? out : reinterpret_cast<T*>(out_row(turn)) + j0;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (j0 + i * TPR * 8 < a.dim) store8<T>(out + i * TPR * 8, h[i]);
+                if (j0 + i * TPR * 8 < a.dim) store8<T>(to + i * TPR * 8, h[i]);
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         float sum = 0.f, z[NV][8];
@@ -502,15 +509,15 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
             barrier();
         }
         if constexpr (!ALIGNED) {
-            if (a.residual_out) put_row<T, NV, TPR>(static_cast<T*>(a.residual_out) + row * a.dim, a.dim, out_row(turn), t);
+            if (a.residual_out) put_row<T, NV, TPR>(out, a.dim, out_row(turn), t);
             // the row before's (a block's first row is below step)
-            if (row >= step) put_codes<NV, TPR>(a.codes + (row - step) * a.dim, a.dim, code_row(turn ^ 1), t);
+            if (row >= step) put_codes<NV, TPR>(codes - out_step, a.dim, code_row(turn ^ 1), t);
         }
         if (!a.group) {
 #pragma unroll
             for (int i = 1; i < NV; ++i) top[i] = top[0];
         }
-        uint2* codes = ALIGNED ? reinterpret_cast<uint2*>(a.codes + row * a.dim + j0) : code_row(turn) + t;
+        uint2* to = ALIGNED ? reinterpret_cast<uint2*>(codes) : code_row(turn) + t;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = j0 + i * TPR * 8;
@@ -518,17 +525,20 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
             const bool ok = sum < INFINITY && top[i].hi < INFINITY;  // false for NaN too
             if (a.group ? (j & (a.group - 1)) == 0 : j == 0) {
                 const float per = rsqrtf(sum * mean + a.eps) * (1.f / 127.f);
-                a.scales[row * a.groups + (a.group ? j / a.group : 0)] =
+                scales[a.group ? j / a.group : 0] =
                     !ok ? __int_as_float(0x7FC00000) : top[i].hi >= SMALLEST ? top[i].hi * per : 0.f;
             }
             uint2 packed = make_uint2(0u, 0u);
             if (ok && top[i].hi >= SMALLEST) packed = codes_of<T>(h[i], w[i], z[i], top[i]);
-            codes[i * TPR] = packed;
+            to[i * TPR] = packed;
         }
+        out += out_step;
+        codes += out_step;
+        scales += scale_step;
     }
     if constexpr (!ALIGNED) {
         barrier();
-        put_codes<NV, TPR>(a.codes + (row - step) * a.dim, a.dim, code_row(turn ^ 1), t);
+        put_codes<NV, TPR>(codes - out_step, a.dim, code_row(turn ^ 1), t);
     }
 }
 
