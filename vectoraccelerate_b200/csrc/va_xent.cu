@@ -54,6 +54,9 @@ constexpr int EPI_WARPS = 8;              // two per quarter of the TMEM lanes: 
 constexpr int THREADS = 64 + 32 * EPI_WARPS;  // TMA warp, MMA warp, epilogue warps
 constexpr int TMEM_COLS = 512;
 constexpr size_t SMEM = 1024 + RING_BYTES + EPI_WARPS * EPI_BYTES + (2 * 6 + 5) * 8 + 16;
+// A gradient tile costs its K blocks, but at least this many: its results leave in that time (64 x 100000 x 768: both
+// products 84 us with 1, 72 with 2 to 4, 86 with 8).
+constexpr int TILE_END = 3;
 constexpr int64_t G_ENTRIES = 1 << 28;    // gradient entries of a chunk (512 MB of bf16)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
@@ -495,6 +498,7 @@ struct GradWork {
     int64_t row0;           // first table row of the chunk
     int64_t rows;           // rows of the whole table
     int dim;
+    int64_t tokens;
     int64_t tokens_pad;     // token_tiles * tile rows: of one split's dh buffer
     int64_t rows_pad;       // row_tiles * tile rows: of one split's dw buffer
     int token_tiles, row_tiles, d_tiles, splits;
@@ -637,8 +641,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!wait_accumulator(r, tile, lane, err, limit_ns)) break;
             const uint32_t at = r.tmem + ((uint32_t)(quarter * 32) << 16) + (tile & 1u) * BN;
             const int row = t.m * TM + (int)r.rank * BM + quarter * 32;
-            if (c0 == c1) release_accumulator(r, tile, lane);
-            for (int c = c0; c < c1; ++c) {
+            // (32 rows behind the last token or row are nobody's)
+            const bool none = is_h ? row >= w.tokens : w.row0 + row >= w.rows;
+            if (c0 == c1 || none) release_accumulator(r, tile, lane);
+            for (int c = none ? c1 : c0; c < c1; ++c) {
                 uint32_t v[64];
                 tmem_ld64(at + 64 * c, v);
                 tmem_wait64(v);
@@ -680,7 +686,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 else
                                     tma_add_2d(&map_dh, piece, col + 32 * i, at_row);
                             }
-                        } else if (col < w.dim && w.row0 + row < w.rows) {
+                        } else if (col < w.dim) {
                             tma_store_2d(&map_dw, piece, col, (int)(w.row0 + row));
                         }
                         bulk_commit();
@@ -803,16 +809,35 @@ __global__ void __launch_bounds__(128)
     }
 }
 
-// Sums K splits in order, applies the token's c g (dh) or rho (dw, tok NULL) and rounds.
-__global__ void __launch_bounds__(256) k_xent_finish(const float4* part, int splits, int64_t pitch, int64_t n, int per_row,
-                                                     const TokenGrad* tok, const float* rho, uint2* out) {
+// Sums K splits in a fixed order, applies the token's c g (dh) or rho (dw, tok NULL) and rounds. `lanes` threads of a
+// block take every lanes-th split of the same four elements (few tokens have many splits: 64 x 100000 x 768 18 us with one).
+__global__ void __launch_bounds__(256) k_xent_finish(const float4* part, int splits, int lanes, int64_t pitch, int64_t n,
+                                                     int per_row, const TokenGrad* tok, const float* rho, uint2* out) {
+    __shared__ float4 s_sum[256];
     pdl_start();
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        float4 v = part[i];
-        for (int s = 1; s < splits; ++s) {
-            const float4 u = part[i + s * pitch];
-            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    const int per = 256 / lanes, first = threadIdx.x / per;
+    for (int64_t b = (int64_t)blockIdx.x * per; b < n; b += (int64_t)gridDim.x * per) {
+        const int64_t i = b + threadIdx.x % per;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < n) {
+            v = part[i + first * pitch];
+#pragma unroll 4
+            for (int s = first + lanes; s < splits; s += lanes) {
+                const float4 u = part[i + s * pitch];
+                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+            }
         }
+        if (lanes > 1) {
+            __syncthreads();
+            s_sum[threadIdx.x] = v;
+            __syncthreads();
+            if (first) continue;
+            for (int k = 1; k < lanes; ++k) {
+                const float4 u = s_sum[threadIdx.x + k * per];
+                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+            }
+        }
+        if (i >= n) continue;
         const float g = tok ? tok[i / per_row].scale : *rho;
         // (a token without loss has no gradient, whatever the table holds)
         if (tok && g == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -895,7 +920,7 @@ BackwardPlan plan_backward(int sms, int64_t tokens, int64_t rows, int dim) {
     // K splits of dh: items of at most half a worker's share of the chunk's work (or 8 K blocks), while
     // the fp32 buffers stay within 64 MB.
     const int64_t chunk_rows = std::min(p.chunk, rows), kb_rows = (chunk_rows + BK - 1) / BK, kb_tokens = (tokens + BK - 1) / BK;
-    const int64_t work = p.d_tiles * (p.token_tiles * kb_rows + (chunk_rows + tm - 1) / tm * kb_tokens);
+    const int64_t work = p.d_tiles * (p.token_tiles * kb_rows + (chunk_rows + tm - 1) / tm * std::max<int64_t>(kb_tokens, TILE_END));
     const int64_t item = std::max<int64_t>(8, work / (2 * workers));
     const int64_t room = std::max<int64_t>(1, ((int64_t)64 << 20) / (p.token_tiles * tm * (int64_t)dim * 4));
     p.splits = (int)std::min(std::min((kb_rows + item - 1) / item, room), kb_rows);
@@ -1092,6 +1117,7 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
         w.row0 = row0;
         w.rows = rows;
         w.dim = dim;
+        w.tokens = tokens;
         w.tokens_pad = tokens_pad;
         w.token_tiles = p.token_tiles;
         w.row_tiles = (int)((count + tm - 1) / tm);
@@ -1105,7 +1131,8 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
         w.kb_tokens = (int)((tokens + BK - 1) / BK);
         w.first = row0 == 0;
         const int items_h = p.token_tiles * p.d_tiles * p.splits, items_w = w.row_tiles * p.d_tiles * p.splits_w;
-        const double cost_h = (double)w.kb_rows / p.splits, cost_w = (double)w.kb_tokens / p.splits_w;
+        const double cost_h = std::max<double>(TILE_END, (double)w.kb_rows / p.splits);
+        const double cost_w = std::max<double>(TILE_END, (double)w.kb_tokens / p.splits_w);
         w.long_h = cost_h >= cost_w;
         w.extra = (int)std::lround(std::max(cost_h, cost_w) / std::max(1.0, std::min(cost_h, cost_w)));
         const uint64_t limit = wait_limit_ns(ctx->timeout_ms);
@@ -1118,8 +1145,11 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
     }
     const auto finish = [&](const float* part, int splits, int64_t pad, int64_t n_rows, const TokenGrad* of, uint16_t* out) {
         const int64_t n4 = n_rows * dim / 4;
-        return launch<k_xent_finish>(ctx, (unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)ctx->sm_count * 8), 256, 0, false,
-                                     "k_xent_finish", (const float4*)part, splits, pad * dim / 4, n4, dim / 4, of,
+        int lanes = 1;
+        while (lanes < 16 && splits >= 4 * lanes && n4 * lanes < (int64_t)ctx->sm_count * 512) lanes *= 2;
+        const int64_t blocks = (n4 * lanes + 255) / 256;
+        return launch<k_xent_finish>(ctx, (unsigned)std::min<int64_t>(blocks, (int64_t)ctx->sm_count * 8), 256, 0, false,
+                                     "k_xent_finish", (const float4*)part, splits, lanes, pad * dim / 4, n4, dim / 4, of,
                                      (const float*)rho, (uint2*)out);
     };
     if (p.splits_w > 1) VA_TRY(finish(dw, p.splits_w, p.rows_pad, rows, nullptr, grad_table));
