@@ -341,6 +341,32 @@ def test_matvec_and_norm_past_32_bit_offsets(tctx):
     torch.cuda.empty_cache()
 
 
+def test_unaligned_norm_and_quantizer_past_32_bit_offsets(tctx):
+    g = gen(10)
+    rows, dim = 530000, 4093  # 2.17e9 elements
+    x = torch.empty(rows, dim, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    w = torch.ones(dim, dtype=torch.bfloat16, device="cuda")
+    parts = (slice(0, 200), slice(rows - 200, rows))
+    r = x[:1].expand(rows, dim).contiguous()
+    h = [(x[p].float() + r[p].float()).bfloat16() for p in parts]
+    codes, scales, out = run_norm(tctx, x, w, r, "bf16", 0, inplace=True)
+    for p, hp in zip(parts, h):
+        want, ws = norm_reference(hp, w, 1e-6, 0)
+        assert torch.equal(out[p], hp) and torch.equal(codes[p].double(), want)
+        assert ((scales[p].double() - ws).abs() <= SCALE_TOL * ws).all()
+    del r, out, codes
+    q = va.Int4GroupQuantizationKernel(tctx)
+    packed = torch.empty(rows, va.scoring.int4_row_bytes(dim), dtype=torch.uint8, device="cuda")
+    s = torch.empty(rows, 32, device="cuda")
+    q.encode(x, rows, dim, 128, packed, s, None, va.DTYPE_BF16, va.DTYPE_F32)
+    tctx.synchronize()
+    for p in parts:
+        want, ws, _ = quantize_reference(x[p].float(), 128, False, torch.float32)
+        assert torch.equal(unpack(packed[p], dim), want) and torch.equal(s[p], ws)
+    del x, packed
+    torch.cuda.empty_cache()
+
+
 def test_matvec_strided_output_and_extreme_queries(tctx):
     g = gen(6)
     codes, scales, _ = make_table(g, 70, 96, 32, "f32", False)
