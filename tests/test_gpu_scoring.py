@@ -253,6 +253,28 @@ def test_quantizer(tctx, group, zeros, n, dim, dtype, scale, pad):
     assert torch.equal(out, (want - zero[:, at]).float() * s[:, at])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantizer_at_borders(tctx, dtype, zeros):
+    # few distinct values: quotients fall on and next to the borders between codes all the time
+    g = gen(77)
+    n, dim = 3000, 517
+    x = (torch.randint(-30, 31, (n, dim), generator=g, device="cuda") / 4).to(DT[dtype])
+    x[::3] *= 1 / 3
+    if dtype == "f32":
+        x[1::3] = torch.nextafter(x[1::3], torch.zeros((), device="cuda"))
+    for scale in ("f32", "bf16"):
+        codes = torch.empty((n, va.scoring.int4_row_bytes(dim)), dtype=torch.uint8, device="cuda")
+        scales = torch.empty((n, 17), dtype=DT[scale], device="cuda")
+        zp = torch.empty((n, 17), dtype=torch.int8, device="cuda") if zeros else None
+        va.Int4GroupQuantizationKernel(tctx).encode(x, n, dim, 32, codes, scales, zp, VA[dtype], VA[scale])
+        tctx.synchronize()
+        want, s, zero = quantize_reference(x.float(), 32, zeros, DT[scale])
+        assert torch.equal(scales.float(), s) and torch.equal(unpack(codes, dim), want)
+        if zeros:
+            assert torch.equal(zp.to(torch.int32), zero)
+
+
 def make_table(g, n, dim, group, scale, zeros):
     stride, groups = va.scoring.int4_row_bytes(dim), -(-dim // group)
     codes = torch.randint(0, 256, (n, stride), generator=g, device="cuda", dtype=torch.uint8)  # padding holds anything
