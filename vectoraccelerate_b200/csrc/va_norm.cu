@@ -192,7 +192,7 @@ struct Top {
         if constexpr (sizeof(T) == 2) {
             hi = max_abs_nan(hi, h);
         } else {
-            const bool more = !(h <= hi) || (h == hi && l > lo);
+            const bool more = hi == hi && (!(h <= hi) || (h == hi && l > lo));  // a NaN wins from either side
             lo = more ? l : lo;
             hi = more ? h : hi;
         }
