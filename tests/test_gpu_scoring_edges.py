@@ -38,3 +38,26 @@ def test_norm_nan_products_at_every_position(tctx, dtype, dim, group, kind):  # 
         others = torch.arange(scales.shape[1], device="cuda") != g0
         assert torch.equal(codes[:, ~here].double(), want_codes[:, ~here]), j
         assert ((scales[:, others].double() - want_scales[:, others]).abs() <= SCALE_TOL * want_scales[:, others]).all(), j
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dim, group", [(64, 0), (200, 32), (1000, 0), (4096, 128), (4095, 0)])
+@pytest.mark.parametrize("eps", [0.0, 1e-30])
+def test_norm_tiny_rows_without_epsilon(tctx, dtype, dim, group, eps):  # noqa: F811
+    # the squares of these rows are below fp32's range, or so near its bottom that they keep few bits
+    g = gen(dim)
+    sizes = torch.tensor([2.0 ** -60, 2.0 ** -64, 2.0 ** -70, 2.0 ** -75, 2.0 ** -78, 2.0 ** -100, 2.0 ** -120, 0.0, 1.0], device="cuda")
+    x = (randn(g, 9, dim).clamp(-4, 4) * sizes[:, None]).to(DT[dtype])
+    for lift in (1.0, 2.0 ** 60):  # (the second lifts the rows of 2^-100 and 2^-120 above what counts as zero)
+        w = ((1 + 0.3 * randn(g, dim)) * lift).to(DT[dtype])
+        codes, scales, _ = run_norm(tctx, x, w, None, dtype, group, eps)
+        want_codes, want_scales = norm_reference(x, w, eps, group)
+        top = want_scales * 127 * torch.sqrt((x.double() ** 2).mean(1) + eps)[:, None]
+        live = top >= 2.0 ** -80
+        assert live[:5].all() and live[8].all() and not live[7].any() and live[5:7].all() == (lift > 1)
+        size = group or dim
+        at = torch.arange(dim, device="cuda") // size
+        assert torch.equal(codes.double(), torch.where(live[:, at], want_codes, 0.0))
+        # a scale near the bottom of fp32's range is off by up to half its last unit, 2^-150, besides
+        want = torch.where(live, want_scales, 0.0)
+        assert ((scales.double() - want).abs() <= SCALE_TOL * want + 2.0 ** -150).all()

@@ -27,8 +27,12 @@
 
 namespace {
 
-// A largest |z| below this counts as zero: fp32 squares and quotients have run out of range by then.
+// A largest |z| below this counts as zero: fp32 quotients have run out of range by then.
 constexpr float SMALLEST = 0x1p-80f;
+// A sum of squares below SMALL_SUM may have lost squares to fp32's range (2^-149 each, 2^-41 of a sum above it). An
+// epsilon of SMALL_EPS covers that; kernels for a smaller one take the sum again, of elements times 2^100. (A
+// variant of their own: in the others the rare case would spill registers.)
+constexpr float SMALL_SUM = 0x1p-96f, SMALL_EPS = 0x1p-80f, LIFT = 0x1p100f;
 
 struct NormArgs {
     const void* x;
@@ -346,13 +350,14 @@ __device__ __forceinline__ void put_codes(int8_t* out, int dim, const uint2* fro
 }
 
 // Vector i of thread t is at (i * TPR + t) * 8.
-template <typename T, bool ALIGNED, int TPR, int NV>
+template <typename T, bool ALIGNED, int TPR, int NV, bool SMALL>
 __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_norm_int8(NormArgs a) {
     using P = Plan<T, ALIGNED, TPR, NV>;
     constexpr int WARPS = TPR / 32, STAGES = P::STAGES, HALVES = P::HALVES;
     constexpr int A = 16 / sizeof(T), ES = sizeof(T);  // elements of a piece
     extern __shared__ uint4 s_in[];
     __shared__ float4 s_part[2][WARPS];  // (sum, hi, lo, -) of each warp
+    __shared__ float s_again[SMALL ? WARPS : 1];  // a small row's sum
     const int t = threadIdx.x, j0 = t * 8;
     Vec<T> w[NV];
 #pragma unroll
@@ -517,6 +522,25 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
 #pragma unroll
             for (int i = 1; i < NV; ++i) top[i] = top[0];
         }
+        // (All threads of the row have the same sum; its sign then says which one it is.)
+        if (SMALL && sum < SMALL_SUM) {
+            float again = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) again = fmaf(h[i][k] * LIFT, h[i][k] * LIFT, again);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) again += __shfl_xor_sync(0xFFFFFFFFu, again, o);
+            if constexpr (WARPS > 1) {
+                // (the next row's barrier lies between these reads and the next writes)
+                if ((t & 31) == 0) s_again[t >> 5] = again;
+                barrier();
+                again = s_again[t & (WARPS - 1)];
+#pragma unroll
+                for (int o = 1; o < WARPS; o <<= 1) again += __shfl_xor_sync(0xFFFFFFFFu, again, o);
+            }
+            sum = -again;
+        }
         uint2* to = ALIGNED ? reinterpret_cast<uint2*>(codes) : code_row(turn) + t;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -524,9 +548,11 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
             if (j >= a.dim) continue;
             const bool ok = sum < INFINITY && top[i].hi < INFINITY;  // false for NaN too
             if (a.group ? (j & (a.group - 1)) == 0 : j == 0) {
-                const float per = rsqrtf(sum * mean + a.eps) * (1.f / 127.f);
-                scales[a.group ? j / a.group : 0] =
-                    !ok ? __int_as_float(0x7FC00000) : top[i].hi >= SMALLEST ? top[i].hi * per : 0.f;
+                const bool lifted = SMALL && signbit(sum);
+                const float per = rsqrtf(lifted ? a.eps * LIFT * LIFT - sum * mean : sum * mean + a.eps) * (1.f / 127.f);
+                // (LIFT in two steps: hi * per alone may leave fp32's range at either end)
+                const float scale = lifted ? top[i].hi * 0x1p40f * per * (LIFT * 0x1p-40f) : top[i].hi * per;
+                scales[a.group ? j / a.group : 0] = !ok ? __int_as_float(0x7FC00000) : top[i].hi >= SMALLEST ? scale : 0.f;
             }
             uint2 packed = make_uint2(0u, 0u);
             if (ok && top[i].hi >= SMALLEST) packed = codes_of<T>(h[i], w[i], z[i], top[i]);
@@ -542,23 +568,28 @@ __global__ void __launch_bounds__(TPR, Plan<T, ALIGNED, TPR, NV>::BLOCKS) k_rms_
     }
 }
 
-template <typename T, bool ALIGNED, int TPR, int NV>
+template <typename T, bool ALIGNED, int TPR, int NV, bool SMALL>
 int launch_rows(va_context* ctx, const NormArgs& a) {
     using P = Plan<T, ALIGNED, TPR, NV>;
-    constexpr auto kern = k_rms_norm_int8<T, ALIGNED, TPR, NV>;
+    constexpr auto kern = k_rms_norm_int8<T, ALIGNED, TPR, NV, SMALL>;
     VA_TRY(va_kernel_once<kern>(ctx->device, P::BYTES));
     const int64_t grid = std::min<int64_t>(a.rows, (int64_t)ctx->sm_count * P::BLOCKS);
     kern<<<(unsigned)grid, TPR, P::BYTES, ctx->stream>>>(a);
     return va_check_launch("k_rms_norm_int8");
 }
 
+template <typename T, bool ALIGNED, bool SMALL>
+int launch_width(va_context* ctx, const NormArgs& a) {
+    if (a.dim <= 256) return launch_rows<T, ALIGNED, 32, 1, SMALL>(ctx, a);
+    if (a.dim <= 512) return launch_rows<T, ALIGNED, 32, 2, SMALL>(ctx, a);
+    if (a.dim <= 1024) return launch_rows<T, ALIGNED, 64, 2, SMALL>(ctx, a);
+    if (a.dim <= 2048) return launch_rows<T, ALIGNED, 128, 2, SMALL>(ctx, a);
+    return launch_rows<T, ALIGNED, 256, 2, SMALL>(ctx, a);
+}
+
 template <typename T, bool ALIGNED>
 int launch_norm(va_context* ctx, const NormArgs& a) {
-    if (a.dim <= 256) return launch_rows<T, ALIGNED, 32, 1>(ctx, a);
-    if (a.dim <= 512) return launch_rows<T, ALIGNED, 32, 2>(ctx, a);
-    if (a.dim <= 1024) return launch_rows<T, ALIGNED, 64, 2>(ctx, a);
-    if (a.dim <= 2048) return launch_rows<T, ALIGNED, 128, 2>(ctx, a);
-    return launch_rows<T, ALIGNED, 256, 2>(ctx, a);
+    return a.eps < SMALL_EPS ? launch_width<T, ALIGNED, true>(ctx, a) : launch_width<T, ALIGNED, false>(ctx, a);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
