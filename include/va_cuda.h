@@ -347,11 +347,13 @@ int va_sq_dequantize_int4_groups(va_context* ctx, const uint8_t* codes, const vo
 /* Scores of nq queries against the coded rows: out[q * out_stride + r] = sum_j x[q, j] *
  * scale[r, g(j)] * (code[r, j] - zero[r, g(j)]), fp32, times x_scales[q] when given. Queries
  * [nq x dim] are fp32 or bf16, or int8 codes (VA_DTYPE_INT8) whose scale per query is x_scales (fp32;
- * NULL: 1), e.g. va_rms_norm_int8's rows. int8 products are exact; fp32 and bf16 queries enter exactly or as
- * 31-bit fixed-point numbers per group, within 2^-30 of the group's largest |x| (a query with an infinity
- * or a NaN has scores that are not finite). Sums over groups are fp32, in a fixed order. Zero points lie in
- * [-8, 7]. The codes are read once per pass of up to 32 int8, 16 bf16 or 8 fp32 queries. No
- * allocation and no wait: the call may be captured into a graph. */
+ * NULL: 1), e.g. va_rms_norm_int8's rows. int8 products are exact. fp32 and bf16 queries enter exactly, but for
+ * elements below 2^-38 (bf16: 2^-54) of the largest |x| of their group in the last one or two queries of a call, which
+ * are off by up to 2^-62 of that |x| (a query with an infinity or a NaN has scores that are not finite). Sums over
+ * groups are fp32, in a fixed order for a given number of queries: one or two are summed in another form than more, so
+ * that the last bits of a query's scores depend on how many come with it. Zero points lie in [-8, 7]. The codes are
+ * read once per pass of up to 32 int8, 16 bf16 (8 above 2048 columns) or 8 fp32 queries. No allocation and no wait:
+ * the call may be captured into a graph. */
 int va_int4_matvec(va_context* ctx, const void* x, int x_dtype, const float* x_scales, int nq, const uint8_t* codes,
                    const void* scales, const int8_t* zeros, int64_t n, int dim, int group, int scale_dtype,
                    float* out, int64_t out_stride);

@@ -8,7 +8,8 @@ import pytest
 import torch
 
 import vectoraccelerate_b200 as va
-from test_gpu_scoring import DT, SCALE_TOL, gen, norm_reference, randn, run_norm, tctx  # noqa: F401
+from test_gpu_scoring import (DT, SCALE_TOL, gen, make_queries, make_table, matvec_reference, matvec_tolerance,  # noqa: F401
+                              norm_reference, randn, run_matvec, run_norm, tctx, unpack)
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +62,46 @@ def test_norm_tiny_rows_without_epsilon(tctx, dtype, dim, group, eps):  # noqa: 
         # a scale near the bottom of fp32's range is off by up to half its last unit, 2^-150, besides
         want = torch.where(live, want_scales, 0.0)
         assert ((scales.double() - want).abs() <= SCALE_TOL * want + 2.0 ** -150).all()
+
+
+# ------------------------------------------------------------------------------------------ 4-bit rows
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n, dim, group, nq, zeros", [(400, 512, 64, 1, False), (333, 520, 32, 2, True), (300, 4096, 32, 1, True), (200, 4096, 128, 2, False),
+                                                     (300, 1544, 64, 3, False), (257, 2304, 32, 8, True), (300, 4090, 128, 17, False), (100, 512, 64, 9, True)])
+@pytest.mark.parametrize("outlier", [2.0 ** 20, 2.0 ** 34])
+def test_matvec_outliers_that_meet_zero(tctx, dtype, n, dim, group, nq, zeros, outlier):  # noqa: F811
+    # the columns of the outliers hold what stands for zero: the answer is made of the other elements alone
+    g = gen(dim + nq)
+    codes, scales, zp = make_table(g, n, dim, group, "f32", zeros)
+    x, _ = make_queries(g, nq, dim, dtype)
+    x = (randn(g, nq, dim)).to(DT[dtype])
+    for j in range(1, dim, 30):
+        x[:, j] *= outlier
+        nibble = (zp[:, j // group].to(torch.int32) & 15 if zeros else torch.zeros(n, dtype=torch.int32, device="cuda")).to(torch.uint8)
+        byte = codes[:, j // 2]
+        codes[:, j // 2] = (byte & 0xF0) | nibble if j % 2 == 0 else (byte & 0x0F) | (nibble << 4)
+    out = run_matvec(tctx, x, None, codes, scales, zp, dim, group)
+    want, size = matvec_reference(x, None, codes, scales, zp, dim, group)
+    # one or two queries are multiples of 2^-62 of the power of two above their group's largest |x| (< 2 times that):
+    # off by at most 2^-62 of it
+    at = torch.arange(dim, device="cuda") // group
+    groups = -(-dim // group)
+    top = torch.nn.functional.pad(x.abs().double(), (0, -dim % group)).view(nq, groups, group).amax(2)[:, at]
+    w = unpack(codes, dim) - (zp.to(torch.int32)[:, at] if zeros else 0)
+    w = (w.double() * scales.double()[:, at]).abs()
+    assert ((out.double() - want).abs() <= matvec_tolerance(dim, group) * size + 2.0 ** -62 * (top @ w.t())).all()
+
+
+def test_matvec_wide_queries_in_strided_rows(tctx):  # noqa: F811
+    # fp32 queries over more than 1536 columns are summed over ranges of columns: rows between the outputs are kept,
+    # what was in the output before is not added
+    g = gen(61)
+    n, dim, nq = 77, 3333, 11
+    codes, scales, zp = make_table(g, n, dim, 64, "bf16", True)
+    x = randn(g, nq, dim)
+    wide = torch.full((nq, 100), 5.0, device="cuda")
+    wide[:, :n] = float("nan")
+    run_matvec(tctx, x, None, codes, scales, zp, dim, 64, out=wide[:, :n])
+    want, size = matvec_reference(x, None, codes, scales, zp, dim, 64)
+    assert ((wide[:, :n].double() - want).abs() <= matvec_tolerance(dim, 64) * size).all()
+    assert (wide[:, n:] == 5.0).all()

@@ -12,16 +12,18 @@
 // through mma.sync (codes are A, 16 rows; queries are B, 8 columns). tcgen05 would need the unpacked codes written
 // to shared memory to use a 128-row tile whose columns stay mostly empty. Two forms:
 //   * DIGITS, integer m16n8k32: three logic instructions turn 8 codes into 8 bytes c + 8. An int8 query is one
-//     column; an fp32 or bf16 query becomes, per group, fixed-point numbers of 31 bits below the power of two above
-//     the group's largest |x| (an error of at most 2^-30 of that |x|), in four columns of signed 8-bit digits. Group
+//     column; an fp32 or bf16 query becomes, per group, fixed-point numbers of 62 bits below the power of two above
+//     the group's largest |x|, in eight columns of signed 8-bit digits: an element keeps all its bits down to 2^-38 of
+//     that |x| (bf16: 2^-54), and below it is off by at most 2^-62 of it. (With 31 bits in four columns, the rest of a
+//     group whose outlier meets codes that stand for zero would lose what the outlier leaves no room for.) Group
 //     sums are exact integers below 2^22; they start at 1.5 * 2^23 as a bit pattern, less (8 + zero) times the digits'
 //     sum, so that the finished accumulator read as fp32 and less 1.5 * 2^23 is the group's sum.
 //   * PIECES, bf16 m16n8k16: 11 instructions turn 8 codes into 8 exact bf16 values c - zero. A bf16 query is one
 //     column, exact; an fp32 query is split by truncation into three bf16 values of 8 mantissa bits each, exact, that
 //     are multiplied in turn into the same sum.
-//   Digits cost four columns and their recombination per group and query, pieces cost more per code: digits serve int8
-//   queries and up to two others, pieces the rest (300000 x 1536, group 128, bf16 queries: two as digits 46 us, as pieces
-//   68 us; 50000 x 4096, group 32, five queries: digits 160 us, pieces 44 us).
+//   Digits cost a column tile and its recombination per group and query, pieces cost more per code: digits serve int8
+//   queries and up to two others, pieces the rest (300000 x 1536, group 128, bf16 queries: two as digits 54 us, as pieces
+//   68 us; 100000 x 4096, group 32, four fp32 queries with zero points: digits in four tiles 202 us, pieces 175 us).
 //   * Logic and issue slots are what remains above the memory time: 2000000 x 768 with one query takes 134 us at the full
 //     clock (6.1 TB/s), 155 us once the power cap has lowered it; 16 int8 queries x 300000 x 1536 69 us (41 us of memory).
 //   * Group scales and query scales are applied and the groups summed in fp32.
@@ -32,6 +34,7 @@
 //   * Few rows: WK warps share a row tile, each takes every WK-th 256-code chunk, and the first adds
 //     the partial sums in order.
 #include <algorithm>
+#include <type_traits>
 
 #include "va_tcgen05.cuh"
 
@@ -51,7 +54,9 @@ struct MatvecArgs {
     float* out;
     int64_t n, out_stride;
     int row_tiles;
-    int dim, groups, nq, x_dtype;
+    int dim, groups, nq, x_dtype;  // columns and groups of this launch
+    int x_pitch, scale_pitch;      // of a whole query and of a row's scales
+    int add;                       // the launch adds to out (a further range of columns)
     int chunks;  // 256-code chunks per row
     int wk;      // warps sharing a row tile
     int ring;    // slots per warp
@@ -138,14 +143,14 @@ struct ChunkScales {
 // First scales of a lane's four rows in a row tile; rows past the end repeat the last one (they are not stored).
 __device__ __forceinline__ void row_bases(const MatvecArgs& a, int tile, int g, int64_t (&base)[4]) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) base[r] = min((int64_t)tile * TR + g + 8 * r, a.n - 1) * a.groups;
+    for (int r = 0; r < 4; ++r) base[r] = min((int64_t)tile * TR + g + 8 * r, a.n - 1) * a.scale_pitch;
 }
 
 // What a block keeps of the queries in shared memory.
 struct QueryShared {
     uint2* frag;    // [chunk][block 8][step 2 of bf16][NT][piece][lane]: in the mma's order
     int* start;     // [group][NT * 8]: MAGIC - 8 * sum of the column's digits
-    float* weight;  // [group][NT * 4]: of a pair of columns (DIGITS_WIDE)
+    float* weight;  // [group][NT][4]: of a query's pairs of columns (DIGITS_WIDE)
 };
 
 // Eight elements of query q from column j on (zeros where there are none) as fp32. The vector form needs queries that start on 16 (int8: 8) bytes and whole vectors.
@@ -153,7 +158,7 @@ __device__ __forceinline__ void load_query(const MatvecArgs& a, int q, int j, bo
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = 0.f;
     if (q >= a.nq || j >= a.dim) return;
-    const int64_t at = (int64_t)q * a.dim + j;
+    const int64_t at = (int64_t)q * a.x_pitch + j;
     if (a.x_dtype == VA_DTYPE_F32) {
         const float* x = static_cast<const float*>(a.x) + at;
         if (vector) {
@@ -222,9 +227,10 @@ __device__ __forceinline__ void lay_out(const MatvecArgs& a, const QueryShared& 
     } else {
         constexpr int LANES = GROUP / 8;  // of a group
         constexpr bool wide = MODE == DIGITS_WIDE;
-        constexpr int planes = wide ? 4 : 1;
+        constexpr int planes = wide ? 8 : 1;
+        using Fixed = std::conditional_t<wide, long long, int>;
         const int grp = (c * CHUNK + lane * 8) / GROUP;
-        int v[8];
+        Fixed v[8];
         if constexpr (wide) {
             float top = 0.f;
             int finite = 1;
@@ -238,15 +244,16 @@ __device__ __forceinline__ void lay_out(const MatvecArgs& a, const QueryShared& 
                 finite &= __shfl_xor_sync(0xFFFFFFFFu, finite, o);
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
             }
-            // 2^e > top; the fixed point's unit is 2^(e - 30), not below the smallest fp32. (The factor may
+            // 2^e > top; the fixed point's unit is 2^(e - 62), not below the smallest fp32. (The factor may
             // exceed fp32: two steps.)
-            const int e = max((int)(__float_as_uint(top) >> 23) - 126, -119);
-            const float up = ldexpf(1.f, (30 - e) / 2), up2 = ldexpf(1.f, 30 - e - (30 - e) / 2);
+            const int e = max((int)(__float_as_uint(top) >> 23) - 126, -87);
+            const float up = ldexpf(1.f, (62 - e) / 2), up2 = ldexpf(1.f, 62 - e - (62 - e) / 2);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = finite ? __float2int_rn(f[k] * up * up2) : 0;
+            for (int k = 0; k < 8; ++k) v[k] = finite ? __float2ll_rn(f[k] * up * up2) : 0;
             if (lane % LANES == 0) {
-                const float w = finite ? ldexpf(1.f, e - 30) : __int_as_float(0x7FC00000);
-                *reinterpret_cast<float2*>(sh.weight + (size_t)grp * NT * 4 + q * 2) = make_float2(w * 65536.f, w);
+                const float none = finite ? 0.f : __int_as_float(0x7FC00000);
+                *reinterpret_cast<float4*>(sh.weight + ((size_t)grp * NT + q) * 4) =
+                    make_float4(ldexpf(1.f, e - 14) + none, ldexpf(1.f, e - 30) + none, ldexpf(1.f, e - 46) + none, ldexpf(1.f, e - 62) + none);
             }
         } else {
 #pragma unroll
@@ -258,9 +265,9 @@ __device__ __forceinline__ void lay_out(const MatvecArgs& a, const QueryShared& 
             uint32_t d[2];  // even and odd elements
 #pragma unroll
             for (int o = 0; o < 2; ++o)
-                d[o] = __byte_perm(__byte_perm(v[o], v[2 + o], 0x0040), __byte_perm(v[4 + o], v[6 + o], 0x0040), 0x5410);
+                d[o] = __byte_perm(__byte_perm((uint32_t)v[o], (uint32_t)v[2 + o], 0x0040), __byte_perm((uint32_t)v[4 + o], (uint32_t)v[6 + o], 0x0040), 0x5410);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = (v[k] - (int)(int8_t)v[k]) >> 8;
+            for (int k = 0; k < 8; ++k) v[k] = (v[k] - (Fixed)(int8_t)v[k]) >> 8;
             sh.frag[((size_t)blk * NT + (col >> 3)) * 32 + (col & 7) * 4 + t] = make_uint2(d[0], d[1]);
             int sum = __dp4a((int)d[0], 0x01010101, __dp4a((int)d[1], 0x01010101, 0));
 #pragma unroll
@@ -325,9 +332,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     row_bases(a, min(first, a.row_tiles - 1), g, base);
     next.load(a, base, part, t);
 
-    constexpr int QUERIES = WIDE ? NT * 2 : NT * 8;
+    constexpr int QUERIES = WIDE ? NT : NT * 8;
     const int item = a.x_dtype == VA_DTYPE_F32 ? 4 : a.x_dtype == VA_DTYPE_BF16 ? 2 : 1;
-    const bool vector = a.dim % 8 == 0 && ((uintptr_t)a.x & (item == 1 ? 7 : 15)) == 0;
+    const bool vector = a.dim % 8 == 0 && a.x_pitch % 8 == 0 && ((uintptr_t)a.x & (item == 1 ? 7 : 15)) == 0;
     for (int i = warp; i < a.chunks * QUERIES; i += WARPS) lay_out<NT, GROUP, MODE>(a, sh, i % QUERIES, i / QUERIES, vector, lane);
     __syncthreads();
 
@@ -508,17 +515,25 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                     for (int hi = 0; hi < 2; ++hi) {
                         const int64_t row = (int64_t)tile * TR + g + 16 * m + 8 * hi;
                         if constexpr (WIDE) {
-                            // Lanes t = 0, 1 hold query 2n (high and low digits), t = 2, 3 query 2n + 1.
-                            const float v = acc[n][m][hi] + __shfl_xor_sync(0xFFFFFFFFu, acc[n][m][hi], 1);
-                            const int q = n * 2 + (t >> 1);
-                            if ((t & 1) == 0 && row < a.n && q < a.nq) a.out[(int64_t)q * a.out_stride + row] = v;
+                            // Lane t holds digits 2t and 2t + 1 of query n.
+                            float v = acc[n][m][hi];
+                            v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+                            v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+                            if (t == 0 && row < a.n && n < a.nq) a.out[(int64_t)n * a.out_stride + row] = v;
                         } else {
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 const int q = n * 8 + 2 * t + i;
-                                if (row < a.n && q < a.nq)
-                                    a.out[(int64_t)q * a.out_stride + row] =
-                                        a.x_scales ? acc[n][m][2 * hi + i] * __ldg(a.x_scales + q) : acc[n][m][2 * hi + i];
+                                if (row < a.n && q < a.nq) {
+                                    float* const to = a.out + (int64_t)q * a.out_stride + row;
+                                    float v = acc[n][m][2 * hi + i];
+                                    if constexpr (MODE == DIGITS_INT8) {
+                                        if (a.x_scales) v *= __ldg(a.x_scales + q);
+                                    } else if constexpr (MODE == BF16X3) {
+                                        if (a.add) v += *to;
+                                    }
+                                    *to = v;
+                                }
                             }
                         }
                     }
@@ -563,28 +578,27 @@ int launch_types(va_context* ctx, const Launch& l) {
     return l.a.zeros ? launch_group<MODE, NT, float, true>(ctx, l) : launch_group<MODE, NT, float, false>(ctx, l);
 }
 
-// A pass: its mode, column tiles and queries.
+// A pass: its mode, column tiles, queries, and chunks of columns per launch.
 struct Pass {
-    int mode, nt, nq;
+    int mode, nt, nq, chunks;
 };
 
-// fp32 and bf16 queries: up to two as digits (one column tile), more as pieces, 8 queries a column tile; three
-// pieces of 8 queries leave the ring two slots up to 1536 dimensions, beyond which fp32 queries go as digits in up to
-// four column tiles. int8 queries: 8 a column tile, up to four. Two tiles of bf16 pieces take twice the memory
-// of one, which is left to the ring above 2048 dimensions.
+// fp32 and bf16 queries: up to two as digits (a column tile each), more as pieces, 8 queries a column tile; three
+// pieces of 8 queries leave the ring two slots up to 1536 dimensions: wider rows are taken in equal ranges of columns,
+// each launch adding to the scores of the one before. int8 queries: 8 a column tile, up to four. Two tiles of bf16 pieces
+// take twice the memory of one, which is left to the ring above 2048 dimensions.
 Pass pass_of(int x_dtype, int left, int chunks) {
     if (x_dtype == VA_DTYPE_INT8) {
         const int nt = left > 16 ? 4 : left > 8 ? 2 : 1;
-        return Pass{DIGITS_INT8, nt, std::min(left, nt * 8)};
+        return Pass{DIGITS_INT8, nt, std::min(left, nt * 8), chunks};
     }
-    if (left <= 2) return Pass{DIGITS_WIDE, 1, left};
+    if (left <= 2) return Pass{DIGITS_WIDE, left, left, chunks};
     if (x_dtype == VA_DTYPE_BF16) {
         const int nt = left > 8 && chunks <= 8 ? 2 : 1;
-        return Pass{BF16, nt, std::min(left, nt * 8)};
+        return Pass{BF16, nt, std::min(left, nt * 8), chunks};
     }
-    if (chunks <= 6) return Pass{BF16X3, 1, std::min(left, 8)};
-    const int nt = left > 4 ? 4 : 2;
-    return Pass{DIGITS_WIDE, nt, std::min(left, nt * 2)};
+    const int ranges = (chunks + 5) / 6;
+    return Pass{BF16X3, 1, std::min(left, 8), (chunks + ranges - 1) / ranges};
 }
 
 int launch_pass(va_context* ctx, const Pass& p, const Launch& l) {
@@ -594,9 +608,7 @@ int launch_pass(va_context* ctx, const Pass& p, const Launch& l) {
                    : p.nt == 2 ? launch_types<DIGITS_INT8, 2>(ctx, l)
                                : launch_types<DIGITS_INT8, 4>(ctx, l);
         case DIGITS_WIDE:
-            return p.nt == 1   ? launch_types<DIGITS_WIDE, 1>(ctx, l)
-                   : p.nt == 2 ? launch_types<DIGITS_WIDE, 2>(ctx, l)
-                               : launch_types<DIGITS_WIDE, 4>(ctx, l);
+            return p.nt == 1 ? launch_types<DIGITS_WIDE, 1>(ctx, l) : launch_types<DIGITS_WIDE, 2>(ctx, l);
         case BF16:
             return p.nt == 1 ? launch_types<BF16, 1>(ctx, l) : launch_types<BF16, 2>(ctx, l);
         default:
@@ -868,49 +880,64 @@ int va_int4_matvec(va_context* ctx, const void* x, int x_dtype, const float* x_s
     const auto enc = get_encode_fn();
     if (!enc) return va_set_error(VA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
     Launch l{};
-    const cuuint64_t dims[2] = {(cuuint64_t)VA_INT4_ROW_BYTES(dim), (cuuint64_t)n};
-    const cuuint64_t strides[1] = {(cuuint64_t)VA_INT4_ROW_BYTES(dim)};
-    const cuuint32_t box[2] = {128, TR}, estr[2] = {1, 1};
-    const CUresult r = enc(&l.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return va_set_error(VA_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
     l.group = group;
     l.scale_dtype = scale_dtype;
     MatvecArgs& a = l.a;
-    a.scales = scales;
-    a.zeros = zeros;
     a.n = n;
     a.out_stride = out_stride;
     a.row_tiles = (int)((n + TR - 1) / TR);
-    a.dim = dim;
-    a.groups = (dim + group - 1) / group;
+    a.x_pitch = dim;
+    a.scale_pitch = (dim + group - 1) / group;
     a.x_dtype = x_dtype;
-    a.chunks = (dim + CHUNK - 1) / CHUNK;
+    const int chunks = (dim + CHUNK - 1) / CHUNK;
     l.grid = std::min(ctx->sm_count, a.row_tiles);
+    int mapped = -1;  // the chunk at which the tensor map starts
+    const auto codes_from = [&](int chunk) {
+        if (chunk == mapped) return VA_OK;
+        mapped = chunk;
+        const cuuint64_t pitch = VA_INT4_ROW_BYTES(dim);
+        const cuuint64_t dims[2] = {pitch - (cuuint64_t)chunk * (CHUNK / 2), (cuuint64_t)n};
+        const cuuint32_t box[2] = {CHUNK / 2, TR}, estr[2] = {1, 1};
+        const CUresult r = enc(&l.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes) + (size_t)chunk * (CHUNK / 2), dims,
+                               &pitch, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return va_set_error(VA_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+        return VA_OK;
+    };
     for (int q0 = 0; q0 < nq; q0 += a.nq) {
-        const Pass p = pass_of(x_dtype, nq - q0, a.chunks);
+        const Pass p = pass_of(x_dtype, nq - q0, chunks);
         a.nq = p.nq;
-        a.x = static_cast<const uint8_t*>(x) + (size_t)q0 * dim * es;
         a.x_scales = x_scales ? x_scales + q0 : nullptr;
         a.out = out + (int64_t)q0 * out_stride;
-        // Warps per row tile: what leaves the busiest warp the least to do, a tile's end counted as half a chunk and a
-        // join as one and a half.
-        const int warps = warps_of(p.nt);
-        double best = 0;
-        for (int wk = 1; wk <= 8 && wk <= a.chunks; wk *= 2) {
-            const int64_t slots = (int64_t)l.grid * (warps / wk);
-            const double cost = (double)((a.row_tiles + slots - 1) / slots) * ((a.chunks + wk - 1) / wk + (wk > 1 ? 2.0 : 0.5));
-            if (wk == 1 || cost < best) {
-                best = cost;
-                a.wk = wk;
+        for (int c0 = 0; c0 < chunks; c0 += p.chunks) {
+            // Chunks c0 .. c0 + a.chunks - 1 of every row.
+            const int g0 = c0 * (CHUNK / group);
+            VA_TRY(codes_from(c0));
+            a.chunks = std::min(p.chunks, chunks - c0);
+            a.dim = std::min(dim - c0 * CHUNK, a.chunks * CHUNK);
+            a.groups = (a.dim + group - 1) / group;
+            a.add = c0 > 0;
+            a.x = static_cast<const uint8_t*>(x) + ((size_t)q0 * dim + (size_t)c0 * CHUNK) * es;
+            a.scales = static_cast<const uint8_t*>(scales) + (size_t)g0 * (scale_dtype == VA_DTYPE_BF16 ? 2 : 4);
+            a.zeros = zeros ? zeros + g0 : nullptr;
+            // Warps per row tile: what leaves the busiest warp the least to do, a tile's end counted as half a chunk and a
+            // join as one and a half.
+            const int warps = warps_of(p.nt);
+            double best = 0;
+            for (int wk = 1; wk <= 8 && wk <= a.chunks; wk *= 2) {
+                const int64_t slots = (int64_t)l.grid * (warps / wk);
+                const double cost = (double)((a.row_tiles + slots - 1) / slots) * ((a.chunks + wk - 1) / wk + (wk > 1 ? 2.0 : 0.5));
+                if (wk == 1 || cost < best) {
+                    best = cost;
+                    a.wk = wk;
+                }
             }
+            const size_t queries = (size_t)p.nt * a.chunks * (frag_bytes(p.mode) + (is_bf16(p.mode) ? 0 : CHUNK / group * (8 + 4) * 4));
+            const size_t rest = 1024 + queries + 16 + (a.wk > 1 ? (size_t)warps * p.nt * 8 * 32 * 4 : 0);
+            a.ring = (int)std::min<size_t>(6, (227 * 1024 - rest) / (warps * (SLOT + 8)));
+            l.smem = rest + (size_t)a.ring * warps * (SLOT + 8);
+            VA_TRY(launch_pass(ctx, p, l));
         }
-        const size_t queries = (size_t)p.nt * a.chunks * (frag_bytes(p.mode) + (is_bf16(p.mode) ? 0 : CHUNK / group * (8 + 4) * 4));
-        const size_t rest = 1024 + queries + 16 + (a.wk > 1 ? (size_t)warps * p.nt * 8 * 32 * 4 : 0);
-        a.ring = (int)std::min<size_t>(6, (227 * 1024 - rest) / (warps * (SLOT + 8)));
-        l.smem = rest + (size_t)a.ring * warps * (SLOT + 8);
-        VA_TRY(launch_pass(ctx, p, l));
     }
     return VA_OK;
 }
