@@ -482,7 +482,8 @@ int va_ivf_search_host(va_context* ctx, const va_ivf* ivf, const float* queries_
 /* ------------------------------------------------------------------------------------------ */
 /* hidden [tokens x dim] and table [rows x dim] are bf16 with row strides in elements (16-byte aligned
  * rows: strides and dim are multiples of 8). Logits logit_scale * hidden_t . table_v are formed tile by
- * tile and never kept. lse[t] = ln sum_v exp(logit), loss[t] = lse[t] - logit[t, labels[t]] (fp32). A label
+ * tile and never kept. lse[t] = ln sum_v exp(logit), loss[t] = lse[t] - logit[t, labels[t]] (fp32, formed from
+ * one set of logits before either is rounded, and never below 0). A label
  * outside [0, rows) marks a token without loss: loss 0, no gradient, and its hidden row is not read into
  * the table's gradient. Sums are fp32 in a fixed order. */
 /* Device bytes of scratch that a call of these sizes needs (backward: 0 or 1). */

@@ -8,8 +8,8 @@ import pytest
 import torch
 
 import vectoraccelerate_b200 as va
-from test_gpu_scoring import (DT, SCALE_TOL, gen, make_queries, make_table, matvec_reference, matvec_tolerance,  # noqa: F401
-                              norm_reference, randn, run_matvec, run_norm, tctx, unpack)
+from test_gpu_scoring import (DT, SCALE_TOL, U32, gen, make_queries, make_table, matvec_reference,  # noqa: F401
+                              matvec_tolerance, norm_reference, randn, run_loss, run_matvec, run_norm, tctx, unpack)
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +105,53 @@ def test_matvec_wide_queries_in_strided_rows(tctx):  # noqa: F811
     want, size = matvec_reference(x, None, codes, scales, zp, dim, 64)
     assert ((wide[:, :n].double() - want).abs() <= matvec_tolerance(dim, 64) * size).all()
     assert (wide[:, n:] == 5.0).all()
+
+
+# ------------------------------------------------------------------------------------------ loss
+@pytest.mark.parametrize("t, v, d", [(1, 1, 64), (70, 900, 128), (333, 5003, 512), (600, 30001, 256)])
+@pytest.mark.parametrize("scale", [1.0, 7.3])
+def test_loss_of_confident_tokens(tctx, t, v, d, scale):  # noqa: F811
+    # Labels that have nearly all of the probability, at logits of hundreds: the loss is a small difference of large
+    # numbers and never below zero.
+    g = gen(t + v)
+    w = randn(g, v, d).bfloat16()
+    labels = torch.randint(0, v, (t,), generator=g, device="cuda")
+    h = (w[labels].float() * torch.linspace(0.02, 4.0, t, device="cuda")[:, None]).bfloat16()
+    loss, lse, _, _ = run_loss(tctx, h, w, labels, scale, None)
+    z = scale * (h.double() @ w.double().t())
+    want = torch.logsumexp(z, 1)
+    zl = z.gather(1, labels[:, None])[:, 0]
+    assert (loss >= 0).all()
+    # The logits come from one set of fp32 sums: D / 16 matrix steps of 18 roundings of the sum of magnitudes each, the
+    # label's and the others'. Of the rest, exponents near 0 and a logarithm of a number above 1/2: 2^-20 in all (the
+    # terms of v rows, 2^-24 each, add up in (v / 256 + 64) steps), and one rounding of the result.
+    size = scale * (h.double().abs() @ w.double().abs().t()).amax(1)
+    dz = 2 * 18 * d / 16 * U32 * size
+    rest = (v / 256 + 64) * U32 + 2.0 ** -20
+    exact = want - zl
+    assert ((loss.double() - exact).abs() <= dz + rest + 2 * U32 * exact).all()
+    # a token with nothing beside its label: the same logit in lse and in the loss, one exponential and one logarithm
+    alone = exact < 1e-9
+    assert (loss[alone] <= 2.0 ** -21).all()
+    assert ((lse.double() - want).abs() <= dz + rest + 2 * U32 * want.abs()).all()
+
+
+def test_loss_of_whole_numbers_is_exact_to_fp32(tctx):  # noqa: F811
+    # small whole numbers: every logit is exact in fp32, so only the statistics can be off
+    g = gen(44)
+    t, v, d = 300, 4001, 64
+    h = torch.randint(-6, 7, (t, d), generator=g, device="cuda").bfloat16()
+    w = torch.randint(-6, 7, (v, d), generator=g, device="cuda").bfloat16()
+    for scale in (1.0, 0.3, 1.7):
+        c = float(torch.tensor(scale))  # as fp32
+        z = c * (h.double() @ w.double().t())
+        labels = z.topk(3, 1).indices[:, torch.randint(0, 3, (1,), generator=g, device="cuda").item()].contiguous()
+        loss, lse, _, _ = run_loss(tctx, h, w, labels, scale, None)
+        want = torch.logsumexp(z, 1)
+        exact = want - z.gather(1, labels[:, None])[:, 0]
+        # An exponent is a difference of logits, off by 3 roundings of its size, which is at most ln v on the average over
+        # the softmax: 25 roundings. The sum of v terms in v / 256 steps and its joins: 39. The exponential and the
+        # logarithm: 2^-21.
+        rest = (v / 256 + 64) * U32 + 2.0 ** -21
+        assert ((loss.double() - exact).abs() <= rest + 3 * U32 * exact.abs()).all()
+        assert ((lse.double() - want).abs() <= rest + 1.01 * U32 * want.abs()).all()

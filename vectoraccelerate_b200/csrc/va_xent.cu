@@ -8,8 +8,8 @@
 //
 // Forward, 2TVD operations: k_xent_scores<FORWARD> walks tiles of tokens x 256 rows (TMA ring, one thread issuing
 // tcgen05.mma, two TMEM accumulators) and its epilogue keeps each token's running maximum and sum of
-// exponentials (in powers of two) in registers; the partial pairs of the row splits are joined by k_xent_join, which
-// also forms the label's logit.
+// exponentials (in powers of two) in registers, and sets the label's logit aside; the partial pairs of the row splits are
+// joined by k_xent_join.
 // Backward, 6TVD: the table is taken in chunks of rows so that G of a chunk (bf16) is at most 512 MB (with 256 MB
 // the last, partly filled round of tiles weighs more: 2% slower at 8192 x 131072 x 1536).
 // k_xent_scores<GRADIENT> recomputes the chunk's logits and stores G; k_xent_grads multiplies it both
@@ -306,7 +306,9 @@ struct ScoreWork {
     int token_tiles, row_tiles, splits, k_blocks;
     int n;                 // table rows of a tile: 256, or 128 (single CTAs)
     float scale2;          // c * log2(e)
-    float2* part;          // forward: (maximum, sum) per [split][column half][token_tiles * tile rows]
+    float2* part;          // forward: (maximum of h . w, sum) per [split][column half][token_tiles * tile rows]
+    const int64_t* labels; // forward
+    float* label_dot;      // forward: h . w of the token's label
     const TokenGrad* tok;  // gradient
 };
 
@@ -317,8 +319,21 @@ __device__ __forceinline__ void score_item(const ScoreWork& w, int item, int& tt
     r1 = (int)((int64_t)w.row_tiles * (split + 1) / w.splits);
 }
 
+// r[i], for an index that is not known to the compiler: halved six times.
+__device__ __forceinline__ float pick(const uint32_t (&r)[64], int i) {
+    uint32_t v[32];
+#pragma unroll
+    for (int k = 0; k < 32; ++k) v[k] = i & 32 ? r[k + 32] : r[k];
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1)
+#pragma unroll
+        for (int k = 0; k < w; ++k) v[k] = i & w ? v[k + w] : v[k];
+    return __uint_as_float(v[0]);
+}
+
 // Running maximum and sum of 2^z over 64 columns of a row, z = acc * scale2; columns at or past
-// `valid` do not exist. The maximum is kept as nb = -max z (finite even while no logit was finite).
+// `valid` do not exist. The maximum is kept as nb = -max z (finite even while no logit was finite), rounded: `sum` is
+// relative to 2^-nb as it is.
 __device__ __forceinline__ void lse_chunk(uint32_t (&r)[64], float scale2, int valid, float& top, float& nb, float& sum) {
     if (valid < 64) {
 #pragma unroll
@@ -332,7 +347,7 @@ __device__ __forceinline__ void lse_chunk(uint32_t (&r)[64], float scale2, int v
     if (mx > top) {
         const float was = nb;
         top = mx;
-        nb = -mx * scale2;
+        nb = __fmul_rn(-mx, scale2);
         if (sum != 0.f) sum *= ex2(nb - was);
     }
     float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -360,10 +375,7 @@ __device__ __forceinline__ void grad_chunk(const uint32_t (&r)[64], float scale2
         stage_unit(piece, lane, u, make_uint4(p[0], p[1], p[2], p[3]));
     }
     if ((unsigned)label < 64u) {
-        float z = 0.f;
-#pragma unroll
-        for (int i = 0; i < 64; ++i)
-            if (i == label) z = __uint_as_float(r[i]);
+        const float z = pick(r, label);
         *reinterpret_cast<uint16_t*>(piece + lane * 128 + ((((unsigned)label >> 3) ^ (lane & 7)) << 4) + (label & 7) * 2) =
             va::f2bf_rn(ex2(fmaf(z, scale2, -tg.lse2)) - 1.f);
     }
@@ -437,8 +449,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int64_t token0 = (int64_t)tt * TM + r.rank * BM + quarter * 32, token = token0 + lane;
             float top = -INFINITY, nb = 0.f, sum = 0.f;
             TokenGrad tg{0.f, 0.f, -1, 0};
-            if constexpr (MODE == GRADIENT) {
-                if (token < w.tokens) tg = w.tok[token];
+            if (token < w.tokens) {
+                if constexpr (MODE == GRADIENT) {
+                    tg = w.tok[token];
+                } else {
+                    const int64_t l = w.labels[token];
+                    if (l >= 0 && l < w.rows) tg.label = (int)l;
+                }
             }
             for (int t = r0; t < r1; ++t, ++tile) {
                 if (!wait_accumulator(r, tile, lane, err, limit_ns)) goto epilogue_done;
@@ -446,17 +463,18 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const uint32_t at = r.tmem + ((uint32_t)(quarter * 32) << 16) + (tile & 1u) * BN + first;
                 const int64_t col0 = (int64_t)t * w.n + first;
                 const int valid = (int)max(min((int64_t)w.n / 2, w.rows - col0), (int64_t)0);
-                int64_t label = -1;
-                if constexpr (MODE == GRADIENT) label = (int64_t)tg.label - w.row0 - col0;
+                const int64_t label = (int64_t)tg.label - w.row0 - col0;  // the label's column of this tile half
                 // 64 columns at a time, the next ones on their way from TMEM meanwhile.
                 const auto use = [&](int c, uint32_t(&v)[64]) {
+                    const int at_label = (int)max(min(label, (int64_t)BN) - 64 * c, (int64_t)-1);
                     if constexpr (MODE == FORWARD) {
                         lse_chunk(v, w.scale2, valid - 64 * c, top, nb, sum);
+                        if ((unsigned)at_label < 64u) w.label_dot[token] = pick(v, at_label);
                     } else {
                         // the store that last used the piece has read it
                         if (lane == 0) bulk_wait_read<0>();
                         __syncwarp();
-                        grad_chunk(v, w.scale2, tg, (int)max(min(label, (int64_t)BN) - 64 * c, (int64_t)-1), piece, lane);
+                        grad_chunk(v, w.scale2, tg, at_label, piece, lane);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) {
@@ -481,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
             if constexpr (MODE == FORWARD)
-                w.part[((int64_t)split * 2 + half) * w.token_tiles * TM + token] = make_float2(-nb, sum);
+                w.part[((int64_t)split * 2 + half) * w.token_tiles * TM + token] = make_float2(top, sum);
         }
     epilogue_done:
         if (MODE == GRADIENT && lane == 0) bulk_wait_all();
@@ -703,61 +721,48 @@ __global__ void __launch_bounds__(THREADS, 1)
 // ------------------------------------------------------------------------------------------------
 // The small kernels around them
 // ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float dot8(uint4 a, uint4 b) {
-    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        s = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), s);
-        s = fmaf(__uint_as_float(x[i] & 0xFFFF0000u), __uint_as_float(y[i] & 0xFFFF0000u), s);
-    }
-    return s;
-}
-
-// One warp per token: joins the (maximum, sum) pairs of the splits' halves and forms the label's logit.
+// One warp per token: joins the (maximum, sum) pairs of the splits' halves and forms lse and the loss.
+// With m the largest h . w, M = fl(m c log2 e) what its part's sum is relative to and d = m c log2 e - M what M was
+// rounded by, lse = c m + ln 2 (log2(sum) - d): the large term is rounded once. The loss takes c (m - h . w_label) in
+// its place, with the label's product from the same tile that entered the sum, so that a label which holds nearly all
+// of the probability costs no cancellation; what rounding leaves below zero is zero.
 __global__ void __launch_bounds__(128)
-    k_xent_join(const float2* part, int splits, int64_t pitch, const uint16_t* h, int64_t h_stride, const uint16_t* table,
-                int64_t w_stride, const int64_t* labels, int64_t tokens, int64_t rows, int dim, float scale, float* loss, float* lse) {
+    k_xent_join(const float2* part, int splits, int64_t pitch, const float* label_dot, const int64_t* labels, int64_t tokens,
+                int64_t rows, float scale, float scale2, float* loss, float* lse) {
     pdl_start();
     const int lane = threadIdx.x & 31;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (t >= tokens) return;
     float top = -INFINITY, sum = 0.f;
+    const auto join = [&](float m, float s) {  // (the products are rounded by themselves, as in the parts)
+        const float both = fmaxf(top, m), base = __fmul_rn(both, scale2);
+        sum = (sum != 0.f ? sum * ex2(__fmul_rn(top, scale2) - base) : 0.f) + (s != 0.f ? s * ex2(__fmul_rn(m, scale2) - base) : 0.f);
+        top = both;
+    };
     // Eight pairs in flight per lane. (Loads of what the kernel before wrote go to L2.)
     for (int i0 = lane; i0 < splits; i0 += 256) {
         float2 p[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) p[k] = i0 + 32 * k < splits ? __ldcg(part + (i0 + 32 * k) * pitch + t) : make_float2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (p[k].y == 0.f) continue;  // no finite logit there
-            const float m = fmaxf(top, p[k].x);
-            sum = (sum != 0.f ? sum * ex2(top - m) : 0.f) + p[k].y * ex2(p[k].x - m);
-            top = m;
-        }
+        for (int k = 0; k < 8; ++k)
+            if (p[k].y != 0.f) join(p[k].x, p[k].y);  // (0: no finite logit there)
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const float ot = __shfl_xor_sync(0xFFFFFFFFu, top, o), os = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        const float m = fmaxf(top, ot);
-        sum = (sum != 0.f ? sum * ex2(top - m) : 0.f) + (os != 0.f ? os * ex2(ot - m) : 0.f);
-        top = m;
+        const float m = __shfl_xor_sync(0xFFFFFFFFu, top, o), s = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        join(m, s);
     }
-    const int64_t label = labels[t];
-    const bool valid = label >= 0 && label < rows;
-    float dot = 0.f;
-    if (valid) {
-        const uint16_t* a = h + t * h_stride;
-        const uint16_t* b = table + label * w_stride;
-        for (int j = lane * 8; j < dim; j += 256)
-            dot += dot8(*reinterpret_cast<const uint4*>(a + j), *reinterpret_cast<const uint4*>(b + j));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
     if (lane == 0) {
-        const float l = sum != 0.f ? (top + log2f(sum)) * LN2 : -INFINITY;
-        lse[t] = l;
-        loss[t] = valid ? l - dot * scale : 0.f;
+        const int64_t label = labels[t];
+        const float rest = LN2 * (log2f(sum) - fmaf(top, scale2, -__fmul_rn(top, scale2)));
+        lse[t] = sum != 0.f ? fmaf(scale, top, rest) : -INFINITY;
+        float l = 0.f;
+        if (label >= 0 && label < rows) {
+            l = sum != 0.f ? fmaf(scale, top - __ldcg(label_dot + t), rest) : __int_as_float(0x7FC00000);
+            l = l < 0.f ? 0.f : l;
+        }
+        loss[t] = l;
     }
 }
 
@@ -872,7 +877,7 @@ bool use_pairs(int sms, int64_t tokens, int64_t rows) {
 struct ForwardPlan {
     bool pair;
     int n, token_tiles, row_tiles, splits;
-    size_t bytes;
+    size_t off_dot, bytes;
 };
 
 ForwardPlan plan_forward(int sms, int64_t tokens, int64_t rows) {
@@ -893,7 +898,8 @@ ForwardPlan plan_forward(int sms, int64_t tokens, int64_t rows) {
             p.splits = sp;
         }
     }
-    p.bytes = (size_t)p.splits * 2 * p.token_tiles * tm * sizeof(float2);
+    p.off_dot = (size_t)p.splits * 2 * p.token_tiles * tm * sizeof(float2);
+    p.bytes = p.off_dot + (size_t)tokens * sizeof(float);
     return p;
 }
 
@@ -1050,10 +1056,12 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
     w.k_blocks = (dim + BK - 1) / BK;
     w.scale2 = logit_scale * LOG2E;
     w.part = static_cast<float2*>(ws);
+    w.labels = labels;
+    w.label_dot = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_dot);
     VA_TRY(launch_scores<FORWARD>(ctx, p.pair, mh, mw, mh, w));
     return launch<k_xent_join>(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_join", (const float2*)w.part, 2 * p.splits,
-                  (int64_t)p.token_tiles * (p.pair ? 2 * BM : BM), hidden, hidden_stride, table, table_stride, labels, tokens, rows,
-                  dim, logit_scale, loss, lse);
+                  (int64_t)p.token_tiles * (p.pair ? 2 * BM : BM), (const float*)w.label_dot, labels, tokens, rows, logit_scale, w.scale2,
+                  loss, lse);
 }
 
 int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hidden_stride, const uint16_t* table,
