@@ -497,8 +497,8 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
 /* Gradients of sum_t grad_loss[t] * loss[t] (grad_loss NULL: 1) with respect to hidden and table, bf16,
  * contiguous [tokens x dim] and [rows x dim], both written whole (neither may be hidden or table); lse is the forward pass's. The logits are
  * recomputed in chunks of table rows. Roundings to bf16 before the products, which are summed in fp32: softmax
- * minus one-hot; and, for grad_table, hidden rows weighted by their grad_loss relative to the first token's (exact
- * where these are equal). */
+ * minus one-hot; and, for grad_table, hidden rows weighted by their grad_loss relative to the largest of the tokens with
+ * a loss (exact where these are equal in size). */
 int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hidden_stride, const uint16_t* table,
                              int64_t table_stride, const int64_t* labels, const float* lse, const float* grad_loss,
                              int64_t tokens, int64_t rows, int dim, float logit_scale, void* workspace,

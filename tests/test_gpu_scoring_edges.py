@@ -8,8 +8,9 @@ import pytest
 import torch
 
 import vectoraccelerate_b200 as va
-from test_gpu_scoring import (DT, SCALE_TOL, U32, gen, make_queries, make_table, matvec_reference,  # noqa: F401
-                              matvec_tolerance, norm_reference, randn, run_loss, run_matvec, run_norm, tctx, unpack)
+from test_gpu_scoring import (DT, SCALE_TOL, U16, U32, check_loss, gen, loss_reference, make_loss,  # noqa: F401
+                              make_queries, make_table, matvec_reference, matvec_tolerance, norm_reference, randn,
+                              run_loss, run_matvec, run_norm, tctx, unpack)
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +156,29 @@ def test_loss_of_whole_numbers_is_exact_to_fp32(tctx):  # noqa: F811
         rest = (v / 256 + 64) * U32 + 2.0 ** -21
         assert ((loss.double() - exact).abs() <= rest + 3 * U32 * exact.abs()).all()
         assert ((lse.double() - want).abs() <= rest + 1.01 * U32 * want.abs()).all()
+
+
+@pytest.mark.parametrize("t, v, d", [(700, 500, 64), (3000, 900, 72), (2100, 20000, 136)])
+@pytest.mark.parametrize("lead", [1, 257, 600])
+def test_loss_equal_weights_wherever_ignored_tokens_lie(tctx, t, v, d, lead):  # noqa: F811
+    # equal weights that are no powers of two: hidden rows enter the table's gradient as they are, so that ignored
+    # tokens in front change nothing but the order of sums
+    h, w, labels, _ = make_loss(t + lead, t, v, d, ignored=0.0)
+    labels[:lead] = -100
+    grad = torch.full((t,), 1.0 / 6553, device="cuda")
+    _, _, _, dw = run_loss(tctx, h, w, labels, 1.0, grad)
+    ones = run_loss(tctx, h, w, labels, 1.0, None)[3]
+    # dw = rho * sum(G h) with the same G and h: the fp32 sums are those of weights of 1
+    want = (ones.double() * float(grad[0])).float()
+    # `ones` is rounded to bf16, and so is dw, the same sums times rho: two roundings of half a step each apart
+    assert ((dw.double() - want.double()).abs() <= 2 * U16 * want.double().abs() * (1 + U16) + 1e-38).all()
+    check_loss(run_loss(tctx, h, w, labels, 1.0, grad), loss_reference(h, w, labels, 1.0, grad))
+
+
+def test_loss_weights_far_apart(tctx):  # noqa: F811
+    # |c g| of 2^-59 first and 2^100 later: nothing overflows on the way to a gradient that fp32 holds
+    h, w, labels, _ = make_loss(18, 300, 900, 64, ignored=0.0)
+    for small, large in ((2.0 ** -59, 2.0 ** 100), (2.0 ** -100, 3.0 ** 60), (2.0 ** -120, 1.0), (1.0, 2.0 ** -120)):
+        grad = torch.full((300,), small, device="cuda")
+        grad[150:] = large
+        check_loss(run_loss(tctx, h, w, labels, 1.0, grad), loss_reference(h, w, labels, 1.0, grad))

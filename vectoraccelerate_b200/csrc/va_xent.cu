@@ -32,8 +32,8 @@
 // Roundings: G is kept as P - [label] in bf16, without c g_t: a label's entry is then -1 to within its p, where
 // c g_t itself would round alike for every token of a mean and bias the gradients by up to 2^-8 (measured: 0.33%
 // instead of 0.20% off at 8192 x 131072 x 1536). dh's rows take c g_t when they are finished, in fp32. dw needs it
-// inside the sum: h's rows enter as bf16(h c g_t / rho) and dw is multiplied by rho, the |c g| of the first token with a
-// loss, so that equal weights leave h as it is. Everything else is fp32. All orders of summation are fixed.
+// inside the sum: h's rows enter as bf16(h c g_t / rho) and dw is multiplied by rho, the largest |c g| of the batch, so that
+// equal weights leave h as it is. Everything else is fp32. All orders of summation are fixed.
 #include <algorithm>
 #include <cmath>
 
@@ -57,6 +57,9 @@ constexpr size_t SMEM = 1024 + RING_BYTES + EPI_WARPS * EPI_BYTES + (2 * 6 + 5) 
 // A gradient tile costs its K blocks, but at least this many: its results leave in that time (64 x 100000 x 768: both
 // products 84 us with 1, 72 with 2 to 4, 86 with 8).
 constexpr int TILE_END = 3;
+// Up to this many tokens every block of k_xent_tokens looks for the largest weight among all of them (2 us at most,
+// as long as the launch that it saves); beyond, WEIGHT_PARTS blocks do it first.
+constexpr int FEW_TOKENS = 2048, WEIGHT_PARTS = 128;
 constexpr int64_t G_ENTRIES = 1 << 28;    // gradient entries of a chunk (512 MB of bf16)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
@@ -771,27 +774,48 @@ __device__ __forceinline__ float token_scale(const int64_t* labels, const float*
     return label >= 0 && label < rows ? scale * (grad ? grad[t] : 1.f) : 0.f;
 }
 
+// The largest of the numbers (not negative) of a block's threads; all of them get it.
+template <int WARPS>
+__device__ __forceinline__ float largest_of_block(float m) {
+    __shared__ float s_max[WARPS];
+    m = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m)));  // (ordered like their bits)
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_max[w]);
+    return m;
+}
+
+// Many tokens: the largest |c g| of each block's share.
+__global__ void __launch_bounds__(256)
+    k_xent_weights(const int64_t* labels, const float* grad, int64_t tokens, int64_t rows, float scale, float* part) {
+    float m = 0.f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tokens; i += (int64_t)gridDim.x * 256)
+        m = fmaxf(m, fabsf(token_scale(labels, grad, i, rows, scale)));
+    m = largest_of_block<8>(m);
+    if (threadIdx.x == 0) part[blockIdx.x] = m;
+}
+
 // One warp per token: what the backward pass needs of it, and its row of h times c g / rho, with tokens without
-// loss set to zero (their rows may hold anything; 0 * NaN would reach the table's gradient). rho is |c g| of the
-// first of the leading 256 tokens that has a loss, if it lies within 2^-60..2^60 (the quotients then stay in range),
-// else 1.
+// loss set to zero (their rows may hold anything; 0 * NaN would reach the table's gradient). rho is the largest |c g|
+// of the batch, so that no quotient is above 1 (where it is not finite, or no token has a loss: 1). It comes from `parts`
+// shares, or, with few tokens, from all of them in every block: a launch takes longer than that.
 __global__ void __launch_bounds__(128)
     k_xent_tokens(const uint16_t* h, int64_t h_stride, const int64_t* labels, const float* lse, const float* grad, int64_t tokens,
-                  int64_t rows, int dim, float scale, TokenGrad* tok, float* rho_out, uint16_t* weighted) {
+                  int64_t rows, int dim, float scale, const float* part, int parts, TokenGrad* tok, float* rho_out, uint16_t* weighted) {
     pdl_start();
     const int lane = threadIdx.x & 31;
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (t >= tokens) return;
-    float rho = 1.f;
-    for (int64_t i = lane; i - lane < min(tokens, (int64_t)256); i += 32) {
-        const float g = i < tokens ? fabsf(token_scale(labels, grad, i, rows, scale)) : 0.f;
-        const uint32_t any = __ballot_sync(0xFFFFFFFFu, g != 0.f);
-        if (any) {
-            const float first = __shfl_sync(0xFFFFFFFFu, g, __ffs(any) - 1);
-            if (first > 0x1p-60f && first < 0x1p60f) rho = first;
-            break;
-        }
+    float rho = 0.f;
+    if (parts) {
+        if (threadIdx.x < parts) rho = part[threadIdx.x];
+    } else {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < (int)tokens; i += 128) rho = fmaxf(rho, fabsf(token_scale(labels, grad, i, rows, scale)));
     }
+    rho = largest_of_block<4>(rho);
+    if (!(rho > 0.f && rho < INFINITY)) rho = 1.f;
+    if (t >= tokens) return;
     const float g = token_scale(labels, grad, t, rows, scale), f = g / rho;
     if (lane == 0) {
         tok[t] = TokenGrad{lse[t] * LOG2E, g, g != 0.f ? (int)labels[t] : -1, 0};
@@ -935,7 +959,7 @@ BackwardPlan plan_backward(int sms, int64_t tokens, int64_t rows, int dim) {
     const int64_t room_w = std::max<int64_t>(1, ((int64_t)64 << 20) / (p.rows_pad * dim * 4));
     p.splits_w = chunks > 1 ? 1 : (int)std::min(std::min((kb_tokens + item - 1) / item, room_w), kb_tokens);
     p.off_rho = (size_t)tokens * sizeof(TokenGrad);
-    p.off_h = (size_t)up((int64_t)p.off_rho + 4, 1024);
+    p.off_h = (size_t)up((int64_t)p.off_rho + 4 * (1 + WEIGHT_PARTS), 1024);
     p.off_dh = p.off_h + (size_t)up(tokens * dim * 2, 1024);
     p.off_dw = p.off_dh + (size_t)up((int64_t)p.splits * p.token_tiles * tm * dim * 4, 1024);
     p.off_g = p.off_dw + (p.splits_w > 1 ? (size_t)up(p.splits_w * p.rows_pad * dim * 4, 1024) : 0);
@@ -1090,8 +1114,12 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
     float* dh = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_dh);
     float* dw = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_dw);
     uint16_t* g = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_g);
+    const int parts = tokens > FEW_TOKENS ? (int)std::min<int64_t>(WEIGHT_PARTS, (tokens + 255) / 256) : 0;
+    if (parts)
+        VA_TRY(launch<k_xent_weights>(ctx, (unsigned)parts, 256, 0, false, "k_xent_weights", labels, grad_loss, tokens, rows, logit_scale,
+                      rho + 1));
     VA_TRY(launch<k_xent_tokens>(ctx, (unsigned)((tokens + 3) / 4), 128, 0, false, "k_xent_tokens", hidden, hidden_stride, labels, lse,
-                  grad_loss, tokens, rows, dim, logit_scale, tok, rho, weighted));
+                  grad_loss, tokens, rows, dim, logit_scale, (const float*)(rho + 1), parts, tok, rho, weighted));
 
     const int tm = p.pair ? 2 * BM : BM;
     const int64_t tokens_pad = (int64_t)p.token_tiles * tm;
