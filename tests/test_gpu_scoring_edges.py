@@ -4,6 +4,8 @@ loss, bounded waits that run out, calls that have to be refused.
 Tolerances count roundings: fp32 2^-24 and bf16 2^-8 of the value each (half a unit in the last place).
 """
 
+import time
+
 import pytest
 import torch
 
@@ -182,3 +184,54 @@ def test_loss_weights_far_apart(tctx):  # noqa: F811
         grad = torch.full((300,), small, device="cuda")
         grad[150:] = large
         check_loss(run_loss(tctx, h, w, labels, 1.0, grad), loss_reference(h, w, labels, 1.0, grad))
+
+
+# ------------------------------------------------------------------------------------------ bounded waits
+@pytest.fixture
+def stalled(monkeypatch):
+    """Issuers of the tile kernels stop after some tiles and waits expire after 50 ms, while the returned call runs."""
+    def run(c, tiles, call):
+        with monkeypatch.context() as m:
+            m.setenv("VA_TC_TEST_STALL_TILES", str(tiles))
+            m.setenv("VA_TC_WAIT_LIMIT_MS", "50")
+            start = time.perf_counter()
+            call()
+            with pytest.raises(va.Timeout, match="bounded device-side wait expired"):
+                c.synchronize()
+            # far below the second that draining a copy which never was may take
+            assert time.perf_counter() - start < 0.9
+        c.synchronize()  # the error has been taken
+    return run
+
+
+@pytest.mark.parametrize("n, dim, nq, dtype, copies", [(200000, 512, 1, "f32", 0), (200000, 512, 1, "f32", 4), (200000, 1536, 16, "int8", 1),
+                                                       (200000, 1536, 16, "int8", 8), (300, 4096, 4, "bf16", 0), (300, 4096, 4, "bf16", 1),
+                                                       (40000, 4096, 5, "f32", 3)])
+def test_matvec_wait_expires_and_the_context_recovers(tctx, stalled, n, dim, nq, dtype, copies):  # noqa: F811
+    g = gen(n)
+    codes, scales, zp = make_table(g, n, dim, 64, "bf16", False)
+    x, xs = make_queries(g, nq, dim, dtype)
+    k = va.Int4MatVecKernel(tctx)
+    out = torch.empty(nq, n, device="cuda")
+    dt = {"f32": va.DTYPE_F32, "bf16": va.DTYPE_BF16, "int8": va.DTYPE_INT8}[dtype]
+    torch.cuda.synchronize()
+    stalled(tctx, copies, lambda: k.encode(x, nq, codes, scales, n, dim, 64, out, zp, dt, xs))
+    out = run_matvec(tctx, x, xs, codes, scales, zp, dim, 64)
+    want, size = matvec_reference(x, xs, codes, scales, zp, dim, 64)
+    assert ((out.double() - want).abs() <= matvec_tolerance(dim, 64) * size).all()
+
+
+@pytest.mark.parametrize("t, v, d, tiles", [(120, 50000, 136, 0), (300, 5003, 320, 0), (513, 30000, 768, 0), (513, 30000, 768, 1),
+                                            (2047, 9999, 1000, 2)])  # single CTAs, narrow tiles, pairs
+def test_loss_wait_expires_and_the_context_recovers(tctx, stalled, t, v, d, tiles):  # noqa: F811
+    h, w, labels, grad = make_loss(t + v, t, v, d)
+    k = va.SoftmaxCrossEntropyKernel(tctx)
+    loss, lse, dh, dw = torch.empty(t, device="cuda"), torch.empty(t, device="cuda"), torch.empty_like(h), torch.empty_like(w)
+    want = loss_reference(h, w, labels, 1.0, grad)
+    torch.cuda.synchronize()
+    stalled(tctx, tiles, lambda: k.encode_forward(h, w, labels, t, v, d, loss, lse))
+    check_loss(run_loss(tctx, h, w, labels, 1.0, grad), want)
+    lse.copy_(want[1])
+    torch.cuda.synchronize()
+    stalled(tctx, tiles, lambda: k.encode_backward(h, w, labels, lse, grad, t, v, d, dh, dw))
+    check_loss(run_loss(tctx, h, w, labels, 1.0, grad), want)

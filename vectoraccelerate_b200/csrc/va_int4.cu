@@ -60,6 +60,7 @@ struct MatvecArgs {
     int chunks;  // 256-code chunks per row
     int wk;      // warps sharing a row tile
     int ring;    // slots per warp
+    int stall;   // -1, or (tests) the copies after which a warp's issuer stops
 };
 
 // What a column of B holds: an int8 query; a digit of a query; a query (bf16) or its three pieces in turn (fp32).
@@ -312,8 +313,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     if (threadIdx.x == 0) *s_abort = 0;
     __syncwarp();
     // Position of the next load to issue (lane 0): slot, row tile and chunk.
-    int64_t left = (int64_t)tiles * mine;
-    uint32_t issued = 0;  // counted to the ring's length only
+    int64_t left = a.stall < 0 ? (int64_t)tiles * mine : min((int64_t)tiles * mine, (int64_t)a.stall);
     int issue_tile = first, issue_chunk = part;
     auto issue = [&](int s) {
         mbar_expect_tx(&full[s], SLOT);
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         }
     };
     if (lane == 0)
-        for (; issued < (uint32_t)a.ring && left > 0; ++issued) issue((int)issued);
+        for (int i = 0; i < a.ring && left > 0; ++i) issue(i);
     Scales next;
     int64_t base[4];
     row_bases(a, min(first, a.row_tiles - 1), g, base);
@@ -344,6 +344,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     bool dead = false;
     int s = 0;
     uint32_t phase = 0;
+    // After a wait for chunk c of tile k has expired: copies in flight, those issued and not yet used, write this block's
+    // shared memory, so it stays until they have landed. None is issued after that.
+    const auto settle = [&](int k, int c) {
+        const int per_tile = (a.chunks - part + a.wk - 1) / a.wk;
+        const int64_t all = (int64_t)tiles * per_tile, copies = a.stall < 0 ? all : min(all, (int64_t)a.stall);
+        const int flying = (int)(copies - left - ((int64_t)k * per_tile + (c - part) / a.wk));
+        for (int i = s; i < s + flying; ++i)
+            mbar_drain(&full[i < a.ring ? i : i - a.ring], i < a.ring ? phase : phase ^ 1u, kDrainLimitNs);
+    };
     constexpr int ACC = WIDE ? 2 : 4;  // sums per row tile half: rows g and g + 8, of a pair of columns each or added up
     for (int k = 0; k < tiles; ++k) {
         const int tile = first + k * step;
@@ -364,7 +373,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 next.load(a, base, part, t);
             }
             // Every lane waits: the phase it has seen is what makes the copy's bytes visible to it.
-            if (!dead) dead = __any_sync(0xFFFFFFFFu, !mbar_wait(&full[s], phase, s_abort, err, limit_ns));
+            if (!dead && __any_sync(0xFFFFFFFFu, !mbar_wait(&full[s], phase, s_abort, err, limit_ns))) {
+                dead = true;
+                if (lane == 0) settle(k, c);
+            }
             if (dead) break;
             const uint32_t slot = slot0 + s * SLOT;
             const uint2* fr = frag0 + (size_t)c * NT * (frag_bytes(MODE) / 8);
@@ -539,11 +551,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                     }
         }
     }
-    // After an expired wait: copies still in flight write this block's shared memory. Of slot i the last
-    // copy issued completes phase `phase` (slots from s on) or the next one (slots already reissued).
-    if (dead && lane == 0)
-        for (int i = 0; i < a.ring && i < (int)issued; ++i)
-            mbar_drain(&full[i], i >= s ? phase : phase ^ 1u, kDrainLimitNs);
 }
 
 // Warps per block: what the registers allow (128 a thread at 16 warps).
@@ -889,6 +896,7 @@ int va_int4_matvec(va_context* ctx, const void* x, int x_dtype, const float* x_s
     a.x_pitch = dim;
     a.scale_pitch = (dim + group - 1) / group;
     a.x_dtype = x_dtype;
+    a.stall = test_stall_tiles();
     const int chunks = (dim + CHUNK - 1) / CHUNK;
     l.grid = std::min(ctx->sm_count, a.row_tiles);
     int mapped = -1;  // the chunk at which the tensor map starts

@@ -943,15 +943,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
 }
 
-// Test hooks of the bounded-wait path, read at every launch: VA_TC_WAIT_LIMIT_MS replaces the
-// device waits' limit; VA_TC_TEST_STALL_TILES makes the single-CTA kernel's MMA issuer stop after
-// that many tiles (the pair kernel ignores it), so a bounded wait expires and the launch reports
-// VA_ERR_TIMEOUT through va_synchronize. Unset in normal use.
-int test_stall_tiles() {
-    const char* e = getenv("VA_TC_TEST_STALL_TILES");
-    return e && e[0] ? std::max(0, atoi(e)) : -1;
-}
-
 int make_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols_elems, int elem_bytes, int box_rows) {
     auto enc = get_encode_fn();
     if (!enc) return va_set_error(VA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
@@ -1142,7 +1133,7 @@ int va_tc_filter(va_context* ctx, const TcFilterArgs& a, const TcPlan& p) {
     w.pair_div = 1;
     w.item_base = 0;
     w.lv = a.levels.n > 0 ? a.levels : one_level(p.kp);
-    w.stall_tiles = test_stall_tiles();
+    w.stall_tiles = test_stall_tiles();  // (the pair kernel ignores it)
     for (int l = 0; l < w.lv.n; ++l)
         if (w.lv.rank[l] < 1 || w.lv.rank[l] > p.kp || w.lv.slots[l] < 1)
             return va_set_error(VA_ERR_INVALID_ARG, "bound level %d: rank %d / slots %d invalid for lists of %d", l,

@@ -205,8 +205,15 @@ inline PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
     return fn;
 }
 
-// Bound of the device waits of a launch; VA_TC_WAIT_LIMIT_MS (a test hook, read at every launch)
-// replaces the context's limit.
+// Test hooks of the bounded-wait path, read at every launch: VA_TC_WAIT_LIMIT_MS replaces the
+// context's limit of the device waits; VA_TC_TEST_STALL_TILES makes a kernel's issuer (of MMAs, or of
+// the matvec's copies) stop after that many tiles, so a bounded wait expires and the launch reports
+// VA_ERR_TIMEOUT through va_synchronize. Unset (-1) in normal use.
+inline int test_stall_tiles() {
+    const char* e = getenv("VA_TC_TEST_STALL_TILES");
+    const int v = e && e[0] ? atoi(e) : -1;
+    return e && e[0] && v < 0 ? 0 : v;
+}
 inline uint64_t wait_limit_ns(unsigned limit_ms) {
     const char* e = getenv("VA_TC_WAIT_LIMIT_MS");
     const long v = e ? atol(e) : 0;

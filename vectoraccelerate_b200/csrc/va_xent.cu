@@ -123,8 +123,8 @@ struct Roles {
         if (leader()) drain_loads(full, Tile<PAIR>::STAGES, issued);
         if constexpr (PAIR) settle_ns(1000000ull);
     }
-    __device__ __forceinline__ void settle_mmas() const {
-        if (!*abort_flag) return;
+    __device__ __forceinline__ void settle_mmas(bool stalled) const {
+        if (!*abort_flag && !stalled) return;
         if constexpr (PAIR)
             mma_commit_pair(map_rank(smem_u32(dbar), 0));
         else
@@ -308,6 +308,7 @@ struct ScoreWork {
     int64_t row0;
     int token_tiles, row_tiles, splits, k_blocks;
     int n;                 // table rows of a tile: 256, or 128 (single CTAs)
+    int stall_tiles;       // -1, or (tests) the tiles after which a worker's MMA issuer stops
     float scale2;          // c * log2(e)
     float2* part;          // forward: (maximum of h . w, sum) per [split][column half][token_tiles * tile rows]
     const int64_t* labels; // forward
@@ -424,6 +425,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int item = r.worker; item < n_items && !*r.abort_flag; item += r.workers) {
                 score_item(w, item, tt, split, r0, r1);
                 for (int t = r0; t < r1; ++t, ++tile) {
+                    if ((int)tile == w.stall_tiles) goto mma_done;
                     if (!r.wait(&r.tempty[tile & 1u], ((tile >> 1) & 1u) ^ 1u, err, limit_ns)) goto mma_done;
                     tc_fence_after();
                     const uint32_t d = r.tmem + (tile & 1u) * BN;
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
         mma_done:
-            r.settle_mmas();
+            r.settle_mmas(w.stall_tiles >= 0);
         }
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
@@ -529,6 +531,7 @@ struct GradWork {
     int kb_rows, kb_tokens; // K blocks of 64: chunk rows, tokens
     int first;              // first chunk: dh is stored, else added
     int long_h;             // dh items are the longer ones and go out first
+    int stall_tiles;        // as in ScoreWork
     int extra;              // shorter items given first to the workers that got one longer item less
 };
 
@@ -628,6 +631,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int k = 0, item; (item = grad_item(w, r.worker, r.workers, k, is_h)) >= 0 && !*r.abort_flag; ++k) {
                 const GradTile t = grad_tile(w, item, is_h);
                 if (t.kb0 >= t.kb1) continue;
+                if ((int)tile == w.stall_tiles) goto mma_done;
                 if (!r.wait(&r.tempty[tile & 1u], ((tile >> 1) & 1u) ^ 1u, err, limit_ns)) goto mma_done;
                 tc_fence_after();
                 const uint32_t d = r.tmem + (tile & 1u) * BN;
@@ -647,7 +651,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 ++tile;
             }
         mma_done:
-            r.settle_mmas();
+            r.settle_mmas(w.stall_tiles >= 0);
         }
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
@@ -1080,6 +1084,7 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
     w.k_blocks = (dim + BK - 1) / BK;
     w.scale2 = logit_scale * LOG2E;
     w.part = static_cast<float2*>(ws);
+    w.stall_tiles = test_stall_tiles();
     w.labels = labels;
     w.label_dot = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_dot);
     VA_TRY(launch_scores<FORWARD>(ctx, p.pair, mh, mw, mh, w));
@@ -1147,6 +1152,7 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
         s.k_blocks = (dim + BK - 1) / BK;
         s.scale2 = logit_scale * LOG2E;
         s.tok = tok;
+        s.stall_tiles = test_stall_tiles();
         VA_TRY(launch_scores<GRADIENT>(ctx, p.pair, mh, mw, mg_out, s));
 
         GradWork w{};
@@ -1166,6 +1172,7 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
         w.kb_rows = (int)((count + BK - 1) / BK);
         w.kb_tokens = (int)((tokens + BK - 1) / BK);
         w.first = row0 == 0;
+        w.stall_tiles = s.stall_tiles;
         const int items_h = p.token_tiles * p.d_tiles * p.splits, items_w = w.row_tiles * p.d_tiles * p.splits_w;
         const double cost_h = std::max<double>(TILE_END, (double)w.kb_rows / p.splits);
         const double cost_w = std::max<double>(TILE_END, (double)w.kb_tokens / p.splits_w);
