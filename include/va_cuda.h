@@ -328,6 +328,8 @@ int va_sq_perdim_minmax(va_context* ctx, const float* x, int64_t n, int dim, flo
 /* 4-bit rows with group scales (no reference counterpart: the reference's int4 quantizer,       */
 /* DataTransformations.metal:226-306, has one scale per array and no product with the codes)     */
 /* ------------------------------------------------------------------------------------------ */
+/* (Here, in the norm and in the cross entropy an output that shares memory with another array of the call is refused,
+ * but for the norm's residual_out in place.) */
 /* Bytes of a row of dim 4-bit codes: element 2i in the low, 2i + 1 in the high nibble of byte i
  * (two's complement, [-8, 7]), padded with zeros to a multiple of 16 bytes. */
 #define VA_INT4_ROW_BYTES(dim) ((((dim) + 31) / 32) * 16)

@@ -235,3 +235,37 @@ def test_loss_wait_expires_and_the_context_recovers(tctx, stalled, t, v, d, tile
     torch.cuda.synchronize()
     stalled(tctx, tiles, lambda: k.encode_backward(h, w, labels, lse, grad, t, v, d, dh, dw))
     check_loss(run_loss(tctx, h, w, labels, 1.0, grad), want)
+
+
+# ------------------------------------------------------------------------------------------ overlaps
+def test_outputs_between_the_rows_of_an_input(tctx):  # noqa: F811
+    # arrays that interleave without sharing a byte are not refused
+    g = gen(70)
+    buf = randn(g, 4, 128).bfloat16()
+    x, w = buf[:, :64], torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    scales = buf[1, 64:72].view(torch.float32)
+    codes = buf[2, 64:].view(torch.int8)
+    codes4 = torch.empty(4, 64, dtype=torch.int8, device="cuda")
+    want_codes, want_scales = norm_reference(x.contiguous(), w, 1e-6, 0)
+    k = va.RMSNormInt8Kernel(tctx)
+    k.encode(x, w, 4, 64, codes4, scales, x_stride=128)
+    tctx.synchronize()
+    assert torch.equal(codes4.double(), want_codes)
+    assert ((scales.double() - want_scales[:, 0]).abs() <= SCALE_TOL * want_scales[:, 0]).all()
+    k.encode(x[:2], w, 2, 64, codes, torch.empty(2, device="cuda"), x_stride=128)
+    tctx.synchronize()
+    assert torch.equal(codes.view(2, 64).double(), want_codes[:2])
+
+
+def test_workspace_over_an_argument_is_refused(tctx):  # noqa: F811
+    t, v, d = 40, 300, 64
+    h, w, labels, grad = make_loss(71, t, v, d)
+    k = va.SoftmaxCrossEntropyKernel(tctx)
+    need = max(k.workspace_bytes(t, v, d, b) for b in (False, True))
+    space = torch.empty(need + 4096, dtype=torch.uint8, device="cuda")
+    loss, lse = space[:4 * t].view(torch.float32), torch.zeros(t, device="cuda")
+    with pytest.raises(va.InvalidInput, match="workspace must not overlap loss"):
+        k.encode_forward(h, w, labels, t, v, d, loss, lse, workspace=space)
+    gh = space[1024:1024 + 2 * t * d].view(torch.bfloat16).view(t, d)
+    with pytest.raises(va.InvalidInput, match="workspace must not overlap grad_hidden"):
+        k.encode_backward(h, w, labels, lse, grad, t, v, d, gh, torch.empty_like(w), workspace=space)

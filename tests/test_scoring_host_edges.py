@@ -1,0 +1,81 @@
+"""More refusals of the scoring head, decided on the host before anything is launched: outputs that overlap other
+arrays of the call."""
+
+import pytest
+
+from test_scoring_host import BF16, CTX, F32, INT8, refused
+
+M = 1 << 20  # far apart: eight arrays of the calls below fit between multiples
+
+
+def args(base, change):
+    assert set(change) <= set(base), change
+    return list({**base, **change}.values())
+
+
+# ------------------------------------------------------------------------------------------ overlaps
+NORM = dict(ctx=CTX, x=M, residual=2 * M, weight=3 * M, rows=4, dim=64, dtype=BF16, xs=64, rs=64, eps=1e-6, group=0, out=4 * M, codes=5 * M,
+            scales=6 * M)
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(out=M + 16), "residual_out must not overlap x"), (dict(out=2 * M - 16), "residual_out must not overlap residual"),
+    (dict(out=M - 510), "residual_out must not overlap x"), (dict(out=3 * M + 126), "residual_out must not overlap weight"),
+    (dict(codes=M + 511), "codes must not overlap x"), (dict(codes=4 * M + 8), "residual_out must not overlap codes"),
+    (dict(out=M, codes=M + 256), "residual_out must not overlap codes"), (dict(scales=5 * M + 252), "codes must not overlap scales"),
+    (dict(scales=3 * M), "scales must not overlap weight"), (dict(scales=2 * M + 508), "scales must not overlap residual"),
+    (dict(out=M + 300, xs=128), "residual_out must not overlap x"),  # longer than the gap between x's rows
+    (dict(scales=M + 124, xs=128), "scales must not overlap x"), (dict(scales=M + 896 - 4, xs=128, codes=M + 512), "codes must not overlap x"),
+    (dict(dtype=F32, out=M + 1020), "residual_out must not overlap x")])
+def test_norm_overlaps(change, word):
+    refused("va_rms_norm_int8", args(NORM, change), word)
+
+
+QUANT = dict(ctx=CTX, x=M, dtype=F32, n=10, dim=64, xs=64, group=64, sd=BF16, codes=2 * M, scales=3 * M, zeros=4 * M)
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(codes=M + 2544), "codes must not overlap x"), (dict(scales=2 * M + 318), "codes must not overlap scales"),
+    (dict(zeros=2 * M), "codes must not overlap zeros"), (dict(zeros=3 * M + 19), "scales must not overlap zeros"),
+    (dict(scales=M), "scales must not overlap x"), (dict(zeros=M + 255), "zeros must not overlap x")])
+def test_quantizer_overlaps(change, word):
+    refused("va_sq_quantize_int4_groups", args(QUANT, change), word)
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(out=M + 300), "out must not overlap codes"), (dict(out=2 * M - 2556), "out must not overlap scales"),
+    (dict(out=3 * M), "out must not overlap zeros")])
+def test_dequantizer_overlaps(change, word):
+    base = dict(ctx=CTX, codes=M, scales=2 * M, zeros=3 * M, n=10, dim=64, group=64, sd=BF16, out=4 * M)
+    refused("va_sq_dequantize_int4_groups", args(base, change), word)
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(out=M + 508), "out must not overlap the queries"), (dict(out=2 * M + 4), "out must not overlap the query scales"),
+    (dict(out=3 * M - 400), "out must not overlap codes"), (dict(out=4 * M + 196), "out must not overlap scales"),
+    (dict(out=5 * M), "out must not overlap zeros"), (dict(out=2 * M - 4000, os=1000), "out must not overlap the query scales")])
+def test_matvec_overlaps(change, word):
+    base = dict(ctx=CTX, x=M, dtype=INT8, xs=2 * M, nq=8, codes=3 * M, scales=4 * M, zeros=5 * M, n=100, dim=64, group=64, sd=BF16, out=6 * M,
+                os=100)
+    refused("va_int4_matvec", args(base, change), word)
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(loss=M + 636), "loss must not overlap hidden"), (dict(lse=2 * M), "lse must not overlap table"),
+    (dict(loss=3 * M), "loss must not overlap labels"), (dict(loss=4 * M + 16, lse=4 * M), "loss must not overlap lse"),
+    (dict(lse=M + 256 - 4, hs=128), "lse must not overlap hidden")])  # the gap is 128 bytes long and starts 128 bytes on
+def test_loss_forward_overlaps(change, word):
+    base = dict(ctx=CTX, h=M, hs=64, w=2 * M, ws=64, labels=3 * M, tokens=5, rows=100, dim=64, scale=1.0, space=None, size=0, loss=4 * M,
+                lse=5 * M)
+    refused("va_softmax_xent_forward", args(base, change), word)
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(gh=M + 16), "grad_hidden must not overlap hidden"), (dict(gh=2 * M + 12784), "grad_hidden must not overlap table"),
+    (dict(gw=2 * M - 16), "grad_table must not overlap table"), (dict(gw=3 * M), "grad_table must not overlap labels"),
+    (dict(gh=4 * M), "grad_hidden must not overlap lse"), (dict(gw=5 * M), "grad_table must not overlap grad_loss"),
+    (dict(gh=7 * M + 12784), "grad_hidden must not overlap grad_table")])
+def test_loss_backward_overlaps(change, word):
+    base = dict(ctx=CTX, h=M, hs=64, w=2 * M, ws=64, labels=3 * M, lse=4 * M, g=5 * M, tokens=5, rows=100, dim=64, scale=1.0, space=None, size=0,
+                gh=6 * M, gw=7 * M)
+    refused("va_softmax_xent_backward", args(base, change), word)

@@ -843,6 +843,12 @@ int va_sq_quantize_int4_groups(va_context* ctx, const void* x, int dtype, int64_
     VA_REQUIRE(x_stride >= dim, "x_stride must be at least the dimension %d, got %lld", dim, (long long)x_stride);
     VA_REQUIRE((uintptr_t)x % (dtype == VA_DTYPE_BF16 ? 2 : 4) == 0, "x must be aligned to its elements");
     if (!n) return VA_OK;
+    const int64_t groups = (dim + group - 1) / group, es = dtype == VA_DTYPE_BF16 ? 2 : 4;
+    const VaSpan sx{"x", x, dim * es, n, x_stride * es}, sc{"codes", codes, n * VA_INT4_ROW_BYTES(dim)},
+        ss{"scales", scales, n * groups * (scale_dtype == VA_DTYPE_BF16 ? 2 : 4)}, sz{"zeros", zeros, n * groups};
+    VA_TRY(va_refuse_overlap(sc, {sx, ss, sz}));
+    VA_TRY(va_refuse_overlap(ss, {sx, sz}));
+    VA_TRY(va_refuse_overlap(sz, {sx}));
     VaDeviceGuard on(ctx->device);
     VA_CUDA_TRY(on.err);
     const GroupArgs a{x, n, x_stride, dim, (dim + group - 1) / group, VA_INT4_ROW_BYTES(dim), scale_dtype, codes, scales, zeros};
@@ -857,6 +863,10 @@ int va_sq_dequantize_int4_groups(va_context* ctx, const uint8_t* codes, const vo
     VA_REQUIRE(ctx && (!n || (codes && scales && out)), "ctx, codes, scales and out must not be NULL");
     VA_TRY(check_table(n, dim, group, scale_dtype, codes, scales));
     if (!n) return VA_OK;
+    const int64_t groups = (dim + group - 1) / group;
+    VA_TRY(va_refuse_overlap({"out", out, n * dim * 4}, {{"codes", codes, n * VA_INT4_ROW_BYTES(dim)},
+                                                         {"scales", scales, n * groups * (scale_dtype == VA_DTYPE_BF16 ? 2 : 4)},
+                                                         {"zeros", zeros, n * groups}}));
     VaDeviceGuard on(ctx->device);
     VA_CUDA_TRY(on.err);
     const GroupArgs a{nullptr, n, 0, dim, (dim + group - 1) / group, VA_INT4_ROW_BYTES(dim), scale_dtype,
@@ -881,6 +891,11 @@ int va_int4_matvec(va_context* ctx, const void* x, int x_dtype, const float* x_s
     VA_REQUIRE((uintptr_t)x % es == 0 && (uintptr_t)out % 4 == 0 && (uintptr_t)x_scales % 4 == 0,
                "queries, query scales and out must be aligned to their elements");
     if (!n || !nq) return VA_OK;
+    const int64_t all_groups = n * ((dim + group - 1) / group);
+    VA_TRY(va_refuse_overlap({"out", out, n * 4, nq, out_stride * 4},
+                             {{"the queries", x, (int64_t)nq * dim * (int64_t)es}, {"the query scales", x_scales, (int64_t)nq * 4},
+                              {"codes", codes, n * VA_INT4_ROW_BYTES(dim)},
+                              {"scales", scales, all_groups * (scale_dtype == VA_DTYPE_BF16 ? 2 : 4)}, {"zeros", zeros, all_groups}}));
     VaDeviceGuard on(ctx->device);
     VA_CUDA_TRY(on.err);
 

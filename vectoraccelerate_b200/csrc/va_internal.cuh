@@ -68,6 +68,33 @@ struct VaDeviceGuard {
     cudaError_t err = cudaSuccess;
 };
 
+// An array that a call reads or writes: `rows` rows of `bytes` each, `pitch` bytes apart (one row: `bytes` of it).
+struct VaSpan {
+    const char* name;
+    const void* at;
+    int64_t bytes;
+    int64_t rows = 1, pitch = 0;
+};
+
+// Whether one of the rows of `a` and the single row `b` share a byte.
+inline bool va_overlap(const VaSpan& a, const VaSpan& b) {
+    if (!a.at || !b.at || a.rows <= 0 || a.bytes <= 0 || b.bytes <= 0) return false;
+    const __int128 from = (__int128)(uintptr_t)b.at - (__int128)(uintptr_t)a.at, to = from + b.bytes;
+    if (a.rows == 1 || a.pitch <= a.bytes) return from < (__int128)(a.rows - 1) * a.pitch + a.bytes && to > 0;
+    // the first row that ends behind b's start
+    const __int128 first = from < a.bytes ? 0 : (from - a.bytes) / a.pitch + 1;
+    return first < a.rows && first * a.pitch < to;
+}
+
+// Refuses a call whose output shares memory with one of its other arrays.
+template <size_t N>
+int va_refuse_overlap(const VaSpan& out, const VaSpan (&others)[N]) {
+    for (const VaSpan& o : others)
+        if (out.rows == 1 ? va_overlap(o, out) : va_overlap(out, o))
+            return va_set_error(VA_ERR_INVALID_ARG, "%s must not overlap %s", out.name, o.name);
+    return VA_OK;
+}
+
 // Once per kernel and device: lets the kernel take up to `smem` bytes of dynamic shared memory (0: leaves that) and asks
 // for the large shared-memory partition, so that kernels of one call do not repartition an SM between them.
 template <auto KERN>

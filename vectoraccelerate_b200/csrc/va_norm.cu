@@ -621,6 +621,16 @@ int va_rms_norm_int8(va_context* ctx, const void* x, const void* residual, const
                 (uintptr_t)scales % 4) == 0,
                "x, residual, weight, residual_out and scales must be aligned to their elements");
     if (!rows) return VA_OK;
+    {
+        const int64_t n = rows * dim, e = (int64_t)es, groups = group ? (dim + group - 1) / group : 1;
+        const VaSpan sx{"x", residual_out == x ? nullptr : x, dim * e, rows, x_stride * e};
+        const VaSpan sr{"residual", residual_out == residual ? nullptr : residual, dim * e, rows, residual_stride * e};
+        const VaSpan sw{"weight", weight, dim * e}, so{"residual_out", residual_out, n * e}, sc{"codes", codes, n},
+            ss{"scales", scales, rows * groups * 4};
+        VA_TRY(va_refuse_overlap(so, {sx, sr, sw, sc, ss}));
+        VA_TRY(va_refuse_overlap(sc, {sx, sr, sw, ss}));
+        VA_TRY(va_refuse_overlap(ss, {sx, sr, sw}));
+    }
     VaDeviceGuard on(ctx->device);
     VA_CUDA_TRY(on.err);
     const NormArgs a{x,    residual, weight,   residual_out,    codes, scales,

@@ -1066,11 +1066,16 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
                "ctx, hidden, table, labels, loss and lse must not be NULL");
     VA_TRY(check_inputs(ctx, hidden, hidden_stride, table, table_stride, tokens, rows, dim, logit_scale));
     if (!tokens) return VA_OK;
+    const VaSpan sh{"hidden", hidden, dim * 2, tokens, hidden_stride * 2}, st{"table", table, dim * 2, rows, table_stride * 2},
+        sy{"labels", labels, tokens * 8}, so{"loss", loss, tokens * 4}, se{"lse", lse, tokens * 4};
+    VA_TRY(va_refuse_overlap(so, {sh, st, sy, se}));
+    VA_TRY(va_refuse_overlap(se, {sh, st, sy}));
     VaDeviceGuard on(ctx->device);
     VA_CUDA_TRY(on.err);
     const ForwardPlan p = plan_forward(ctx->sm_count, tokens, rows);
     void* ws;
     VA_TRY(workspace_of(ctx, workspace, workspace_bytes, p.bytes, &ws));
+    VA_TRY(va_refuse_overlap({"workspace", workspace, (int64_t)p.bytes}, {sh, st, sy, so, se}));
     CUtensorMap mh, mw;
     VA_TRY(make_map(&mh, hidden, false, dim, tokens, hidden_stride, BK, BM));
     VA_TRY(make_map(&mw, table, false, dim, rows, table_stride, BK, p.pair ? BN / 2 : p.n));
@@ -1104,6 +1109,11 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
                "grad_hidden and grad_table must be aligned to 16 bytes");
     VA_REQUIRE(grad_table != table && (!tokens || (grad_hidden != hidden && grad_hidden != table && grad_table != hidden)),
                "grad_hidden and grad_table must not be hidden or table: those are read until the end");
+    const VaSpan sh{"hidden", hidden, dim * 2, tokens, hidden_stride * 2}, st{"table", table, dim * 2, rows, table_stride * 2},
+        sy{"labels", labels, tokens * 8}, se{"lse", lse, tokens * 4}, sg{"grad_loss", grad_loss, tokens * 4},
+        gh{"grad_hidden", grad_hidden, tokens * dim * 2}, gt{"grad_table", grad_table, rows * dim * 2};
+    VA_TRY(va_refuse_overlap(gh, {sh, st, sy, se, sg, gt}));
+    VA_TRY(va_refuse_overlap(gt, {sh, st, sy, se, sg}));
     VaDeviceGuard on(ctx->device);
     VA_CUDA_TRY(on.err);
     if (!tokens) {
@@ -1113,6 +1123,7 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
     const BackwardPlan p = plan_backward(ctx->sm_count, tokens, rows, dim);
     void* ws;
     VA_TRY(workspace_of(ctx, workspace, workspace_bytes, p.bytes, &ws));
+    VA_TRY(va_refuse_overlap({"workspace", workspace, (int64_t)p.bytes}, {sh, st, sy, se, sg, gh, gt}));
     TokenGrad* tok = static_cast<TokenGrad*>(ws);
     float* rho = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.off_rho);
     uint16_t* weighted = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + p.off_h);
