@@ -1,5 +1,5 @@
 """More refusals of the scoring head, decided on the host before anything is launched: outputs that overlap other
-arrays of the call."""
+arrays of the call, addresses that do not suit their elements."""
 
 import pytest
 
@@ -79,3 +79,29 @@ def test_loss_backward_overlaps(change, word):
     base = dict(ctx=CTX, h=M, hs=64, w=2 * M, ws=64, labels=3 * M, lse=4 * M, g=5 * M, tokens=5, rows=100, dim=64, scale=1.0, space=None, size=0,
                 gh=6 * M, gw=7 * M)
     refused("va_softmax_xent_backward", args(base, change), word)
+
+
+# ------------------------------------------------------------------------------------------ alignment
+FORWARD = dict(ctx=CTX, h=M, hs=64, w=2 * M, ws=64, labels=3 * M, tokens=5, rows=100, dim=64, scale=1.0, space=None, size=0, loss=4 * M, lse=5 * M)
+BACKWARD = dict(ctx=CTX, h=M, hs=64, w=2 * M, ws=64, labels=3 * M, lse=4 * M, g=5 * M, tokens=5, rows=100, dim=64, scale=1.0, space=None, size=0,
+                gh=6 * M, gw=7 * M)
+
+
+@pytest.mark.parametrize("change", [dict(labels=3 * M + 4), dict(loss=4 * M + 2), dict(lse=5 * M + 1)])
+def test_loss_forward_alignment(change):
+    refused("va_softmax_xent_forward", args(FORWARD, change), "aligned")
+
+
+@pytest.mark.parametrize("change", [dict(labels=3 * M + 4), dict(lse=4 * M + 2), dict(g=5 * M + 2)])
+def test_loss_backward_alignment(change):
+    refused("va_softmax_xent_backward", args(BACKWARD, change), "aligned")
+
+
+def test_loss_scale_beyond_powers_of_two():
+    refused("va_softmax_xent_forward", args(FORWARD, dict(scale=3e38)), "logit_scale")
+    refused("va_softmax_xent_backward", args(BACKWARD, dict(scale=3e38)), "logit_scale")
+
+
+def test_dequantizer_alignment():
+    base = dict(ctx=CTX, codes=M, scales=2 * M, zeros=3 * M, n=10, dim=64, group=64, sd=BF16, out=4 * M + 2)
+    refused("va_sq_dequantize_int4_groups", list(base.values()), "aligned")

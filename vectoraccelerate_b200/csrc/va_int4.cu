@@ -862,6 +862,7 @@ int va_sq_dequantize_int4_groups(va_context* ctx, const uint8_t* codes, const vo
                                  int dim, int group, int scale_dtype, float* out) {
     VA_REQUIRE(ctx && (!n || (codes && scales && out)), "ctx, codes, scales and out must not be NULL");
     VA_TRY(check_table(n, dim, group, scale_dtype, codes, scales));
+    VA_REQUIRE(((uintptr_t)out & 3) == 0, "out must be aligned to its elements");
     if (!n) return VA_OK;
     const int64_t groups = (dim + group - 1) / group;
     VA_TRY(va_refuse_overlap({"out", out, n * dim * 4}, {{"codes", codes, n * VA_INT4_ROW_BYTES(dim)},

@@ -989,7 +989,8 @@ int check_inputs(va_context* ctx, const void* h, int64_t h_stride, const void* t
     VA_REQUIRE(table_stride >= dim && table_stride % 8 == 0 && table_stride < ((int64_t)1 << 36),
                "table_stride must be a multiple of 8 and at least the dimension %d, got %lld", dim, (long long)table_stride);
     VA_REQUIRE((((uintptr_t)h | (uintptr_t)table) & 15) == 0, "hidden and table must be aligned to 16 bytes");
-    VA_REQUIRE(scale > 0.f && scale < INFINITY, "logit_scale must be positive and finite, got %g", (double)scale);
+    // (the kernels work in powers of two)
+    VA_REQUIRE(scale > 0.f && scale * LOG2E < INFINITY, "logit_scale must be positive and finite, and below 2^127, got %g", (double)scale);
     return VA_OK;
 }
 
@@ -1065,6 +1066,8 @@ int va_softmax_xent_forward(va_context* ctx, const uint16_t* hidden, int64_t hid
     VA_REQUIRE(ctx && (!tokens || (hidden && table && labels && loss && lse)),
                "ctx, hidden, table, labels, loss and lse must not be NULL");
     VA_TRY(check_inputs(ctx, hidden, hidden_stride, table, table_stride, tokens, rows, dim, logit_scale));
+    VA_REQUIRE((((uintptr_t)labels & 7) | (((uintptr_t)loss | (uintptr_t)lse) & 3)) == 0,
+               "labels, loss and lse must be aligned to their elements");
     if (!tokens) return VA_OK;
     const VaSpan sh{"hidden", hidden, dim * 2, tokens, hidden_stride * 2}, st{"table", table, dim * 2, rows, table_stride * 2},
         sy{"labels", labels, tokens * 8}, so{"loss", loss, tokens * 4}, se{"lse", lse, tokens * 4};
@@ -1109,6 +1112,8 @@ int va_softmax_xent_backward(va_context* ctx, const uint16_t* hidden, int64_t hi
                "grad_hidden and grad_table must be aligned to 16 bytes");
     VA_REQUIRE(grad_table != table && (!tokens || (grad_hidden != hidden && grad_hidden != table && grad_table != hidden)),
                "grad_hidden and grad_table must not be hidden or table: those are read until the end");
+    VA_REQUIRE((((uintptr_t)labels & 7) | (((uintptr_t)lse | (uintptr_t)grad_loss) & 3)) == 0,
+               "labels, lse and grad_loss must be aligned to their elements");
     const VaSpan sh{"hidden", hidden, dim * 2, tokens, hidden_stride * 2}, st{"table", table, dim * 2, rows, table_stride * 2},
         sy{"labels", labels, tokens * 8}, se{"lse", lse, tokens * 4}, sg{"grad_loss", grad_loss, tokens * 4},
         gh{"grad_hidden", grad_hidden, tokens * dim * 2}, gt{"grad_table", grad_table, rows * dim * 2};
