@@ -1,9 +1,12 @@
 """More refusals of the scoring head, decided on the host before anything is launched: outputs that overlap other
-arrays of the call, addresses that do not suit their elements."""
+arrays of the call, addresses that do not suit their elements, buffers that have been freed."""
 
+import numpy as np
 import pytest
 
-from test_scoring_host import BF16, CTX, F32, INT8, refused
+import vectoraccelerate_b200 as va
+
+from test_scoring_host import BF16, CTX, F32, INT8, _Context, refused
 
 M = 1 << 20  # far apart: eight arrays of the calls below fit between multiples
 
@@ -105,3 +108,34 @@ def test_loss_scale_beyond_powers_of_two():
 def test_dequantizer_alignment():
     base = dict(ctx=CTX, codes=M, scales=2 * M, zeros=3 * M, n=10, dim=64, group=64, sd=BF16, out=4 * M + 2)
     refused("va_sq_dequantize_int4_groups", list(base.values()), "aligned")
+
+
+# ------------------------------------------------------------------------------------------ the classes
+def freed():
+    """A DeviceBuffer as free() leaves it, without a device."""
+    b = va.DeviceBuffer.__new__(va.DeviceBuffer)
+    b.context, b.nbytes, b.dtype, b.shape, b.ptr = _Context(), 1 << 30, np.dtype(np.uint8), (1 << 30,), None
+    return b
+
+
+def test_freed_buffers_are_refused():
+    # (an optional argument that has been freed would pass for one that is not there)
+    gone = freed()
+    norm, matvec, xent = (k(_Context()) for k in (va.RMSNormInt8Kernel, va.Int4MatVecKernel, va.SoftmaxCrossEntropyKernel))
+    quant = va.Int4GroupQuantizationKernel(_Context())
+    calls = [("x", lambda: norm.encode(gone, P(3), 4, 64, P(5), P(6))),
+             ("residual", lambda: norm.encode(P(1), P(3), 4, 64, P(5), P(6), residual=gone)),
+             ("residual_out", lambda: norm.encode(P(1), P(3), 4, 64, P(5), P(6), residual=P(2), residual_out=gone)),
+             ("zero_points", lambda: quant.encode(P(1), 10, 64, 64, P(2), P(3), gone)),
+             ("zero_points", lambda: matvec.encode(P(1), 8, P(3), P(4), 100, 64, 64, P(6), zero_points=gone)),
+             ("query_scales", lambda: matvec.encode(P(1), 8, P(3), P(4), 100, 64, 64, P(6), query_dtype=INT8, query_scales=gone)),
+             ("workspace", lambda: xent.encode_forward(P(1), P(2), P(3), 5, 100, 64, P(4), P(5), workspace=gone)),
+             ("grad_loss", lambda: xent.encode_backward(P(1), P(2), P(3), P(4), gone, 5, 100, 64, P(6), P(7)))]
+    for name, call in calls:
+        with pytest.raises(va.InvalidInput, match=f"{name} has been freed"):
+            call()
+
+
+def P(i):
+    return i * M
+

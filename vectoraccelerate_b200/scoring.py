@@ -107,6 +107,8 @@ def _device_of(device: int, x, name: str) -> None:
 def _buffer(device: int, x, nbytes: int, name: str):
     if not isinstance(x, DeviceBuffer):
         raise InvalidInput(f"{name} must be a DeviceBuffer, a device address or have data_ptr(), got {type(x).__name__}")
+    if x.ptr is None:
+        raise InvalidInput(f"{name} has been freed")
     if x.context.device != device:
         raise InvalidInput(f"{name} is on device {x.context.device}, the context on device {device}")
     if x.nbytes < nbytes:
@@ -229,8 +231,12 @@ class Int4GroupQuantizationKernel(_ScoringKernel):
         """The fp32 values that the codes stand for."""
         ctx = self.context
         out = ctx.get_buffer(4 * rows.n * rows.dim, np.float32, (rows.n, rows.dim))
-        _ffi.call("va_sq_dequantize_int4_groups", self._h, rows.codes.ptr, rows.scales.ptr,
-                  rows.zero_points.ptr if rows.zero_points else None, rows.n, rows.dim, rows.group, rows.scale_dtype, out.ptr)
+        groups = -(-rows.dim // rows.group)
+        _ffi.call("va_sq_dequantize_int4_groups", self._h,
+                  _dense(self._device, rows.codes, rows.n * int4_row_bytes(rows.dim), 1, "codes"),
+                  _dense(self._device, rows.scales, rows.n * groups, _ITEM[rows.scale_dtype], "scales"),
+                  None if rows.zero_points is None else _dense(self._device, rows.zero_points, rows.n * groups, 1, "zero_points"),
+                  rows.n, rows.dim, rows.group, rows.scale_dtype, out.ptr)
         return out.download()
 
 
