@@ -1,5 +1,5 @@
 """More refusals of the scoring head, decided on the host before anything is launched: outputs that overlap other
-arrays of the call, addresses that do not suit their elements, buffers that have been freed."""
+arrays of the call, addresses that do not suit their elements, buffers that have been freed, sizes past 32 bits."""
 
 import numpy as np
 import pytest
@@ -139,3 +139,20 @@ def test_freed_buffers_are_refused():
 def P(i):
     return i * M
 
+
+def test_sizes_past_32_bits_are_refused():
+    norm, matvec, xent = (k(_Context()) for k in (va.RMSNormInt8Kernel, va.Int4MatVecKernel, va.SoftmaxCrossEntropyKernel))
+    quant = va.Int4GroupQuantizationKernel(_Context())
+    big = (1 << 32) + 64  # 64 when cut to 32 bits
+    calls = [("dimension", lambda: norm.encode(P(1), P(3), 4, big, P(5), P(6))),
+             ("group", lambda: norm.encode(P(1), P(3), 4, 64, P(5), P(6), group=big)),
+             ("dimension", lambda: quant.encode(P(1), 10, big, 64, P(2), P(3))),
+             ("dimension", lambda: matvec.encode(P(1), 8, P(3), P(4), 100, big, 64, P(6))),
+             ("num_queries", lambda: matvec.encode(P(1), big, P(3), P(4), 100, 64, 64, P(6))),
+             ("num_queries", lambda: matvec.encode(P(1), -1, P(3), P(4), 100, 64, 64, P(6))),
+             ("dimension", lambda: xent.workspace_bytes(5, 100, big, True)),
+             ("dimension", lambda: xent.encode_forward(P(1), P(2), P(3), 5, 100, big, P(4), P(5))),
+             ("dimension", lambda: xent.encode_backward(P(1), P(2), P(3), P(4), None, 5, 100, big, P(6), P(7)))]
+    for name, call in calls:
+        with pytest.raises(va.InvalidInput, match=f"{name} must be in"):
+            call()

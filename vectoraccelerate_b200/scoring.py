@@ -116,6 +116,13 @@ def _buffer(device: int, x, nbytes: int, name: str):
     return x.ptr
 
 
+def _fits(**sizes) -> None:
+    """Sizes that the library takes as 32-bit numbers, which the call would cut without a word."""
+    for name, n in sizes.items():
+        if n >> 31:
+            raise InvalidInput(f"{name} must be in 0..2147483647, got {n}")
+
+
 def _to_bf16(a) -> np.ndarray:
     """fp32 -> bf16 bit patterns (round to nearest even), for the host-array methods."""
     u = np.ascontiguousarray(a, np.float32).view(np.uint32)
@@ -143,6 +150,8 @@ class RMSNormInt8Kernel(_ScoringKernel):
         h = x + residual; ``residual_out`` receives h. Strides in elements; the dimension by default."""
         if dtype not in (_ffi.DTYPE_F32, _ffi.DTYPE_BF16):
             raise InvalidInput(f"dtype must be DTYPE_F32 or DTYPE_BF16, got {dtype}")
+        if (dimension | group) >> 31:
+            _fits(dimension=dimension, group=group)
         dev, item = self._device, _ITEM[dtype]
         xs = dimension if x_stride is None else x_stride
         rs = dimension if residual_stride is None else residual_stride
@@ -196,6 +205,8 @@ class Int4GroupQuantizationKernel(_ScoringKernel):
     def encode(self, x, rows: int, dimension: int, group: int, codes, scales, zero_points=None,
                dtype: int = _ffi.DTYPE_F32, scale_dtype: int = _ffi.DTYPE_BF16, x_stride: int | None = None) -> None:
         _check_types(dtype, scale_dtype, group, (_ffi.DTYPE_F32, _ffi.DTYPE_BF16))
+        if dimension >> 31:
+            _fits(dimension=dimension)
         dev = self._device
         stride = dimension if x_stride is None else x_stride
         groups = -(-dimension // group)
@@ -258,6 +269,8 @@ class Int4MatVecKernel(_ScoringKernel):
         """Queries [num_queries x dimension] contiguous, of ``query_dtype``; int8 queries take a scale each from
         ``query_scales``."""
         _check_types(query_dtype, scale_dtype, group, _ITEM)
+        if (dimension | num_queries) >> 31:
+            _fits(dimension=dimension, num_queries=num_queries)
         dev = self._device
         stride = rows if out_stride is None else out_stride
         groups = -(-dimension // group)
@@ -333,6 +346,7 @@ class SoftmaxCrossEntropyKernel(_ScoringKernel):
     ``Database``."""
 
     def workspace_bytes(self, tokens: int, rows: int, dimension: int, backward: bool) -> int:
+        _fits(dimension=dimension)
         n = ctypes.c_size_t()
         _ffi.call("va_softmax_xent_workspace", self._h, tokens, rows, dimension, int(backward), ctypes.byref(n))
         return n.value
@@ -363,6 +377,8 @@ class SoftmaxCrossEntropyKernel(_ScoringKernel):
                        workspace=None) -> None:
         """hidden [tokens x dimension], table [rows x dimension] bf16; labels int64 (outside [0, rows): no
         loss); loss and lse [tokens] fp32. An integer ``workspace`` address must hold workspace_bytes()."""
+        if dimension >> 31:
+            _fits(dimension=dimension)
         dev = self._device
         hs = dimension if hidden_stride is None else hidden_stride
         ts = dimension if table_stride is None else table_stride
@@ -377,6 +393,8 @@ class SoftmaxCrossEntropyKernel(_ScoringKernel):
                         grad_table, logit_scale: float = 1.0, hidden_stride: int | None = None,
                         table_stride: int | None = None, workspace=None) -> None:
         """Gradients of sum(grad_loss * loss) (``grad_loss`` None: 1), bf16 and contiguous, written whole."""
+        if dimension >> 31:
+            _fits(dimension=dimension)
         dev = self._device
         hs = dimension if hidden_stride is None else hidden_stride
         ts = dimension if table_stride is None else table_stride
