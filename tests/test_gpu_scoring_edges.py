@@ -110,6 +110,28 @@ def test_matvec_wide_queries_in_strided_rows(tctx):  # noqa: F811
     assert (wide[:, n:] == 5.0).all()
 
 
+def test_quantizer_of_groups_wider_than_fp32(tctx):  # noqa: F811
+    # finite rows whose largest and smallest elements are further apart than fp32's largest number
+    g = gen(13)
+    n, dim = 40, 256
+    x = randn(g, n, dim).clamp(-3, 3) * 1e38
+    x[::2] = x[::2].clamp(-0.5e38, 3e38)
+    for scale in ("f32", "bf16"):
+        codes = torch.empty((n, va.scoring.int4_row_bytes(dim)), dtype=torch.uint8, device="cuda")
+        scales = torch.empty((n, 4), dtype=DT[scale], device="cuda")
+        zp = torch.empty((n, 4), dtype=torch.int8, device="cuda")
+        va.Int4GroupQuantizationKernel(tctx).encode(x, n, dim, 64, codes, scales, zp, va.DTYPE_F32, va.DTYPE_F32 if scale == "f32" else va.DTYPE_BF16)
+        tctx.synchronize()
+        z = x.double().view(n, 4, 64)
+        lo, hi = z.amin(2).clamp(max=0), z.amax(2).clamp(min=0)
+        s = ((hi.float() / 2 - lo.float() / 2).double() / 7.5).float().to(DT[scale])  # hi - lo rounded once, at half its size
+        assert torch.isfinite(scales.float()).all() and torch.equal(scales, s)
+        zero = torch.round(-8 - (lo.float() / s.float())).clamp(-8, 7)
+        assert torch.equal(zp.float(), zero)
+        want = torch.round(x.view(n, 4, 64) / s.float()[:, :, None] + zero[:, :, None]).clamp(-8, 7).view(n, dim)
+        assert torch.equal(unpack(codes, dim).float(), want)
+
+
 # ------------------------------------------------------------------------------------------ loss
 @pytest.mark.parametrize("t, v, d", [(1, 1, 64), (70, 900, 128), (333, 5003, 512), (600, 30001, 256)])
 @pytest.mark.parametrize("scale", [1.0, 7.3])

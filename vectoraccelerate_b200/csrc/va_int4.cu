@@ -713,7 +713,8 @@ __global__ void __launch_bounds__(256) k_sq_q4_groups(GroupArgs a) {
             lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
             hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
         }
-        float s = a.zeros ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(-lo, hi), 7.f);
+        // (halves: hi - lo itself may leave fp32's range; the same bits otherwise, above the scales' floor)
+        float s = a.zeros ? __fdiv_rn(fmaf(hi, 0.5f, -0.5f * lo), 7.5f) : __fdiv_rn(fmaxf(-lo, hi), 7.f);
         s = fmaxf(s, 1e-8f);
         // The codes are those of the scale as it is stored.
         if (a.scale_dtype == VA_DTYPE_BF16) s = va::bf2f(va::f2bf_rn(s));
