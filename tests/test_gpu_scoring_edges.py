@@ -6,6 +6,7 @@ Tolerances count roundings: fp32 2^-24 and bf16 2^-8 of the value each (half a u
 
 import time
 
+import numpy as np
 import pytest
 import torch
 
@@ -130,6 +131,31 @@ def test_quantizer_of_groups_wider_than_fp32(tctx):  # noqa: F811
         assert torch.equal(zp.float(), zero)
         want = torch.round(x.view(n, 4, 64) / s.float()[:, :, None] + zero[:, :, None]).clamp(-8, 7).view(n, dim)
         assert torch.equal(unpack(codes, dim).float(), want)
+
+
+@pytest.mark.parametrize("kind", ["f32", "int8"])
+def test_search_keeps_a_bounded_piece_of_the_scores(ctx, monkeypatch, kind):
+    rng = np.random.default_rng(8)
+    rows, q = rng.standard_normal((20000, 96)).astype(np.float32), rng.standard_normal((333, 96)).astype(np.float32)
+    db = va.Int4Database(ctx, rows, group=32, type="asymmetric")
+    scales = None
+    if kind == "int8":
+        q, scales, _ = va.RMSNormInt8Kernel(ctx).compute(q, np.ones(96, np.float32))
+    want = db.search(q, 9, query_scales=scales)
+    sizes = []
+    get = ctx.get_buffer
+    monkeypatch.setattr(ctx, "get_buffer", lambda size, *a: sizes.append(size) or get(size, *a))
+    monkeypatch.setattr(va.Int4Database, "SCORE_BYTES", 4 * 20000 * 100)  # 96 queries
+    vals, ids = db.search(q, 9, query_scales=scales)
+    assert max(sizes) == 4 * 20000 * 96
+    # whole passes: the same scores
+    assert (ids == want[1]).all() and (vals == want[0]).all()
+    monkeypatch.setattr(va.Int4Database, "SCORE_BYTES", 1)
+    vals, ids = db.search(q, 9, query_scales=scales)
+    assert (ids == want[1]).all() and (vals == want[0]).all()
+    none, no_ids = db.search(q[:0], 9, query_scales=None if scales is None else scales[:0])
+    assert none.shape == no_ids.shape == (0, 9)
+    db.close()
 
 
 # ------------------------------------------------------------------------------------------ loss

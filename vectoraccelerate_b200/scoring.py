@@ -22,8 +22,9 @@ import numpy as np
 from . import _ffi
 from .context import DeviceBuffer, GPUContext
 from .errors import InvalidInput, raise_for_status
-from .kernels import MAXIMUM, Database, TopKSelectionKernel, _f32, _Kernel
+from .kernels import Database, TopKSelectionKernel, _f32, _Kernel
 
+_PASS = 32  # queries that no pass over 4-bit codes exceeds (va_int4_matvec)
 _ITEM = {_ffi.DTYPE_F32: 4, _ffi.DTYPE_BF16: 2, _ffi.DTYPE_INT8: 1}
 
 
@@ -297,14 +298,16 @@ class Int4MatVecKernel(_ScoringKernel):
 
 class Int4Database:
     """Resident 4-bit rows searched by inner product: scores of every row (Int4MatVecKernel), then the
-    k largest (TopKSelectionKernel), ids by (score, id). The fp32 rows are not kept."""
+    k largest (TopKSelectionKernel's selection), ids by (score, id). The fp32 rows are not kept."""
+
+    SCORE_BYTES = 1 << 28  # of scores that a search keeps at a time (at least those of 32 queries)
 
     def __init__(self, context: GPUContext, rows, group: int = 64, type: str = "symmetric",  # noqa: A002
                  scale_dtype: int = _ffi.DTYPE_BF16):
         self.context = context
         self.table = Int4GroupQuantizationKernel(context).quantize(rows, group, type, scale_dtype)
         self.n, self.dim = self.table.n, self.table.dim
-        self._matvec, self._select = Int4MatVecKernel(context), TopKSelectionKernel(context)
+        self._matvec = Int4MatVecKernel(context)
 
     def scores(self, queries) -> np.ndarray:
         return self._matvec.compute(queries, self.table)
@@ -328,10 +331,17 @@ class Int4Database:
                 raise InvalidInput(f"query_scales must have one entry per query ({nq}), got {s.size}")
             ds = ctx.get_buffer_for(s)
         dq = ctx.get_buffer_for(q)
-        scores = ctx.get_buffer(4 * nq * self.n, np.float32, (nq, self.n))
-        self._matvec.encode(dq, nq, t.codes, t.scales, self.n, self.dim, t.group, scores, t.zero_points,
-                            _ffi.DTYPE_INT8 if int8 else _ffi.DTYPE_F32, ds, t.scale_dtype)
-        vals, ids = self._select.execute(scores, nq, self.n, k, MAXIMUM)
+        # Scores of so many queries at a time as SCORE_BYTES hold, a multiple of what a pass over the codes takes.
+        chunk = max(1, min(nq, max(_PASS, self.SCORE_BYTES // (4 * self.n) // _PASS * _PASS)))
+        scores = ctx.get_buffer(4 * chunk * self.n, np.float32, (chunk, self.n))
+        vals, ids = ctx.get_buffer(4 * nq * k, np.float32, (nq, k)), ctx.get_buffer(4 * nq * k, np.uint32, (nq, k))
+        for q0 in range(0, nq, chunk):
+            count = min(chunk, nq - q0)
+            self._matvec.encode(dq.ptr + q0 * self.dim * q.itemsize, count, t.codes, t.scales, self.n, self.dim, t.group, scores,
+                                t.zero_points, _ffi.DTYPE_INT8 if int8 else _ffi.DTYPE_F32, ds.ptr + 4 * q0 if int8 else None,
+                                t.scale_dtype)
+            _ffi.call("va_topk_select", ctx.handle, scores.ptr, count, self.n, self.n, k, _ffi.SELECT_MAX, vals.ptr + 4 * q0 * k,
+                      ids.ptr + 4 * q0 * k, k)
         return vals.download(), ids.download()
 
     def close(self) -> None:
