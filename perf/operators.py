@@ -203,14 +203,16 @@ _kept = {}
 
 
 def _kernels():
-    """The context and kernel objects a program keeps, one set per device."""
+    """The context and kernel objects a program keeps, one set per device and stream: the calls go to the stream
+    that torch's own work around them is on."""
     device = torch.cuda.current_device()
-    if device not in _kept:
+    # Stream handle 1 is CUDA's name of the default stream (torch calls it 0).
+    stream = torch.cuda.current_stream(device).cuda_stream or 1
+    if (device, stream) not in _kept:
         import vectoraccelerate_b200 as va
-        # Stream handle 1 is CUDA's name of the default stream that torch runs on.
-        ctx = va.GPUContext(va.Metal4Configuration(device=device, stream=1))
-        _kept[device] = (va, va.RMSNormInt8Kernel(ctx), va.Int4MatVecKernel(ctx), va.SoftmaxCrossEntropyKernel(ctx))
-    return _kept[device]
+        ctx = va.GPUContext(va.Metal4Configuration(device=device, stream=stream))
+        _kept[device, stream] = (va, va.RMSNormInt8Kernel(ctx), va.Int4MatVecKernel(ctx), va.SoftmaxCrossEntropyKernel(ctx))
+    return _kept[device, stream]
 
 
 def _norm_own(s):
