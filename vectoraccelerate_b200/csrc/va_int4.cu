@@ -34,7 +34,6 @@
 //   * Few rows: WK warps share a row tile, each takes every WK-th 256-code chunk, and the first adds
 //     the partial sums in order.
 #include <algorithm>
-#include <type_traits>
 
 #include "va_tcgen05.cuh"
 
@@ -229,9 +228,8 @@ __device__ __forceinline__ void lay_out(const MatvecArgs& a, const QueryShared& 
         constexpr int LANES = GROUP / 8;  // of a group
         constexpr bool wide = MODE == DIGITS_WIDE;
         constexpr int planes = wide ? 8 : 1;
-        using Fixed = std::conditional_t<wide, long long, int>;
         const int grp = (c * CHUNK + lane * 8) / GROUP;
-        Fixed v[8];
+        uint32_t v[8][wide ? 2 : 1];  // (low and high word)
         if constexpr (wide) {
             float top = 0.f;
             int finite = 1;
@@ -247,28 +245,36 @@ __device__ __forceinline__ void lay_out(const MatvecArgs& a, const QueryShared& 
             }
             // 2^e > top; the fixed point's unit is 2^(e - 62), not below the smallest fp32. (The factor may
             // exceed fp32: two steps.)
+            const auto power = [](int n) { return __int_as_float((n + 127) << 23); };
             const int e = max((int)(__float_as_uint(top) >> 23) - 126, -87);
-            const float up = ldexpf(1.f, (62 - e) / 2), up2 = ldexpf(1.f, 62 - e - (62 - e) / 2);
+            const float up = power((62 - e) / 2), up2 = power(62 - e - (62 - e) / 2);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = finite ? __float2ll_rn(f[k] * up * up2) : 0;
+            for (int k = 0; k < 8; ++k) {
+                // With 128 added to each byte but the highest, no digit is below zero: the bytes are the digits, plus 128.
+                const long long u = (finite ? __float2ll_rn(f[k] * up * up2) : 0) + 0x0080808080808080ll;
+                v[k][0] = (uint32_t)u;
+                v[k][1] = (uint32_t)(u >> 32);
+            }
             if (lane % LANES == 0) {
-                const float none = finite ? 0.f : __int_as_float(0x7FC00000);
+                const float w = finite ? power(e - 14) : __int_as_float(0x7FC00000);
                 *reinterpret_cast<float4*>(sh.weight + ((size_t)grp * NT + q) * 4) =
-                    make_float4(ldexpf(1.f, e - 14) + none, ldexpf(1.f, e - 30) + none, ldexpf(1.f, e - 46) + none, ldexpf(1.f, e - 62) + none);
+                    make_float4(w, w * 0x1p-16f, w * 0x1p-16f * 0x1p-16f, w * 0x1p-16f * 0x1p-16f * 0x1p-16f);
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = (int)f[k];
+            for (int k = 0; k < 8; ++k) v[k][0] = (uint32_t)(int)f[k];
         }
 #pragma unroll
-        for (int p = planes - 1; p >= 0; --p) {  // digits from the lowest; column p = 0 has the highest
-            const int col = q * planes + p;
+        for (int p = 0; p < planes; ++p) {  // column 0 has the highest digit
+            constexpr int LAST = planes - 1;
+            const int col = q * planes + p, word = (LAST - p) / 4;
+            const uint32_t byte = (LAST - p) & 3, pick = byte | ((byte + 4) << 4);
             uint32_t d[2];  // even and odd elements
 #pragma unroll
-            for (int o = 0; o < 2; ++o)
-                d[o] = __byte_perm(__byte_perm((uint32_t)v[o], (uint32_t)v[2 + o], 0x0040), __byte_perm((uint32_t)v[4 + o], (uint32_t)v[6 + o], 0x0040), 0x5410);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = (v[k] - (Fixed)(int8_t)v[k]) >> 8;
+            for (int o = 0; o < 2; ++o) {
+                d[o] = __byte_perm(__byte_perm(v[o][word], v[2 + o][word], pick), __byte_perm(v[4 + o][word], v[6 + o][word], pick), 0x5410);
+                if (wide && p > 0) d[o] ^= 0x80808080u;
+            }
             sh.frag[((size_t)blk * NT + (col >> 3)) * 32 + (col & 7) * 4 + t] = make_uint2(d[0], d[1]);
             int sum = __dp4a((int)d[0], 0x01010101, __dp4a((int)d[1], 0x01010101, 0));
 #pragma unroll
