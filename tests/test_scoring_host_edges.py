@@ -1,10 +1,12 @@
 """More refusals of the scoring head, decided on the host before anything is launched: outputs that overlap other
-arrays of the call, addresses that do not suit their elements, buffers that have been freed, sizes past 32 bits."""
+arrays of the call, addresses that do not suit their elements, buffers that have been freed, sizes past 32 bits,
+arrays of another kind of number."""
 
 import numpy as np
 import pytest
 
 import vectoraccelerate_b200 as va
+from vectoraccelerate_b200 import scoring
 
 from test_scoring_host import BF16, CTX, F32, INT8, _Context, refused
 
@@ -156,3 +158,18 @@ def test_sizes_past_32_bits_are_refused():
     for name, call in calls:
         with pytest.raises(va.InvalidInput, match=f"{name} must be in"):
             call()
+
+
+def test_arrays_of_another_kind_of_number_are_refused():
+    # (they were cut to the type that the call takes)
+    db = va.Int4Database.__new__(va.Int4Database)
+    db.context, db.n, db.dim, db.table = _Context(), 10, 8, None
+    for q in (np.full((2, 8), 0.7, np.float32), np.full((2, 8), 200), np.full((2, 8), 255, np.uint8), np.full((2, 8), -129)):
+        with pytest.raises(va.InvalidInput, match="queries with query_scales"):
+            db.search(q, 3, query_scales=np.ones(2, np.float32))
+    xent = va.SoftmaxCrossEntropyKernel(_Context())
+    for y in (np.array([1.5, 2.0]), np.array([1 << 63, 0], np.uint64), np.array(["1", "2"])):
+        with pytest.raises(va.InvalidInput, match="labels"):
+            xent.compute(np.zeros((2, 8), np.float32), np.zeros((3, 8), np.float32), y)
+    assert scoring._whole([1, -128, 127], np.int8, "q").tolist() == [1, -128, 127]
+    assert scoring._whole([], np.int64, "labels").shape == (0,)

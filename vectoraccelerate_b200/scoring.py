@@ -132,6 +132,14 @@ def _to_bf16(a) -> np.ndarray:
     return np.where(nan, ((u >> np.uint32(16)) | np.uint32(0x40)).astype(np.uint16), r)
 
 
+def _whole(a, dtype, name: str) -> np.ndarray:
+    """Host array of whole numbers as ``dtype``, which has to hold them."""
+    a = np.asarray(a)
+    if a.size and (a.dtype.kind not in "iu" or int(a.min()) < np.iinfo(dtype).min or int(a.max()) > np.iinfo(dtype).max):
+        raise InvalidInput(f"{name} must be whole numbers that {np.dtype(dtype)} holds, got {a.dtype}")
+    return np.ascontiguousarray(a, dtype)
+
+
 def _from_bf16(b) -> np.ndarray:
     return (np.ascontiguousarray(b, np.uint16).astype(np.uint32) << np.uint32(16)).view(np.float32)
 
@@ -316,7 +324,7 @@ class Int4Database:
         """-> (values [Q, k], ids [Q, k]). Queries are fp32, or int8 codes with a scale per query (the output of
         RMSNormInt8Kernel)."""
         int8 = query_scales is not None
-        q = np.ascontiguousarray(queries, np.int8 if int8 else np.float32)
+        q = _whole(queries, np.int8, "queries with query_scales") if int8 else np.ascontiguousarray(queries, np.float32)
         if q.ndim == 1:
             q = q[None, :]
         if q.shape[1] != self.dim:
@@ -420,7 +428,7 @@ class SoftmaxCrossEntropyKernel(_ScoringKernel):
         """Host arrays (hidden and table are rounded to bf16) -> (loss [T], lse [T], grad_hidden [T, D],
         grad_table [V, D]), fp32."""
         h, w = _to_bf16(_f32(hidden)), _to_bf16(_f32(table))
-        y = np.ascontiguousarray(labels, np.int64).ravel()
+        y = _whole(labels, np.int64, "labels").ravel()
         if h.shape[1] != w.shape[1]:
             raise InvalidInput("Dimension mismatch in input vectors")
         if y.shape != (h.shape[0],):
