@@ -20,7 +20,8 @@
 // (3 bytes an element) the instructions show: 65536 x 4096 bf16 244 us, 3.3 TB/s.
 // Rows that do not start on 16-byte boundaries are copied as the 16-byte pieces that hold them and cut out by shifts;
 // results go through shared memory to whole 16-byte (codes: 8-byte) stores, one row later for the codes: 32768 x 4091 fp32
-// within 2% of the aligned time, 16384 x 4095 bf16 with residual 140 us (element by element 281, aligned 78).
+// within 2% of the aligned time, 16384 x 4095 bf16 with residual 140 us (element by element 281, aligned 78). Narrow rows lose by
+// it: 400000 x 67 bf16 took 166 us element by element and takes 175 to 184.
 #include <algorithm>
 
 #include "va_internal.cuh"
@@ -295,8 +296,8 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
 
 // A block works on one row at a time with TPR threads of NV vectors (8 elements) each. (Narrow rows do not share a
 // block: with rows, addresses and barriers of a warp's own, 200000 x 128 bf16 took 72 us instead of 68.) Two vectors
-// share the reductions' cost (bf16, 65536 x 4096: 316 us, with one 390 us); two of fp32 overflow the registers
-// (10007 x 1000: 31 us, with one 25 us).
+// share the reductions' cost (bf16, 65536 x 4096: 316 us, with one 390 us; fp32, at 128 registers, 32768 x 4096: 395 us, with
+// one at 80 475 us).
 template <typename T, bool ALIGNED, int TPR, int NV>
 struct Plan {
     static constexpr int HALVES = sizeof(T) / 2;  // 16-byte pieces of a vector

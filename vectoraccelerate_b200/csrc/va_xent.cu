@@ -18,7 +18,9 @@
 // chunk's rows) add into an fp32 buffer per K split, which k_xent_finish sums and rounds. Where few rows meet many
 // tokens dw is split the same way (8192 x 1000 x 64: backward 60 us in one go, 30 split).
 // Both directions are compute-bound once T and V pass a few hundred: the tensor pipe and its operand feed are the
-// limit, and the exponentials (16 per clock and SM) hide behind it above D = 256.
+// limit. Below D = 256 neither it nor the exponentials (16 per clock and SM) are: 5982 x 6479 x 120 takes 31 us forward, 9 us of
+// exponentials and a tensor pipe in use for 18%; the epilogue's instructions and the hand-over of an accumulator every
+// two K blocks take the time.
 //
 // Tiles: a CTA's 128 x 256 tile takes 48 KB of operands per 64 of K, more than shared memory and L2 feed at the
 // full rate; a pair of CTAs (cta_group::2) works on 256 x 256 and loads 32 KB each. Measured per chunk of 8192 x
@@ -27,11 +29,11 @@
 // are 128 wide (333 x 5003 x 512: 7.8 us instead of 12.4).
 //
 // Measured (B200, 8192 x 131072 x 1536): forward 2.4 ms, 1380 TFLOP/s; forward and backward 10.6 ms under the power cap,
-// 8TVD at 1240 TFLOP/s, where cuBLAS runs the same three products at 1330; 45 us of it are the three small kernels.
+// 8TVD at 1240 TFLOP/s, where cuBLAS runs the same three products at 1330; 45 us of it are the four small kernels.
 //
 // Roundings: G is kept as P - [label] in bf16, without c g_t: a label's entry is then -1 to within its p, where
 // c g_t itself would round alike for every token of a mean and bias the gradients by up to 2^-8 (measured: 0.33%
-// instead of 0.20% off at 8192 x 131072 x 1536). dh's rows take c g_t when they are finished, in fp32. dw needs it
+// instead of 0.17% off at 8192 x 131072 x 1536). dh's rows take c g_t when they are finished, in fp32. dw needs it
 // inside the sum: h's rows enter as bf16(h c g_t / rho) and dw is multiplied by rho, the largest |c g| of the batch, so that
 // equal weights leave h as it is. Everything else is fp32. All orders of summation are fixed.
 #include <algorithm>
