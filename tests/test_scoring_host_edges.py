@@ -173,3 +173,15 @@ def test_arrays_of_another_kind_of_number_are_refused():
             xent.compute(np.zeros((2, 8), np.float32), np.zeros((3, 8), np.float32), y)
     assert scoring._whole([1, -128, 127], np.int8, "q").tolist() == [1, -128, 127]
     assert scoring._whole([], np.int64, "labels").shape == (0,)
+
+
+def test_an_empty_workspace_is_not_the_contexts(monkeypatch):
+    torch = pytest.importorskip("torch")
+    xent = va.SoftmaxCrossEntropyKernel(_Context())
+    monkeypatch.setattr(scoring, "_device_of", lambda *a: None)  # (a CPU tensor stands for one of the GPU)
+    monkeypatch.setattr(xent, "workspace_bytes", lambda *a: 1000)
+    for nothing in (torch.empty(0, dtype=torch.uint8), 0):
+        with pytest.raises(va.InvalidInput, match="workspace of 0 bytes"):
+            xent.encode_forward(P(1), P(2), P(3), 5, 100, 64, P(4), P(5), workspace=nothing)
+        with pytest.raises(va.InvalidInput, match="workspace of 0 bytes"):
+            xent.encode_backward(P(1), P(2), P(3), P(4), None, 5, 100, 64, P(6), P(7), workspace=nothing)

@@ -382,13 +382,17 @@ class SoftmaxCrossEntropyKernel(_ScoringKernel):
         if workspace is None:
             return None, 0
         if isinstance(workspace, int):
-            return workspace, self.workspace_bytes(tokens, rows, dimension, backward)
-        if not hasattr(workspace, "data_ptr"):
-            return _buffer(self._device, workspace, 0, "workspace"), workspace.nbytes
-        _device_of(self._device, workspace, "workspace")
-        if not workspace.is_contiguous():
-            raise InvalidInput("workspace must be contiguous")
-        return workspace.data_ptr(), workspace.nbytes
+            at, nbytes = workspace, self.workspace_bytes(tokens, rows, dimension, backward)
+        elif not hasattr(workspace, "data_ptr"):
+            at, nbytes = _buffer(self._device, workspace, 0, "workspace"), workspace.nbytes
+        else:
+            _device_of(self._device, workspace, "workspace")
+            if not workspace.is_contiguous():
+                raise InvalidInput("workspace must be contiguous")
+            at, nbytes = workspace.data_ptr(), workspace.nbytes
+        if not at and tokens > 0:  # (address 0 would stand for the context's scratch)
+            raise InvalidInput("workspace of 0 bytes is too small")
+        return at, nbytes
 
     def encode_forward(self, hidden, table, labels, tokens: int, rows: int, dimension: int, loss, lse,
                        logit_scale: float = 1.0, hidden_stride: int | None = None, table_stride: int | None = None,
